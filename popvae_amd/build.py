@@ -1,7 +1,8 @@
 """In-tree build of the native libraries (no cmake, no JIT cache):
 
 * ``libpvae_prep.so``  g++   host-only genotype front end (csrc/pvae_prep.cpp)
-* ``libpvae.so``       hipcc --offload-arch=gfx950   HIP kernels + engine + C ABI (csrc/pvae_engine.hip)
+* ``libpvae.so``       hipcc --offload-arch=gfx950   HIP kernels + engine + C ABI (csrc/pvae_engine.hip) and the
+                       operators on device tensors (csrc/pvae_ops.hip)
 
 Both land next to this file so that they travel to the GPU box with the source snapshot.
 """
@@ -11,6 +12,7 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -40,12 +42,23 @@ def build_prep(force=False):
 def build_engine(force=False, extra=()):
     out = os.path.join(HERE, "libpvae.so")
     srcs = [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC)) if f.endswith((".hip", ".h", ".hpp"))]
-    srcs.append(os.path.join(INC, "pvae.h"))
-    main = os.path.join(CSRC, "pvae_engine.hip")
+    srcs += [os.path.join(INC, "pvae.h"), os.path.join(INC, "pvae_ops.h")]
     if force or _newer(out, srcs):
         hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
-        _run([hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-shared", "-fPIC",
-              "-Wall", "-Wno-unused-function", "-Wno-unused-value", *extra, "-o", out, main])
+        flags = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function", "-Wno-unused-value", *extra]
+        with tempfile.TemporaryDirectory() as tmp:
+            objs, running = [], []
+            # no packed float32 instructions: some of their forms have given wrong results on this part (the host pass of hipcc
+            # does not know the feature and says so)
+            for name, more in (("pvae_engine", []), ("pvae_ops", ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"])):
+                objs.append(os.path.join(tmp, name + ".o"))
+                cmd = [hipcc, *flags, *more, "-c", "-o", objs[-1], os.path.join(CSRC, name + ".hip")]
+                print("+", " ".join(cmd), flush=True)
+                running.append((cmd, subprocess.Popen(cmd)))
+            for cmd, p in running:
+                if p.wait():
+                    raise subprocess.CalledProcessError(p.returncode, cmd)
+            _run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", out, *objs])
     return out
 
 

@@ -1,0 +1,455 @@
+// pvae_ops.hip -- the operators of include/pvae_ops.h: argument checks, choice of kernel, launches.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdarg>
+#include <cstdio>
+#include <new>
+#include <string>
+#include <utility>
+#include <vector>
+
+#include "../../include/pvae_ops.h"
+#include "pvae_dense.h"
+#include "pvae_multi.h"
+
+namespace {
+
+thread_local char g_err[512];
+
+int refuse(int code, const char* fmt, ...) {
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(g_err, sizeof g_err, fmt, ap);
+    va_end(ap);
+    return code;
+}
+int launched(const char* what) {
+    const hipError_t s = hipGetLastError();
+    return s == hipSuccess ? 0 : refuse(-11, "launch of %s failed: %s", what, hipGetErrorString(s));
+}
+
+int esize(int dt) { return dt == PVAE_F32 ? 4 : 2; }
+bool aligned(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % (uintptr_t)bytes == 0; }
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// [rows][cols] with a row stride: the strides the kernels' 64-bit offsets hold
+int check_matrix(const char* name, const void* p, int64_t rows, int64_t cols, int64_t ld, int size) {
+    if (rows == 0 || cols == 0) return 0;
+    if (!p) return refuse(-1, "%s is NULL", name);
+    if (!aligned(p, size)) return refuse(-2, "%s is not aligned to its %d-byte elements", name, size);
+    if (ld < cols && rows > 1) return refuse(-2, "%s: row stride %lld below the row's %lld elements", name, (long long)ld, (long long)cols);
+    if (rows > 1 && ld > (int64_t(1) << 60) / rows / size) return refuse(-2, "%s: row stride %lld too large", name, (long long)ld);
+    return 0;
+}
+int check_sizes(int32_t dtype, int32_t act, int64_t m, int64_t k, int64_t n) {
+    if (dtype < PVAE_F32 || dtype > PVAE_F16) return refuse(-2, "unknown type %d", dtype);
+    if (act < PVAE_LINEAR || act > PVAE_GELU) return refuse(-2, "unknown activation %d", act);
+    const int64_t top = int64_t(1) << 31;
+    if (m < 0 || k < 0 || n < 0 || m >= top || k >= top || n >= top)
+        return refuse(-2, "sizes m = %lld, k = %lld, n = %lld: 0 .. 2^31 - 1 each", (long long)m, (long long)k, (long long)n);
+    return 0;
+}
+int check_weights(const void* w, int64_t k, int64_t n, int64_t sk, int64_t sn, int size) {
+    if (k == 0 || n == 0) return 0;
+    if (sn == 1 || n == 1) return check_matrix("w", w, k, n, std::max(sk, n == 1 ? int64_t(1) : sk), size);
+    if (sk == 1 || k == 1) return check_matrix("w^T", w, n, k, sn, size);
+    return refuse(-2, "w: neither rows nor columns are contiguous (strides %lld, %lld)", (long long)sk, (long long)sn);
+}
+
+// an operand of the tile kernel: rows x K, and whether sixteen bytes along its unit stride can be read at once
+PvdOperand operand(const void* p, int64_t rows, int64_t cols_k, int64_t sr, int64_t sk, int size) {
+    PvdOperand o{};
+    o.p = p;
+    o.rows = rows;
+    if (sk != 1 && sr != 1) (cols_k == 1 ? sk : sr) = 1;  // a single row or column: its stride is never used
+    o.sr = sr;
+    o.sk = sk;
+    const int64_t other = sk == 1 ? sr : sk;
+    const bool one = sk == 1 ? rows <= 1 : cols_k <= 1;
+    o.vec = aligned(p, 16) && (one || other * size % 16 == 0);
+    return o;
+}
+void with_grad(PvdOperand& o, const float* pre, int64_t pr, int64_t pk, int act) {
+    o.pre = pre;
+    o.pr = pr;
+    o.pk = pk;
+    o.act = act;
+    if (act != PVD_LINEAR) o.vec = o.vec && aligned(pre, 16) && (pk == 1 ? pr : pk) % 4 == 0;
+}
+PvdOut output(int64_t rows, int64_t cols, void* y, int64_t ldy, const void* bias, const void* res, int64_t ldr, float* pre, int64_t ldp,
+              int act, int size) {
+    PvdOut o{rows, cols, y, ldy, bias, res, ldr, pre, ldp, act, 0};
+    auto fits = [&](const void* p, int64_t ld, int s) { return !p || (aligned(p, 4 * s) && (rows <= 1 || ld % 4 == 0)); };
+    o.vec = fits(y, ldy, size) && fits(bias, 0, size) && fits(res, ldr, size) && fits(pre, ldp, 4);
+    return o;
+}
+
+// pieces of the contraction: enough workgroups for the chip when the result has few tiles, each with at least 512 bytes of
+// every row
+void split_tile_job(PvdTileJob& J, int size, int64_t wanted) {
+    const int64_t step = 128 / size, tiles = (int64_t)J.mt * J.nt, most = std::max<int64_t>(1, J.K / (4 * step));
+    const int64_t pieces = tiles ? std::min(most, std::max<int64_t>(1, wanted / tiles)) : 1;
+    J.kper = std::max<int64_t>(step, ceil_div(ceil_div(J.K, pieces), step) * step);
+    J.splits = (int)std::max<int64_t>(1, ceil_div(J.K, J.kper));
+}
+PvdTileJob tile_job(const PvdOperand& X, const PvdOperand& W, const PvdOut& O, int64_t K, int size) {
+    PvdTileJob J{X, W, O, K, (int)ceil_div(O.rows, PVD_T), (int)ceil_div(O.cols, PVD_T), 1, 0, nullptr};
+    split_tile_job(J, size, 512);
+    return J;
+}
+int64_t tile_job_bytes(const PvdTileJob& J) { return J.splits > 1 ? (int64_t)J.splits * J.O.rows * J.O.cols * 4 : 0; }
+
+#define PVD_BY_TYPE(dt, CALL)                                          \
+    switch (dt) {                                                      \
+        case PVAE_F32: { constexpr int D_ = PVD_F32; CALL; } break;    \
+        case PVAE_BF16: { constexpr int D_ = PVD_BF16; CALL; } break;  \
+        default: { constexpr int D_ = PVD_F16; CALL; } break;          \
+    }
+
+int launch_join(int dt, const PvdTileJob& J, hipStream_t s) {
+    const int64_t quads = J.O.rows * ceil_div(J.O.cols, 4);
+    PVD_BY_TYPE(dt, hipLaunchKernelGGL(pvk_dense_join<D_>, dim3((unsigned)ceil_div(quads, 256)), dim3(256), 0, s, J.O, (const float*)J.part, J.splits));
+    return launched("dense_join");
+}
+
+PvdTileJob dense_job(const pvae_dense_args& a) {
+    const int size = esize(a.dtype);
+    return tile_job(operand(a.x, a.m, a.k, a.ldx, 1, size), operand(a.w, a.n, a.k, a.w_sn, a.w_sk, size),
+                    output(a.m, a.n, a.y, a.ldy, a.bias, a.residual, a.ldr, a.pre, a.ldp, a.act, size), a.k, size);
+}
+int check_dense(const pvae_dense_args* a) {
+    if (!a) return refuse(-1, "no arguments");
+    if (int rc = check_sizes(a->dtype, a->act, a->m, a->k, a->n)) return rc;
+    const int size = esize(a->dtype);
+    if (int rc = check_matrix("x", a->x, a->m, a->k, a->ldx, size)) return rc;
+    if (int rc = check_weights(a->w, a->k, a->n, a->w_sk, a->w_sn, size)) return rc;
+    if (int rc = check_matrix("y", a->y, a->m, a->n, a->ldy, size)) return rc;
+    if (a->bias)
+        if (int rc = check_matrix("bias", a->bias, 1, a->n, a->n, size)) return rc;
+    if (a->residual)
+        if (int rc = check_matrix("residual", a->residual, a->ldr == 0 ? 1 : a->m, a->n, a->ldr, size)) return rc;
+    if (a->pre)
+        if (int rc = check_matrix("pre", a->pre, a->m, a->n, a->ldp, 4)) return rc;
+    return 0;
+}
+
+struct BwdPlan {
+    PvdBwdJob J;
+    int64_t n_db;
+};
+BwdPlan bwd_plan(const pvae_dense_bwd_args& a) {
+    const int size = esize(a.dtype);
+    BwdPlan p{};
+    PvdOperand gx = operand(a.dy, a.m, a.n, a.lddy, 1, size), gw = operand(a.dy, a.n, a.m, 1, a.lddy, size);
+    with_grad(gx, a.pre, a.ldp, 1, a.act);
+    with_grad(gw, a.pre, 1, a.ldp, a.act);
+    // w as an operand of dx: rows are the k of the layer, the contraction its n
+    if (a.dx)
+        p.J.dx = tile_job(gx, operand(a.w, a.k, a.n, a.w_sk, a.w_sn, size),
+                          output(a.m, a.k, a.dx, a.lddx, nullptr, a.dx_add, a.ldadd, nullptr, 0, PVD_LINEAR, size), a.n, size);
+    if (a.dw)
+        p.J.dw = tile_job(operand(a.x, a.k, a.m, 1, a.ldx, size), gw,
+                          output(a.k, a.n, a.dw, a.n, nullptr, nullptr, 0, nullptr, 0, PVD_LINEAR, size), a.m, size);
+    p.J.n_dx = a.dx ? (int64_t)p.J.dx.mt * p.J.dx.nt * p.J.dx.splits : 0;
+    p.J.n_dw = a.dw ? (int64_t)p.J.dw.mt * p.J.dw.nt * p.J.dw.splits : 0;
+    p.J.dy = a.dy;
+    p.J.lddy = a.lddy;
+    p.J.pre = a.pre;
+    p.J.ldp = a.ldp;
+    p.J.act = a.act;
+    p.J.m = a.m;
+    p.J.n = a.n;
+    p.J.dbias = a.dbias;
+    p.J.dpre = a.dpre;
+    p.n_db = a.dbias || a.dpre ? ceil_div(a.n, 64) : 0;
+    return p;
+}
+int64_t bwd_bytes(const BwdPlan& p) { return (p.J.n_dx ? tile_job_bytes(p.J.dx) : 0) + (p.J.n_dw ? tile_job_bytes(p.J.dw) : 0); }
+int check_dense_bwd(const pvae_dense_bwd_args* a) {
+    if (!a) return refuse(-1, "no arguments");
+    if (int rc = check_sizes(a->dtype, a->act, a->m, a->k, a->n)) return rc;
+    const int size = esize(a->dtype);
+    if (int rc = check_matrix("dy", a->dy, a->m, a->n, a->lddy, size)) return rc;
+    if (a->act != PVAE_LINEAR)
+        if (int rc = check_matrix("pre", a->pre, a->m, a->n, a->ldp, 4)) return rc;
+    if (a->dw)
+        if (int rc = check_matrix("x", a->x, a->m, a->k, a->ldx, size)) return rc;
+    if (a->dx) {
+        if (int rc = check_weights(a->w, a->k, a->n, a->w_sk, a->w_sn, size)) return rc;
+        if (int rc = check_matrix("dx", a->dx, a->m, a->k, a->lddx, size)) return rc;
+        if (a->dx_add)
+            if (int rc = check_matrix("dx_add", a->dx_add, a->ldadd == 0 ? 1 : a->m, a->k, a->ldadd, size)) return rc;
+    }
+    if (a->dw && !aligned(a->dw, size)) return refuse(-2, "dw is not aligned to its elements");
+    if (a->dbias && !aligned(a->dbias, size)) return refuse(-2, "dbias is not aligned to its elements");
+    if (a->dpre && !aligned(a->dpre, 4)) return refuse(-2, "dpre is not aligned to its elements");
+    return 0;
+}
+int check_workspace(const char* what, const void* p, int64_t have, int64_t need) {
+    if (need == 0) return 0;
+    if (!p || have < need) return refuse(-8, "%s needs a workspace of %lld bytes (got %lld)", what, (long long)need, (long long)(p ? have : 0));
+    if (!aligned(p, 16)) return refuse(-2, "the workspace is not aligned to 16 bytes");
+    return 0;
+}
+int check_grid(int64_t blocks) {
+    if (blocks > 0x7fffffff) return refuse(-2, "%lld workgroups: the operands are too large for one launch", (long long)blocks);
+    return 0;
+}
+
+// ---- many tensors ----
+int check_tensors(const char* name, const pvae_tensor* t, int64_t count, bool tiles) {
+    if (count < 0 || count > 65536) return refuse(-2, "%lld tensors: 0 .. 65536", (long long)count);
+    if (count && !t) return refuse(-1, "%s is NULL", name);
+    for (int64_t i = 0; i < count; ++i) {
+        if (t[i].dtype < PVAE_F32 || t[i].dtype > PVAE_F16) return refuse(-2, "%s %lld: unknown type %d", name, (long long)i, t[i].dtype);
+        if (t[i].n < 0 || t[i].n > (int64_t(1) << 40)) return refuse(-2, "%s %lld: %lld elements", name, (long long)i, (long long)t[i].n);
+        if (t[i].n && !t[i].data) return refuse(-1, "%s %lld is NULL", name, (long long)i);
+        if (!aligned(t[i].data, esize(t[i].dtype))) return refuse(-2, "%s %lld is not aligned to its elements", name, (long long)i);
+        if (t[i].tile && (!tiles || t[i].tile < 0 || t[i].tile % 4 || t[i].n % t[i].tile))
+            return refuse(-2, "%s %lld: bad interleave %d", name, (long long)i, t[i].tile);
+    }
+    return 0;
+}
+struct Span { uintptr_t lo, hi; };
+void add_spans(std::vector<Span>& v, const pvae_tensor* t, int64_t count) {
+    for (int64_t i = 0; i < count; ++i)
+        if (t[i].n) {
+            const uintptr_t lo = reinterpret_cast<uintptr_t>(t[i].data);
+            v.push_back({lo, lo + (uintptr_t)t[i].n * esize(t[i].dtype)});
+        }
+}
+bool overlap(std::vector<Span>& v) {
+    std::sort(v.begin(), v.end(), [](const Span& a, const Span& b) { return a.lo < b.lo; });
+    for (size_t i = 1; i < v.size(); ++i)
+        if (v[i].lo < v[i - 1].hi) return true;
+    return false;
+}
+// whether t reads what one of the spans (sorted, disjoint) writes
+bool reads_from(const std::vector<Span>& v, const pvae_tensor& t) {
+    if (t.n == 0) return false;
+    const uintptr_t lo = reinterpret_cast<uintptr_t>(t.data), hi = lo + (uintptr_t)t.n * esize(t.dtype);
+    const auto it = std::lower_bound(v.begin(), v.end(), hi, [](const Span& s, uintptr_t h) { return s.lo < h; });
+    return it != v.begin() && std::prev(it)->hi > lo;
+}
+
+// the tensors in tables of PVM_MAXT, empty ones left out: f(table) per launch; `fill` sets a table's other pointers
+template <typename Fill, typename Launch> int for_tables(const pvae_tensor* g, int64_t count, Fill fill, Launch launch) {
+    PvmTab T;
+    T.count = 0;
+    T.first[0] = 0;
+    for (int64_t i = 0; i <= count; ++i) {
+        const int64_t chunks = i < count ? ceil_div(g[i].n, PVM_CHUNK) : 0;
+        if (T.count && (i == count || T.count == PVM_MAXT || T.first[T.count] + chunks > 0x7fffffff)) {
+            if (int rc = launch(T)) return rc;
+            T.count = 0;
+        }
+        if (i == count || chunks == 0) continue;
+        const int c = T.count;
+        T.a[c] = g[i].data;
+        T.n[c] = g[i].n;
+        T.dt[c] = (unsigned char)g[i].dtype;
+        T.vec[c] = aligned(g[i].data, 4 * esize(g[i].dtype));
+        T.b[c] = nullptr;
+        T.m[c] = T.v[c] = nullptr;
+        T.tile[c] = 0;
+        fill(T, c, i);
+        T.first[c + 1] = T.first[c] + (int)chunks;
+        T.count = c + 1;
+    }
+    return 0;
+}
+int tables_of(const pvae_tensor* g, int64_t count) {
+    int n = 0;
+    for_tables(g, count, [](PvmTab&, int, int64_t) {}, [&](PvmTab&) { ++n; return 0; });
+    return n;
+}
+// the partial sums of g^2: at most PVM_PARTS over all launches
+int launch_sumsq(const pvae_tensor* g, int64_t count, double* part, int* nparts, hipStream_t s) {
+    const int tables = tables_of(g, count), each = tables ? std::max(1, std::min(1024, PVM_PARTS / tables)) : 0;
+    *nparts = 0;
+    return for_tables(g, count, [](PvmTab&, int, int64_t) {}, [&](PvmTab& T) {
+        const int blocks = std::min(each, T.first[T.count]);
+        hipLaunchKernelGGL(pvk_sumsq, dim3(blocks), dim3(PVM_THREADS), 0, s, T, part + *nparts);
+        *nparts += blocks;
+        return launched("sumsq");
+    });
+}
+int launch_norm(const pvae_tensor* g, int64_t count, float* norm, void* ws, int* nparts, hipStream_t s) {
+    double* part = static_cast<double*>(ws);
+    if (int rc = launch_sumsq(g, count, part, nparts, s)) return rc;
+    if (!norm) return 0;
+    hipLaunchKernelGGL(pvk_norm_final, dim3(1), dim3(PVM_THREADS), 0, s, (const double*)part, *nparts, norm);
+    return launched("norm_final");
+}
+
+template <typename F> int guarded(F f) {  // no C++ exception leaves a C entry
+    try {
+        return f();
+    } catch (const std::bad_alloc&) {
+        return refuse(-9, "out of host memory");
+    } catch (...) {
+        return refuse(-9, "unexpected error");
+    }
+}
+
+}  // namespace
+
+extern "C" {
+
+const char* pvae_ops_last_error(void) { return g_err; }
+
+int64_t pvae_dense_workspace(const pvae_dense_args* a) {
+    if (check_dense(a) || a->m == 0 || a->n == 0) return 0;
+    return tile_job_bytes(dense_job(*a));
+}
+
+int pvae_dense(const pvae_dense_args* a, void* workspace, int64_t workspace_bytes, void* hip_stream) {
+    if (int rc = check_dense(a)) return rc;
+    if (a->m == 0 || a->n == 0) return 0;
+    hipStream_t s = static_cast<hipStream_t>(hip_stream);
+    PvdTileJob J = dense_job(*a);
+    if (int rc = check_workspace("pvae_dense", workspace, workspace_bytes, tile_job_bytes(J))) return rc;
+    const int64_t blocks = (int64_t)J.mt * J.nt * J.splits;
+    if (int rc = check_grid(blocks)) return rc;
+    J.part = static_cast<float*>(workspace);
+    PVD_BY_TYPE(a->dtype, hipLaunchKernelGGL(pvk_dense_tile<D_>, dim3((unsigned)blocks), dim3(256), 0, s, J));
+    if (int rc = launched("dense_tile")) return rc;
+    return J.splits > 1 ? launch_join(a->dtype, J, s) : 0;
+}
+
+int64_t pvae_dense_bwd_workspace(const pvae_dense_bwd_args* a) {
+    if (check_dense_bwd(a)) return 0;
+    return bwd_bytes(bwd_plan(*a));
+}
+
+int pvae_dense_bwd(const pvae_dense_bwd_args* a, void* workspace, int64_t workspace_bytes, void* hip_stream) {
+    if (int rc = check_dense_bwd(a)) return rc;
+    hipStream_t s = static_cast<hipStream_t>(hip_stream);
+    BwdPlan p = bwd_plan(*a);
+    if (int rc = check_workspace("pvae_dense_bwd", workspace, workspace_bytes, bwd_bytes(p))) return rc;
+    const int64_t blocks = p.J.n_dx + p.J.n_dw + p.n_db;
+    if (int rc = check_grid(blocks)) return rc;
+    if (blocks == 0) return 0;
+    p.J.dx.part = static_cast<float*>(workspace);
+    p.J.dw.part = static_cast<float*>(workspace) + (p.J.n_dx ? tile_job_bytes(p.J.dx) / 4 : 0);
+    PVD_BY_TYPE(a->dtype, hipLaunchKernelGGL(pvk_dense_bwd_tile<D_>, dim3((unsigned)blocks), dim3(256), 0, s, p.J));
+    if (int rc = launched("dense_bwd_tile")) return rc;
+    if (p.J.n_dx && p.J.dx.splits > 1)
+        if (int rc = launch_join(a->dtype, p.J.dx, s)) return rc;
+    if (p.J.n_dw && p.J.dw.splits > 1)
+        if (int rc = launch_join(a->dtype, p.J.dw, s)) return rc;
+    return 0;
+}
+
+int64_t pvae_norm_workspace(void) { return PVM_PARTS * (int64_t)sizeof(double); }
+
+int pvae_global_norm(const pvae_tensor* g, int64_t count, float* norm, void* workspace, int64_t workspace_bytes, void* hip_stream) {
+    if (int rc = check_tensors("g", g, count, false)) return rc;
+    if (!norm) return refuse(-1, "norm is NULL");
+    if (int rc = check_workspace("pvae_global_norm", workspace, workspace_bytes, pvae_norm_workspace())) return rc;
+    int nparts;
+    return launch_norm(g, count, norm, workspace, &nparts, static_cast<hipStream_t>(hip_stream));
+}
+
+int pvae_clip_by_global_norm(const pvae_tensor* g, const pvae_tensor* out, int64_t count, double max_norm, float* norm, void* workspace,
+                             int64_t workspace_bytes, void* hip_stream) {
+    return guarded([&]() -> int {
+        if (int rc = check_tensors("g", g, count, false)) return rc;
+        if (int rc = check_tensors("out", out, count, false)) return rc;
+        if (!(max_norm > 0.0)) return refuse(-2, "max_norm %g: a positive number", max_norm);
+        bool in_place = true;
+        for (int64_t i = 0; i < count; ++i) {
+            if (out[i].n != g[i].n || out[i].dtype != g[i].dtype)
+                return refuse(-2, "tensor %lld: out differs from g in size or type", (long long)i);
+            in_place = in_place && (out[i].data == g[i].data || g[i].n == 0);
+        }
+        std::vector<Span> spans;
+        spans.reserve(2 * (size_t)count);
+        add_spans(spans, out, count);
+        if (overlap(spans)) return refuse(-2, "two of out's tensors overlap");
+        // a gradient may appear twice in g, but none may lie where another one's copy is written
+        for (int64_t i = 0; i < count && !in_place; ++i)
+            if (out[i].data != g[i].data && reads_from(spans, g[i])) return refuse(-2, "tensor %lld of g overlaps an output", (long long)i);
+        if (int rc = check_workspace("pvae_clip_by_global_norm", workspace, workspace_bytes, pvae_norm_workspace())) return rc;
+        hipStream_t s = static_cast<hipStream_t>(hip_stream);
+        double* part = static_cast<double*>(workspace);
+        int nparts;
+        if (int rc = launch_sumsq(g, count, part, &nparts, s)) return rc;
+        if (nparts == 0) return norm ? launch_norm(g, 0, norm, workspace, &nparts, s) : 0;
+        return for_tables(
+            g, count,
+            [&](PvmTab& T, int c, int64_t i) {
+                T.b[c] = out[i].data;
+                T.vec[c] = T.vec[c] && aligned(out[i].data, 4 * esize(out[i].dtype));
+            },
+            [&](PvmTab& T) {
+                hipLaunchKernelGGL(pvk_clip_apply, dim3(std::min(2048, T.first[T.count])), dim3(PVM_THREADS), 0, s, T, (const double*)part,
+                                   nparts, max_norm, norm);
+                return launched("clip_apply");
+            });
+    });
+}
+
+int pvae_adam_step(const pvae_tensor* p, const pvae_tensor* g, const pvae_tensor* m, const pvae_tensor* v, int64_t count, double lr,
+                   double beta1, double beta2, double eps, int64_t step, const int32_t* step_dev, double clip_norm, float* norm,
+                   void* workspace, int64_t workspace_bytes, void* hip_stream) {
+    return guarded([&]() -> int {
+        if (int rc = check_tensors("p", p, count, true)) return rc;
+        if (int rc = check_tensors("g", g, count, false)) return rc;
+        if (int rc = check_tensors("m", m, count, true)) return rc;
+        if (int rc = check_tensors("v", v, count, true)) return rc;
+        if (!std::isfinite(lr) || !(beta1 >= 0 && beta1 < 1) || !(beta2 >= 0 && beta2 < 1) || !(eps > 0) || !std::isfinite(eps))
+            return refuse(-2, "lr %g, beta1 %g, beta2 %g, eps %g: finite, 0 <= beta < 1, eps > 0", lr, beta1, beta2, eps);
+        if (!step_dev && step < 1) return refuse(-2, "step %lld: counted from 1", (long long)step);
+        if (!(clip_norm >= 0)) return refuse(-2, "clip_norm %g: a positive number, or 0 for none", clip_norm);
+        std::vector<Span> spans;
+        spans.reserve(4 * (size_t)count);
+        for (int64_t i = 0; i < count; ++i) {
+            if (p[i].dtype != PVAE_F32 || m[i].dtype != PVAE_F32 || v[i].dtype != PVAE_F32)
+                return refuse(-2, "tensor %lld: p, m and v are float32", (long long)i);
+            if (p[i].n != g[i].n || m[i].n != g[i].n || v[i].n != g[i].n || m[i].tile != p[i].tile || v[i].tile != p[i].tile)
+                return refuse(-2, "tensor %lld: p, g, m and v differ in size", (long long)i);
+            if (p[i].tile && (static_cast<float*>(m[i].data) != static_cast<float*>(p[i].data) + p[i].tile ||
+                              static_cast<float*>(v[i].data) != static_cast<float*>(p[i].data) + 2 * p[i].tile))
+                return refuse(-2, "tensor %lld: p, m and v are not interleaved by %d elements", (long long)i, p[i].tile);
+            if (p[i].tile && p[i].n) {
+                const uintptr_t lo = reinterpret_cast<uintptr_t>(p[i].data);
+                spans.push_back({lo, lo + (uintptr_t)p[i].n * 12});
+            } else {
+                add_spans(spans, p + i, 1);
+                add_spans(spans, m + i, 1);
+                add_spans(spans, v + i, 1);
+            }
+        }
+        if (overlap(spans)) return refuse(-2, "two of the tensors p, m and v overlap");
+        for (int64_t i = 0; i < count; ++i)
+            if (reads_from(spans, g[i])) return refuse(-2, "tensor %lld: g overlaps one of p, m and v", (long long)i);
+        hipStream_t s = static_cast<hipStream_t>(hip_stream);
+        double* part = static_cast<double*>(workspace);
+        int nparts = 0;
+        if (clip_norm > 0 || norm) {
+            if (int rc = check_workspace("pvae_adam_step", workspace, workspace_bytes, pvae_norm_workspace())) return rc;
+            if (int rc = launch_sumsq(g, count, part, &nparts, s)) return rc;
+            if (nparts == 0) return norm ? launch_norm(g, 0, norm, workspace, &nparts, s) : 0;
+        }
+        const PvmAdam A{lr, beta1, beta2, (float)eps, step, step_dev};
+        return for_tables(
+            g, count,
+            [&](PvmTab& T, int c, int64_t i) {
+                T.b[c] = p[i].data;
+                T.m[c] = static_cast<float*>(m[i].data);
+                T.v[c] = static_cast<float*>(v[i].data);
+                T.tile[c] = p[i].tile;
+                T.vec[c] = T.vec[c] && aligned(p[i].data, 16) && aligned(m[i].data, 16) && aligned(v[i].data, 16);
+            },
+            [&](PvmTab& T) {
+                hipLaunchKernelGGL(pvk_adam_apply, dim3(std::min(2048, T.first[T.count])), dim3(PVM_THREADS), 0, s, T, (const double*)part,
+                                   nparts, clip_norm, norm, A);
+                return launched("adam_apply");
+            });
+    });
+}
+
+}  // extern "C"

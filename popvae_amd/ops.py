@@ -1,0 +1,319 @@
+"""Operators on the caller's own GPU tensors (include/pvae_ops.h through ctypes): a dense layer with bias, activation and
+residual in one pass, its gradients, the global gradient norm, clipping by it, and the Adam update with that clipping.
+
+They are what the engine's layers and optimizer do, for tensors that do not live in an ``Engine``: any size, float32, bfloat16
+or float16, other activations.  Everything runs on torch's current stream of the tensors' device, allocates through torch's
+allocator (outputs and scratch memory), never waits for the GPU and may be captured into a graph.  A call that cannot be
+computed raises ValueError before anything is launched.  There is no CPU path.
+
+    y = ops.dense(x, w, b, "elu", residual=x, pre=z)               # z: float32, kept for the backward
+    dx, dw, db = ops.dense_backward(dy, x, w, z, "elu", dx_add=dy)  # dx_add: the layer's residual was its own input
+    grads = ops.TensorSet([...])
+    norm = ops.adam_step(params, grads, m, v, step, clip_norm=1.0)
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import engine
+
+OPS_SYMBOLS = ["pvae_ops_last_error", "pvae_dense_workspace", "pvae_dense", "pvae_dense_bwd_workspace", "pvae_dense_bwd",
+               "pvae_norm_workspace", "pvae_global_norm", "pvae_clip_by_global_norm", "pvae_adam_step"]
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+ACTIVATIONS = {"linear": 0, "relu": 1, "elu": 2, "sigmoid": 3, "tanh": 4, "silu": 5, "gelu": 6}
+
+
+class _Dense(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("act", C.c_int32), ("m", C.c_int64), ("k", C.c_int64), ("n", C.c_int64),
+                ("x", C.c_void_p), ("ldx", C.c_int64), ("w", C.c_void_p), ("w_sk", C.c_int64), ("w_sn", C.c_int64),
+                ("bias", C.c_void_p), ("residual", C.c_void_p), ("ldr", C.c_int64), ("y", C.c_void_p), ("ldy", C.c_int64),
+                ("pre", C.c_void_p), ("ldp", C.c_int64)]
+
+
+class _DenseBwd(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("act", C.c_int32), ("m", C.c_int64), ("k", C.c_int64), ("n", C.c_int64),
+                ("dy", C.c_void_p), ("lddy", C.c_int64), ("x", C.c_void_p), ("ldx", C.c_int64), ("w", C.c_void_p),
+                ("w_sk", C.c_int64), ("w_sn", C.c_int64), ("pre", C.c_void_p), ("ldp", C.c_int64), ("dx", C.c_void_p),
+                ("lddx", C.c_int64), ("dx_add", C.c_void_p), ("ldadd", C.c_int64), ("dw", C.c_void_p), ("dbias", C.c_void_p),
+                ("dpre", C.c_void_p)]
+
+
+class _Tensor(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("n", C.c_int64), ("dtype", C.c_int32), ("tile", C.c_int32)]
+
+
+_lib = None
+
+
+def lib():
+    """libpvae.so with the operators' signatures set."""
+    global _lib
+    if _lib is None:
+        L = engine.lib()
+        vp, i32, i64, f64, tp = C.c_void_p, C.c_int32, C.c_int64, C.c_double, C.POINTER(_Tensor)
+        L.pvae_ops_last_error.restype = C.c_char_p
+        for name, args in (("pvae_dense", _Dense), ("pvae_dense_bwd", _DenseBwd)):
+            work = getattr(L, name + "_workspace")
+            work.restype, work.argtypes = i64, [C.POINTER(args)]
+            getattr(L, name).argtypes = [C.POINTER(args), vp, i64, vp]
+        L.pvae_norm_workspace.restype = i64
+        L.pvae_global_norm.argtypes = [tp, i64, vp, vp, i64, vp]
+        L.pvae_clip_by_global_norm.argtypes = [tp, tp, i64, f64, vp, vp, i64, vp]
+        L.pvae_adam_step.argtypes = [tp, tp, tp, tp, i64, f64, f64, f64, f64, i64, vp, f64, vp, vp, i64, vp]
+        _lib = L
+    return _lib
+
+
+def _check(rc):
+    if rc:
+        text = lib().pvae_ops_last_error().decode()
+        if rc <= -9:
+            raise RuntimeError(f"libpvae ({rc}): {text}")
+        raise ValueError(text)
+
+
+class _On:
+    """The tensors' device made current for a call, where it is not."""
+
+    def __init__(self, device):
+        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *a):
+        if self.guard is not None:
+            self.guard.__exit__(*a)
+
+
+def _matrix(name, t, rows, cols, dtype, device, expand=False):
+    """Row stride of a [rows, cols] tensor whose rows are contiguous."""
+    if t.dtype != dtype or t.device != device:
+        raise ValueError(f"{name}: expected {dtype} on {device}, got {t.dtype} on {t.device}")
+    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
+        raise ValueError(f"{name}: expected shape ({rows}, {cols}), got {tuple(t.shape)}")
+    if cols > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name}: rows are not contiguous (strides {t.stride()})")
+    ld = t.stride(0) if rows > 1 else cols
+    if rows > 1 and ld < cols and not (expand and ld == 0):
+        raise ValueError(f"{name}: rows overlap (strides {t.stride()})")
+    return ld
+
+
+def _vector(name, t, n, dtype, device):
+    if t.dtype != dtype or t.device != device or t.dim() != 1 or t.shape[0] != n:
+        raise ValueError(f"{name}: expected {dtype} of shape ({n},) on {device}, got {t.dtype} of {tuple(t.shape)} on {t.device}")
+    if n > 1 and t.stride(0) != 1:
+        raise ValueError(f"{name} is not contiguous")
+
+
+def _act(name):
+    try:
+        return ACTIVATIONS[name]
+    except KeyError:
+        raise ValueError(f"activation {name!r}: one of {', '.join(ACTIVATIONS)}") from None
+
+
+def _layer(x, w):
+    """Checks x [m, k] and w [k, n]; returns (type code, m, k, n, row stride of x)."""
+    dtype, device = x.dtype, x.device
+    if dtype not in DTYPES:
+        raise ValueError(f"x: {dtype} is not one of float32, bfloat16, float16")
+    if device.type != "cuda":
+        raise ValueError(f"x is on {device}: the operators run on a GPU only")
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[0]:
+        raise ValueError(f"x {tuple(x.shape)} and w {tuple(w.shape)}: expected [m, k] and [k, n]")
+    m, k = x.shape
+    n = w.shape[1]
+    ldx = _matrix("x", x, m, k, dtype, device)
+    if w.dtype != dtype or w.device != device:
+        raise ValueError(f"w: expected {dtype} on {device}, got {w.dtype} on {w.device}")
+    return DTYPES[dtype], m, k, n, ldx
+
+
+def _spans(t):
+    """First and last byte behind a 2-D or 1-D tensor's elements."""
+    if t.numel() == 0:
+        return 0, 0
+    lo = t.data_ptr()
+    return lo, lo + (sum((s - 1) * st for s, st in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def _apart(outs, ins):
+    """Outputs overlap neither one another nor an input (their byte ranges)."""
+    spans = [(n, *_spans(t)) for n, t in outs if t is not None]
+    for i, (name, lo, hi) in enumerate(spans):
+        for other, t in [(o, (a, b)) for o, a, b in spans[:i]] + [(n, _spans(t)) for n, t in ins if t is not None]:
+            if lo < t[1] and t[0] < hi:
+                raise ValueError(f"{name} overlaps {other}")
+
+
+def _workspace(n, device):
+    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def dense(x, w, bias=None, activation="linear", residual=None, pre=None, out=None):
+    """``activation(x @ w + bias) + residual``, one rounding at the end.
+
+    x [m, k] (contiguous rows, any row stride), w [k, n] (a Keras kernel, or a transposed view), bias [n], residual [m, n]
+    (an expanded row is fine), all of one type; sums are float32.  pre: float32 [m, n], receives ``x @ w + bias`` for
+    ``dense_backward``.  out: [m, n] to write to (may be the residual), otherwise a new tensor.  Returns it."""
+    dt, m, k, n, ldx = _layer(x, w)
+    dtype, device, act = x.dtype, x.device, _act(activation)
+    if bias is not None:
+        _vector("bias", bias, n, dtype, device)
+    ldr = 0 if residual is None else _matrix("residual", residual, m, n, dtype, device, expand=True)
+    ldp = 0 if pre is None else _matrix("pre", pre, m, n, torch.float32, device)
+    if out is None:
+        out, ldy = torch.empty((m, n), dtype=dtype, device=device), n
+        if pre is not None:
+            _apart([("pre", pre)], [("x", x), ("w", w), ("bias", bias), ("residual", residual)])
+    else:
+        ldy = _matrix("out", out, m, n, dtype, device)
+        same = residual is not None and out.data_ptr() == residual.data_ptr() and (ldr == ldy or m <= 1)
+        ins = [("x", x), ("w", w), ("bias", bias)]
+        _apart([("out", out)], ins + ([] if same else [("residual", residual)]))
+        _apart([("pre", pre), ("out", out)], ins) if pre is not None else None
+        if pre is not None and not same:
+            _apart([("pre", pre)], [("residual", residual)])
+    a = _Dense(dt, act, m, k, n, x.data_ptr(), ldx, w.data_ptr(), w.stride(0), w.stride(1), _ptr(bias), _ptr(residual), ldr,
+               out.data_ptr(), ldy, _ptr(pre), ldp)
+    L = lib()
+    with _On(device):
+        need = L.pvae_dense_workspace(a)
+        work = _workspace(need, device)
+        _check(L.pvae_dense(a, _ptr(work), need, torch.cuda.current_stream().cuda_stream))
+    return out
+
+
+def dense_backward(dy, x, w, pre=None, activation="linear", dx_add=None, need_dx=True, need_dw=True, need_bias=True):
+    """Gradients of ``dense``: ``(dx, dw, db)``, with None for what is not needed.
+
+    dy [m, n]; x, w and activation as in the forward, pre what it left (not needed for "linear").  dx_add [m, k] is added to
+    dx before its rounding: a layer whose residual is its own input passes dy.  (The gradient of the residual is dy itself;
+    summed over the rows for an expanded one.)  With a 16-bit type, dy * f'(pre) is rounded to it before the two products."""
+    dt, m, k, n, ldx = _layer(x, w)
+    dtype, device, act = x.dtype, x.device, _act(activation)
+    lddy = _matrix("dy", dy, m, n, dtype, device)
+    if pre is None and act:
+        raise ValueError(f"the gradient of {activation!r} needs pre, which dense leaves")
+    ldp = 0 if pre is None else _matrix("pre", pre, m, n, torch.float32, device)
+    ldadd = 0 if dx_add is None else _matrix("dx_add", dx_add, m, k, dtype, device, expand=True)
+    dx = torch.empty((m, k), dtype=dtype, device=device) if need_dx else None
+    dw = torch.empty((k, n), dtype=dtype, device=device) if need_dw else None
+    db = torch.empty(n, dtype=dtype, device=device) if need_bias else None
+    a = _DenseBwd(dt, act, m, k, n, dy.data_ptr(), lddy, x.data_ptr(), ldx, w.data_ptr(), w.stride(0), w.stride(1), _ptr(pre), ldp,
+                  _ptr(dx), k, _ptr(dx_add), ldadd, _ptr(dw), _ptr(db), None)
+    L = lib()
+    with _On(device):
+        need = L.pvae_dense_bwd_workspace(a)
+        work = _workspace(need, device)
+        _check(L.pvae_dense_bwd(a, _ptr(work), need, torch.cuda.current_stream().cuda_stream))
+    return dx, dw, db
+
+
+class TensorSet:
+    """A list of contiguous tensors on one GPU, checked and described once: what the operators over all tensors of a model take
+    (a plain list works too, and is described anew by every call).  The tensors must keep their storage: a set one of
+    whose tensors has moved is refused."""
+
+    def __init__(self, tensors):
+        ts = list(tensors)
+        self.device = ts[0].device if ts else None
+        for i, t in enumerate(ts):
+            if t.dtype not in DTYPES:
+                raise ValueError(f"tensor {i}: {t.dtype} is not one of float32, bfloat16, float16")
+            if t.device.type != "cuda" or t.device != self.device:
+                raise ValueError(f"tensor {i} is on {t.device}: all tensors are on one GPU")
+            if not t.is_contiguous():
+                raise ValueError(f"tensor {i} is not contiguous")
+        self.tensors = ts
+        self._ptrs = [t.data_ptr() for t in ts]
+        self._sizes = [t.numel() for t in ts]
+        self._types = [t.dtype for t in ts]
+        self._table = (_Tensor * len(ts))(*[(p, n, DTYPES[d], 0) for p, n, d in zip(self._ptrs, self._sizes, self._types)])
+
+    def __len__(self):
+        return len(self._sizes)
+
+    def _same(self):
+        if [t.data_ptr() for t in self.tensors] != self._ptrs:
+            raise ValueError("a tensor of the set has another storage than when the set was made")
+        return self._table
+
+
+def _set(t):
+    return t if isinstance(t, TensorSet) else TensorSet(t)
+
+
+def _device_of(s):
+    if s.device is None:
+        raise ValueError("no tensors")
+    return s.device
+
+
+def global_norm(tensors):
+    """``sqrt(sum of squares)`` over all tensors, summed in float64: a 0-d float32 tensor."""
+    s = _set(tensors)
+    device, L = _device_of(s), lib()
+    table, norm = s._same(), torch.empty((), dtype=torch.float32, device=device)
+    with _On(device):
+        need = L.pvae_norm_workspace()
+        work = _workspace(need, device)
+        _check(L.pvae_global_norm(table, len(s), norm.data_ptr(), work.data_ptr(), need, torch.cuda.current_stream().cuda_stream))
+    return norm
+
+
+def clip_by_global_norm(tensors, max_norm, out=None):
+    """Scales all tensors by ``min(1, max_norm / norm)`` into ``out`` (tensors of the same sizes and types; default: in place)
+    and returns the norm before clipping, a 0-d float32 tensor.  A norm that is not finite makes every output NaN."""
+    s = _set(tensors)
+    o = s if out is None else _set(out)
+    device, L = _device_of(s), lib()
+    if len(o) != len(s) or o.device != device:
+        raise ValueError("out: as many tensors as there are gradients, on their GPU")
+    table, norm = s._same(), torch.empty((), dtype=torch.float32, device=device)
+    with _On(device):
+        need = L.pvae_norm_workspace()
+        work = _workspace(need, device)
+        _check(L.pvae_clip_by_global_norm(table, o._same(), len(s), float(max_norm), norm.data_ptr(), work.data_ptr(), need,
+                                          torch.cuda.current_stream().cuda_stream))
+    return norm
+
+
+def adam_step(params, grads, m, v, step, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-7, clip_norm=None):
+    """One update of the engine's Adam (Keras') over all tensors, in place: params, m and v float32, grads of any type.
+
+    step: the update's number, counted from 1, or an int32 tensor of one element on the GPU holding it (a captured graph's
+    replays read it anew).  clip_norm: the gradients enter scaled by ``min(1, clip_norm / norm)``; the norm before clipping is
+    returned (a 0-d float32 tensor; None without clipping)."""
+    p, g, m, v = _set(params), _set(grads), _set(m), _set(v)
+    device, L = _device_of(p), lib()
+    for name, s in (("grads", g), ("m", m), ("v", v)):
+        if s.device != device or s._sizes != p._sizes:
+            raise ValueError(f"{name}: as many tensors of the same sizes as there are parameters, on their GPU")
+    step_dev = None
+    if isinstance(step, torch.Tensor):
+        if step.dtype != torch.int32 or step.numel() != 1 or step.device != device:
+            raise ValueError("step: a number, or an int32 tensor of one element on the parameters' GPU")
+        step_dev, step = step.data_ptr(), 0
+    if clip_norm is not None and not clip_norm > 0:
+        raise ValueError(f"clip_norm {clip_norm}: a positive number, or None")
+    tables = [s._same() for s in (p, g, m, v)]
+    norm = work = None
+    need = 0
+    with _On(device):
+        if clip_norm is not None:
+            norm = torch.empty((), dtype=torch.float32, device=device)
+            need = L.pvae_norm_workspace()
+            work = _workspace(need, device)
+        _check(L.pvae_adam_step(*tables, len(p), lr, beta1, beta2, eps, int(step), step_dev, float(clip_norm or 0.0), _ptr(norm),
+                                _ptr(work), need, torch.cuda.current_stream().cuda_stream))
+    return norm

@@ -1,0 +1,102 @@
+"""The operators' C ABI and refusals without a GPU: a refused call launches nothing, so these run on the CPU."""
+import ctypes as C
+import os
+import re
+
+import pytest
+import torch
+
+from popvae_amd import ops
+
+
+def test_header_symbols():
+    hdr = open(os.path.join(os.path.dirname(__file__), "..", "include", "pvae_ops.h")).read()
+    declared = set(re.findall(r"\b(pvae_\w+)\s*\(", hdr))
+    assert declared == set(ops.OPS_SYMBOLS)
+    for s in declared:
+        assert hasattr(ops.lib(), s)
+
+
+def test_structures_match_the_header():
+    hdr = open(os.path.join(os.path.dirname(__file__), "..", "include", "pvae_ops.h")).read()
+    for name, struct in (("pvae_dense_args", ops._Dense), ("pvae_dense_bwd_args", ops._DenseBwd), ("pvae_tensor", ops._Tensor)):
+        body = re.search(r"typedef struct %s \{(.*?)\}" % name, hdr, re.S).group(1)
+        fields = [f.strip(" *") for line in re.findall(r"[^;]+;", body) for f in
+                  re.sub(r"^\s*(const\s+)?(int32_t|int64_t|void|float)\b", "", line.strip().rstrip(";")).split(",")]
+        assert fields == [f for f, _ in struct._fields_]
+
+
+def test_cpu_tensors_are_refused():
+    x, w = torch.zeros(2, 3), torch.zeros(3, 4)
+    with pytest.raises(ValueError, match="GPU"):
+        ops.dense(x, w)
+    with pytest.raises(ValueError, match="GPU"):
+        ops.dense_backward(torch.zeros(2, 4), x, w)
+    with pytest.raises(ValueError):
+        ops.global_norm([x])
+    with pytest.raises(ValueError):
+        ops.TensorSet([x])
+
+
+def dense_args(**kw):
+    a = dict(dtype=0, act=0, m=2, k=4, n=8, x=4096, ldx=4, w=8192, w_sk=8, w_sn=1, bias=None, residual=None, ldr=0, y=16384, ldy=8,
+             pre=None, ldp=0)
+    a.update(kw)
+    return ops._Dense(**a)
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(dtype=3), "type"), (dict(act=7), "activation"), (dict(m=-1), "sizes"), (dict(n=1 << 31), "sizes"), (dict(x=None), "x is NULL"),
+    (dict(x=4097), "aligned"), (dict(ldx=3), "x: row stride"), (dict(ldx=1 << 60), "too large"), (dict(w_sk=7), "w: row stride"),
+    (dict(w_sk=16, w_sn=2), "neither"), (dict(w_sk=1, w_sn=3), "w\\^T"), (dict(y=None), "y is NULL"), (dict(ldy=7), "y: row stride"),
+    (dict(residual=4096, ldr=5), "residual"), (dict(pre=4098, ldp=8), "pre is not aligned"), (dict(pre=4096, ldp=4), "pre: row")])
+def test_dense_refusals(kw, text):
+    a = dense_args(**kw)
+    assert ops.lib().pvae_dense(a, None, 0, None) < 0
+    assert re.search(text, ops.lib().pvae_ops_last_error().decode())
+    assert ops.lib().pvae_dense_workspace(a) == 0
+
+
+def test_empty_calls_do_nothing():
+    assert ops.lib().pvae_dense(dense_args(m=0, x=None, y=None), None, 0, None) == 0
+    assert ops.lib().pvae_dense(dense_args(n=0, w=None, y=None), None, 0, None) == 0
+    assert ops.lib().pvae_dense(None, None, 0, None) == -1
+
+
+def test_a_missing_workspace_is_refused():
+    a = dense_args(m=64, k=100_000, n=64, ldx=100_000, w_sk=64, ldy=64)
+    need = ops.lib().pvae_dense_workspace(a)
+    assert need > 0
+    for ptr, have in ((None, need), (4096, need - 1), (4097, need)):
+        assert ops.lib().pvae_dense(a, ptr, have, None) < 0
+        assert "workspace" in ops.lib().pvae_ops_last_error().decode()
+
+
+def table(*rows):
+    return (ops._Tensor * len(rows))(*rows)
+
+
+def test_many_tensor_refusals():
+    L = ops.lib()
+    need = L.pvae_norm_workspace()
+    ok = table((4096, 10, 0, 0))
+    for t, n in ((ok, -1), (ok, 65537), (None, 1), (table((None, 5, 0, 0)), 1), (table((4097, 5, 0, 0)), 1), (table((4096, 5, 3, 0)), 1),
+                 (table((4096, -5, 0, 0)), 1), (table((4096, 8, 0, 4)), 1)):
+        assert L.pvae_global_norm(t, n, 64, 4096, need, None) < 0
+    assert L.pvae_global_norm(ok, 1, None, 4096, need, None) < 0
+    assert L.pvae_global_norm(ok, 1, 64, 4096, need - 1, None) < 0
+    for out, c in ((table((4100, 10, 0, 0)), 1.0), (table((8192, 9, 0, 0)), 1.0), (table((8192, 10, 1, 0)), 1.0), (ok, 0.0),
+                   (ok, float("nan")), (ok, -1.0)):
+        assert L.pvae_clip_by_global_norm(ok, out, 1, c, None, 4096, need, None) < 0
+    p, g, m, v = (table((i * 4096, 8, 0, 0)) for i in range(1, 5))
+    good = [1e-3, 0.9, 0.999, 1e-7, 1, None, 0.0]
+
+    def adam(p=p, g=g, m=m, v=v, **kw):
+        a = dict(zip(("lr", "b1", "b2", "eps", "step", "step_dev", "clip"), good), **kw)
+        return L.pvae_adam_step(p, g, m, v, 1, a["lr"], a["b1"], a["b2"], a["eps"], a["step"], a["step_dev"], a["clip"], None, None, 0, None)
+
+    for kw in (dict(lr=float("inf")), dict(b1=1.0), dict(b2=-0.1), dict(eps=0.0), dict(step=0), dict(clip=-1.0), dict(clip=1.0),
+               dict(p=g), dict(m=v), dict(p=table((4096, 8, 1, 0))), dict(g=table((8192, 9, 0, 0))), dict(p=table((4096, 8, 0, 4))),
+               dict(p=table((4096, 8, 0, 4)), m=table((4096 + 16, 8, 0, 4)), v=table((4096 + 16, 8, 0, 4)))):
+        assert adam(**kw) < 0, kw
+    assert L.pvae_adam_step(p, g, m, v, 0, *good, None, None, 0, None) == 0  # no tensors: nothing to do
