@@ -78,6 +78,18 @@ int pvae_get_lr(pvae_engine* e, float* lr);
  * reference: which path Keras takes is not visible there, so both are offered and tested against the oracle. */
 int pvae_set_bce_mode(pvae_engine* e, int mode);
 
+/* Keras' Adam(global_clipnorm = clip_norm), which the reference leaves unset: from the next train step on all gradients are
+ * scaled by min(1, clip_norm / norm), norm = the square root of the sum of squares over every tensor, before Adam sees them
+ * (pvae_clip_by_global_norm's rule; a norm that is not finite makes the model NaN).  0 turns it off.  Such a step stores
+ * its gradients (4 bytes per parameter more) and updates in a pass of its own.  Not under SNP sharding (world > 1: -5), nor
+ * through the staged calls and pvae_train_step_noalloc.  pvae_get_grad_norm: the last such step's norm before clipping. */
+int pvae_set_clip_norm(pvae_engine* e, float clip_norm);
+int pvae_get_grad_norm(pvae_engine* e, float* norm);
+/* No counterpart in the reference: hidden layers of equal width as residual layers, h = elu(h W + b) + h (encoder layers
+ * 2 .. depth, decoder layers 2 .. depth; the first layer of each side and the heads stay as they are).  Same tensors, same
+ * weight files; runs layer by layer (pvae_dense, pvae_dense_bwd), 32 rows per device pass.  0 returns to plain layers. */
+int pvae_set_residual(pvae_engine* e, int on);
+
 /* one train_step of vae.fit (popvae.py:490): rows = sample indices into the resident matrix (n <= batch_size),
  * eps = injected N(0,1) [n][latent_dim] or NULL for the engine's own stream.
  * out3 = {loss, mean reconstruction, mean KL} or NULL (no host sync when NULL). */

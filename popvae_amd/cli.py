@@ -58,6 +58,11 @@ def build_parser():
     p.add_argument("--bce_mode", default="logits", choices=("logits", "probs"),
                    help="(popvae_amd) form of Keras' binary cross-entropy: from the logits (Keras in graph mode, default) or "
                         "from probabilities clipped to [1e-7, 1 - 1e-7]; they differ where |logit| > 16")
+    p.add_argument("--clip_norm", default=None, type=float,
+                   help="(popvae_amd) scale each step's gradients to at most this global norm (Keras' Adam(global_clipnorm=...)); "
+                        "default: not clipped, as in the reference")
+    p.add_argument("--residual", default=False, action="store_true",
+                   help="(popvae_amd) residual hidden layers, h = elu(h W + b) + h (for deep networks; not a model of the reference)")
     p.add_argument("--init_weights", default=None,
                    help="(popvae_amd) initialise the model from a Keras weight file (.hdf5) or .npz instead of glorot_uniform")
     return p
@@ -123,6 +128,10 @@ def main(argv=None):
         raise SystemExit(0)
     if args.infile is None:
         raise SystemExit("--infile is required")
+    if args.clip_norm is not None and not args.clip_norm > 0:
+        raise SystemExit("--clip_norm: a positive number")
+    if args.clip_norm is not None and int(os.environ.get("WORLD_SIZE", "1")) > 1:
+        raise SystemExit("--clip_norm: not with the SNP axis sharded over several GPUs (the norm spans all shards)")
 
     from . import fit as F
     from . import prep
@@ -198,6 +207,9 @@ def main(argv=None):
         e.load_genotypes(packed)
         e.init_weights(eng_seed)
         e.set_bce_mode(args.bce_mode)
+        if args.residual:
+            e.set_residual(True)
+        e.set_clip_norm(args.clip_norm)
         return e
 
     width, depth = args.width, args.depth
@@ -227,6 +239,8 @@ def main(argv=None):
         eng.load_genotypes(packed)
         eng.init_weights(eng_seed)
         eng.eng.set_bce_mode(args.bce_mode)
+        if args.residual:
+            eng.eng.set_residual(True)
     else:
         eng = make_single(width, depth)
     if args.init_weights:  # vae.load_weights before fit (per-step parity from a Keras export)

@@ -25,6 +25,7 @@
 #include <dlfcn.h>
 
 #include "../../include/pvae.h"
+#include "../../include/pvae_ops.h"
 #include "pvae_kernels.h"
 #include "pvae_narrow.h"
 #include "pvae_pca.h"
@@ -70,8 +71,8 @@ struct TensorRef {
     int64_t rows, cols;  // Keras shape (cols = 0 for bias)
 };
 
-enum Cat { C_GATHER, C_ENC_FWD, C_NARROW_FWD, C_DEC, C_NARROW_BWD, C_ENC_BWD, C_XCH0, C_XCH1, C_DEC_UPD, C_REDUCE, C_NCAT };
-const char* kCatNames[C_NCAT] = {"gather", "enc_fwd", "narrow_fwd", "dec", "narrow_bwd", "enc_bwd", "xch0", "xch1", "dec_upd", "reduce"};
+enum Cat { C_GATHER, C_ENC_FWD, C_NARROW_FWD, C_DEC, C_NARROW_BWD, C_ENC_BWD, C_XCH0, C_XCH1, C_DEC_UPD, C_REDUCE, C_UPDATE, C_NCAT };
+const char* kCatNames[C_NCAT] = {"gather", "enc_fwd", "narrow_fwd", "dec", "narrow_bwd", "enc_bwd", "xch0", "xch1", "dec_upd", "reduce", "update"};
 
 }  // namespace
 
@@ -166,6 +167,18 @@ struct pvae_engine {
     float lr_host = 1e-3f;
     int bce_probs = 0;  // pvae_set_bce_mode
     bool has_best = false;
+    // pvae_set_clip_norm: a train step dumps its gradients, and pvae_adam_step applies them scaled by the global norm
+    double clip_norm = 0.0;
+    float* grad_norm = nullptr;   // the last such step's norm
+    void* norm_ws = nullptr;
+    bool clip_stepped = false;    // grad_norm holds one
+    // pvae_set_residual: hidden layers h = elu(h W + b) + h through pvae_dense / pvae_dense_bwd, one launch per layer; their
+    // pre-activations [32][Wp] are kept for the backward.  The fused chain and the multi-tile passes are off meanwhile.
+    bool residual = false, fused_full = false;
+    int T_full = 1;
+    std::vector<float*> enc_pre, dec_pre;
+    void* dense_ws = nullptr;
+    int64_t dense_ws_bytes = 0;
     // SNP-axis sharding with the engine's own RCCL communicator (pvae_comm_init): the two all-reduces of a step are
     // enqueued on the engine's stream between the stages, no host code and no cross-stream events in between
     void* comm = nullptr;
@@ -672,21 +685,67 @@ int narrow_fused_fwd(pvae_engine* e, bool encoder_only, bool decoder_only = fals
     return launch_check(e, "narrow_fwd");
 }
 
+// residual hidden layers (pvae_set_residual): all 32 rows of the tile; rows beyond the batch are finite, and their gradients,
+// which arrive as zeros, stay zeros
+pvae_dense_args residual_fwd_args(const pvae_engine* e, const Dense& d, const float* in, float* out, float* pre) {
+    pvae_dense_args a{};
+    a.dtype = PVAE_F32;
+    a.act = d.act == PV_ACT_ELU ? PVAE_ELU : PVAE_LINEAR;
+    a.m = 32; a.k = d.kin; a.n = d.nout;
+    a.x = in; a.ldx = d.kin;
+    a.w = d.W.w; a.w_sk = d.nout; a.w_sn = 1;
+    a.bias = d.B.w;
+    a.residual = in; a.ldr = d.kin;
+    a.y = out; a.ldy = d.nout;
+    a.pre = pre; a.ldp = d.nout;
+    return a;
+}
+pvae_dense_bwd_args residual_bwd_args(const pvae_engine* e, const Dense& d, const float* dY, const float* pre, float* dIn, float* dpre) {
+    pvae_dense_bwd_args a{};
+    a.dtype = PVAE_F32;
+    a.act = d.act == PV_ACT_ELU ? PVAE_ELU : PVAE_LINEAR;
+    a.m = 32; a.k = d.kin; a.n = d.nout;
+    a.dy = dY; a.lddy = d.nout;
+    a.w = d.W.w; a.w_sk = d.nout; a.w_sn = 1;
+    a.pre = pre; a.ldp = d.nout;
+    a.dx = dIn; a.lddx = d.kin;
+    a.dx_add = dY; a.ldadd = d.kin;
+    a.dpre = dpre;
+    return a;
+}
+int run_residual_fwd(pvae_engine* e, const Dense& d, const float* in, float* out, float* pre) {
+    const pvae_dense_args a = residual_fwd_args(e, d, in, out, pre);
+    const int rc = pvae_dense(&a, e->dense_ws, e->dense_ws_bytes, e->stream);
+    return rc ? set_err(e, rc, "residual layer: %s", pvae_ops_last_error()) : 0;
+}
+int run_residual_bwd(pvae_engine* e, const Dense& d, const float* dY, const float* pre, float* dIn, float* dpre) {
+    const pvae_dense_bwd_args a = residual_bwd_args(e, d, dY, pre, dIn, dpre);
+    const int rc = pvae_dense_bwd(&a, e->dense_ws, e->dense_ws_bytes, e->stream);
+    return rc ? set_err(e, rc, "residual layer's gradient: %s", pvae_ops_last_error()) : 0;
+}
+
 // narrow encoder: h1 = elu(P + b1), hidden layers, heads, reparameterisation + KL
 int narrow_encoder(pvae_engine* e) {
     int rc;
     if (e->fused_narrow) return narrow_fused_fwd(e, true);
+    if (e->residual) {
+        hipLaunchKernelGGL(pvk_bias_act, dim3((32 * e->Wp + 255) / 256), dim3(256), 0, e->stream, (const float*)e->P, (const float*)e->b1.w,
+                           e->Wp, (int)PV_ACT_ELU, e->h[0]);
+        if ((rc = launch_check(e, "bias_act"))) return rc;
+        for (int i = 0; i < e->D - 1; ++i)
+            if ((rc = run_residual_fwd(e, e->enc[i], e->h[i], e->h[i + 1], e->enc_pre[i]))) return rc;
+    }
     // h1 = elu(P + b1) is formed inside the first consumer's staging loop (workgroup 0 writes it out for the backward)
-    for (int i = 0; i < e->D - 1; ++i)
+    for (int i = 0; i < e->D - 1 && !e->residual; ++i)
         if ((rc = i == 0 ? run_dense_fwd(e, e->enc[0], e->P, e->h[1], e->b1.w, e->h[0])
                          : run_dense_fwd(e, e->enc[i], e->h[i], e->h[i + 1]))) return rc;
     // the heads layer is one workgroup (Kh = 32 outputs): the sampling layer + KL run in its tail
     if (e->Kh == 32) {
         const PvRepFwd rp{e->eps, e->z, e->kl, e->K, e->Kz};
-        return e->D == 1 ? run_dense_fwd(e, e->heads, e->P, e->headout, e->b1.w, e->h[0], rp)
+        return e->D == 1 && !e->residual ? run_dense_fwd(e, e->heads, e->P, e->headout, e->b1.w, e->h[0], rp)
                          : run_dense_fwd(e, e->heads, e->h[e->D - 1], e->headout, nullptr, nullptr, rp);
     }
-    if ((rc = e->D == 1 ? run_dense_fwd(e, e->heads, e->P, e->headout, e->b1.w, e->h[0])
+    if ((rc = e->D == 1 && !e->residual ? run_dense_fwd(e, e->heads, e->P, e->headout, e->b1.w, e->h[0])
                         : run_dense_fwd(e, e->heads, e->h[e->D - 1], e->headout))) return rc;
     hipLaunchKernelGGL(pvk_reparam, dim3(1), dim3(64), 0, e->stream, e->headout, e->Kh, e->K, e->eps, e->z, e->Kz, e->kl);
     return launch_check(e, "reparam");
@@ -696,7 +755,8 @@ int narrow_decoder(pvae_engine* e) {
     int rc;
     if ((rc = run_dense_fwd(e, e->dec[0], e->z, e->g[0]))) return rc;
     for (int i = 1; i < e->D; ++i)
-        if ((rc = run_dense_fwd(e, e->dec[i], e->g[i - 1], e->g[i]))) return rc;
+        if ((rc = e->residual ? run_residual_fwd(e, e->dec[i], e->g[i - 1], e->g[i], e->dec_pre[i])
+                              : run_dense_fwd(e, e->dec[i], e->g[i - 1], e->g[i]))) return rc;
     return 0;
 }
 
@@ -919,6 +979,12 @@ int stage_c(pvae_engine* e, int mode, float* d_out3, bool fuse = false, int next
         // buffer (what the Adam launch reads) and the consumer stages it as it comes -- no pass over Y and no act' in between
         bool chained = false;  // dY is already the dpre of the layer about to run
         for (int i = D - 1; i >= 1; --i) {
+            if (e->residual) {
+                if ((rc = run_residual_bwd(e, e->dec[i], dY, e->dec_pre[i], bufs[pp], e->dpre_bufs[li++]))) return rc;
+                dY = bufs[pp];
+                pp ^= 1;
+                continue;
+            }
             const bool to_next = i - 1 >= 1 && dense16_bwd_ok(e, e->dec[i]) && dense16_bwd_ok(e, e->dec[i - 1]);
             float* dst = to_next ? e->dpre_bufs[li + 1] : bufs[pp];
             if ((rc = run_dense_bwd(e, e->dec[i], e->g[i], dY, dst, e->dpre_bufs[li], PvRepBwd{}, chained,
@@ -942,6 +1008,12 @@ int stage_c(pvae_engine* e, int mode, float* d_out3, bool fuse = false, int next
         pp ^= 1;
         chained = false;
         for (int i = D - 2; i >= 0; --i) {
+            if (e->residual) {
+                if ((rc = run_residual_bwd(e, e->enc[i], dY, e->enc_pre[i], bufs[pp], e->dpre_bufs[li++]))) return rc;
+                dY = bufs[pp];
+                pp ^= 1;
+                continue;
+            }
             const bool to_next = i - 1 >= 0 && dense16_bwd_ok(e, e->enc[i]) && dense16_bwd_ok(e, e->enc[i - 1]);
             float* dst = to_next ? e->dpre_bufs[li + 1] : bufs[pp];
             if ((rc = run_dense_bwd(e, e->enc[i], e->h[i + 1], dY, dst, e->dpre_bufs[li], PvRepBwd{}, chained,
@@ -971,6 +1043,25 @@ int stage_c(pvae_engine* e, int mode, float* d_out3, bool fuse = false, int next
         if ((rc = launch_check(e, "narrow_adam/bias_bwd"))) return rc;
     }
     return enc_bwd_launch(e, km, fuse, next_off, next_n, nullptr, Xn);
+}
+
+// the update of a step with clipping: all gradients have been dumped (mode 2), Adam's t advanced by the step's head
+int clipped_update(pvae_engine* e) {
+    Timer t(e, C_UPDATE);
+    std::vector<pvae_tensor> p, g, m, v;
+    for_each_buf(e, [&](Buf3& b) {
+        const int32_t tile = (int32_t)b.il_tile;
+        p.push_back({b.w, b.n, PVAE_F32, tile});
+        g.push_back({b.g, b.n, PVAE_F32, 0});
+        m.push_back({b.m, b.n, PVAE_F32, tile});
+        v.push_back({b.v, b.n, PVAE_F32, tile});
+    });
+    const int rc = pvae_adam_step(p.data(), g.data(), m.data(), v.data(), (int64_t)p.size(), e->lr_host, e->adam.b1, e->adam.b2, e->adam.eps,
+                                  0, &e->st->t, e->clip_norm, e->grad_norm, e->norm_ws, pvae_norm_workspace(), e->stream);
+    if (rc) return set_err(e, rc, "clipped update: %s", pvae_ops_last_error());
+    e->narrow_pack_dirty = true;
+    e->clip_stepped = true;
+    return 0;
 }
 
 int ensure_rows(pvae_engine* e, int64_t n) {
@@ -1275,20 +1366,24 @@ int full_step(pvae_engine* e, const int32_t* rows, int32_t n, const float* eps, 
         return set_err(e, -5, "world > 1: call pvae_comm_init first, or drive the step through pvae_stage_a/b/c with "
                               "all-reduces in between");
     if (n <= 0 || n > e->cfg.batch_size) return set_err(e, -2, "batch of %d rows (batch_size %d)", n, e->cfg.batch_size);
+    const bool clip = mode == 0 && e->clip_norm > 0;  // every pass dumps its gradients, one update at the end
     if (n <= 32) {
+        const int pass = clip ? 2 : mode;
         if ((rc = ensure_loss(e, 1))) return rc;
         if ((rc = begin_batch(e, rows, n, eps, mode == 0))) return rc;
         if ((rc = stage_a(e, 0, true))) return rc;
         if ((rc = shard_allreduce(e, 0))) return rc;
-        if ((rc = stage_b(e, mode))) return rc;
+        if ((rc = stage_b(e, pass))) return rc;
         if ((rc = shard_allreduce(e, 1))) return rc;
-        if ((rc = stage_c(e, mode, e->d_loss))) return rc;
+        if ((rc = stage_c(e, pass, e->d_loss))) return rc;
+        if (clip && (rc = clipped_update(e))) return rc;
         return fetch_out3(e, out3);
     }
     if (mode == 0 && e->T > 1 && n <= 32 * e->T) {  // one weight pass for the whole batch
         if ((rc = ensure_loss(e, 1))) return rc;
         if ((rc = begin_batch(e, rows, n, eps, true, 32 * e->T))) return rc;
-        if ((rc = multi_tile_train(e, 0, e->d_loss))) return rc;
+        if ((rc = multi_tile_train(e, 0, e->d_loss, clip ? 2 : 0))) return rc;
+        if (clip && (rc = clipped_update(e))) return rc;
         return fetch_out3(e, out3);
     }
     const int R = 32 * e->T;
@@ -1319,7 +1414,7 @@ int full_step(pvae_engine* e, const int32_t* rows, int32_t n, const float* eps, 
             const int nb = std::min(R, n - R * c);
             // begin_batch uploads this chunk's rows (+ eps) and, on the first chunk, advances Adam's t
             if ((rc = begin_batch(e, rows + R * c, nb, eps ? eps + (size_t)R * c * e->K : nullptr, c == 0, R))) return rc;
-            if ((rc = run_chunk(e, 0, nb, n, c, c == nt - 1, e->d_loss + 3 * c))) return rc;
+            if ((rc = run_chunk(e, 0, nb, n, c, c == nt - 1 && !clip, e->d_loss + 3 * c))) return rc;
         }
     }
     if (!chunks && (rc = ensure_loss(e, nt))) return rc;
@@ -1327,9 +1422,10 @@ int full_step(pvae_engine* e, const int32_t* rows, int32_t n, const float* eps, 
         const int nb = std::min(32, n - 32 * t);
         // begin_batch uploads this tile's rows (+ eps) and, on the first tile of a train step, advances Adam's t
         if ((rc = begin_batch(e, rows + 32 * t, nb, eps ? eps + (size_t)32 * t * e->K : nullptr, mode == 0 && t == 0))) return rc;
-        const int tm = mode == 1 ? 1 : (mode == 0 && t == nt - 1) ? 4 : 2;
+        const int tm = mode == 1 ? 1 : (mode == 0 && t == nt - 1 && !clip) ? 4 : 2;
         if ((rc = run_tile(e, 0, nb, n, t, tm, e->d_loss + 3 * t))) return rc;
     }
+    if (clip && (rc = clipped_update(e))) return rc;
     std::vector<float> hl((size_t)nt * 3);
     HIPCHK(hipMemcpyAsync(hl.data(), e->d_loss, hl.size() * sizeof(float), hipMemcpyDeviceToHost, e->stream));
     HIPCHK(hipStreamSynchronize(e->stream));
@@ -1671,6 +1767,8 @@ int pvae_create(const pvae_config* cfg, pvae_engine** out) {
     HK(hipHostMalloc((void**)&e->h_out3, 4 * sizeof(float), hipHostMallocDefault));
     CK(scratch_address(e, e->dev, &e->scratch));
     e->fused_narrow = e->Wp <= 128 && 2 * e->D + 2 <= PVN_MAXOPS && !getenv("PVAE_NO_FUSED_NARROW");
+    e->fused_full = e->fused_narrow;
+    e->T_full = e->T;
     e->narrow_warm = !getenv("PVAE_NO_NARROW_WARM");
     {
         const char* sd = getenv("PVAE_SPLIT_DEC");
@@ -1728,6 +1826,9 @@ int pvae_destroy(pvae_engine* e) {
     for (auto p : fl) hipFree(p);
     hipFree(e->d_fwd_ops); hipFree(e->d_bwd_ops); hipFree(e->d_bwd_ops_grad);
     for (auto p : e->dpre_bufs) hipFree(p);
+    for (auto p : e->enc_pre) hipFree(p);
+    for (auto p : e->dec_pre) hipFree(p);
+    hipFree(e->dense_ws); hipFree(e->norm_ws); hipFree(e->grad_norm);
     hipFree(e->probs);
     hipFree(e->enc_out);
     hipFree(e->Xt); hipFree(e->Xr); hipFree(e->Xrn); hipFree(e->Xt2); hipFree(e->geno); hipFree(e->st); hipFree(e->d_rows); hipFree(e->d_ntotal); hipFree(e->d_counter);
@@ -1846,6 +1947,58 @@ int pvae_set_bce_mode(pvae_engine* e, int mode) {
     return 0;
 }
 
+int pvae_set_clip_norm(pvae_engine* e, float clip_norm) {
+    if (!(clip_norm >= 0.f)) return set_err(e, -2, "clip_norm %g: a positive number, or 0 for none", clip_norm);
+    if (clip_norm > 0.f && e->cfg.world != 1)
+        return set_err(e, -5, "clipping under SNP sharding is not offered: the norm spans the shards of all ranks");
+    HIPCHK(hipSetDevice(e->dev));
+    if (clip_norm > 0.f && !e->norm_ws) {
+        HIPCHK(hipMalloc(&e->norm_ws, (size_t)pvae_norm_workspace()));
+        HIPCHK(hipMalloc(&e->grad_norm, sizeof(float)));
+    }
+    e->promised_rows.clear();
+    e->clip_norm = clip_norm;
+    e->clip_stepped = false;
+    return 0;
+}
+
+int pvae_get_grad_norm(pvae_engine* e, float* norm) {
+    if (!norm) return set_err(e, -1, "norm is NULL");
+    if (!e->clip_stepped) return set_err(e, -6, "no train step with clipping yet");
+    HIPCHK(hipMemcpyAsync(e->h_out3 + 3, e->grad_norm, sizeof(float), hipMemcpyDeviceToHost, e->stream));
+    HIPCHK(hipStreamSynchronize(e->stream));
+    *norm = e->h_out3[3];
+    return 0;
+}
+
+int pvae_set_residual(pvae_engine* e, int on) {
+    int rc;
+    HIPCHK(hipSetDevice(e->dev));
+    HIPCHK(hipStreamSynchronize(e->stream));  // the op tables are rewritten below
+    e->promised_rows.clear();
+    if (on) {
+        e->enc_pre.resize(e->D - 1, nullptr);
+        e->dec_pre.resize(e->D, nullptr);  // dec_pre[0] stays NULL: the first decoder layer has another input size
+        for (auto& p : e->enc_pre)
+            if (!p && (rc = allocf(e, &p, (int64_t)32 * e->Wp))) return rc;
+        for (int i = 1; i < e->D; ++i)
+            if (!e->dec_pre[i] && (rc = allocf(e, &e->dec_pre[i], (int64_t)32 * e->Wp))) return rc;
+        if (e->D > 1 && !e->dense_ws) {  // one layer's sizes are every layer's
+            const pvae_dense_args f = residual_fwd_args(e, e->dec[1], e->g[0], e->g[1], e->dec_pre[1]);
+            const pvae_dense_bwd_args b = residual_bwd_args(e, e->dec[1], e->dA, e->dec_pre[1], e->dB, e->dpre1);
+            const int64_t need = std::max(pvae_dense_workspace(&f), pvae_dense_bwd_workspace(&b));
+            if (need) HIPCHK(hipMalloc(&e->dense_ws, (size_t)need));
+            e->dense_ws_bytes = need;
+        }
+    }
+    e->residual = on != 0;
+    e->fused_narrow = e->fused_full && !e->residual;
+    e->T = e->residual ? 1 : e->T_full;
+    e->narrow_pack_dirty = true;
+    if ((rc = build_bwd_ops(e, false, &e->d_bwd_ops))) return rc;
+    return e->d_bwd_ops_grad ? build_bwd_ops(e, true, &e->d_bwd_ops_grad) : 0;
+}
+
 int pvae_get_lr(pvae_engine* e, float* lr) {
     *lr = e->lr_host;
     return 0;
@@ -1870,6 +2023,8 @@ int pvae_train_step_noalloc(pvae_engine* e, const int32_t* rows, int32_t n, cons
                               "tiles with gradient dumps that pvae_train_step allocates on first use", n);
     if (e->cfg.world != 1 || has_comm(e))
         return set_err(e, -5, "pvae_train_step_noalloc: SNP-sharded engines exchange through RCCL, which allocates");
+    if (e->clip_norm > 0)
+        return set_err(e, -6, "pvae_train_step_noalloc: a step with clipping keeps gradient dumps, which it allocates on first use");
     if (e->timing) return set_err(e, -6, "pvae_train_step_noalloc: switch event timing off first (events are created on demand)");
     auto al = [](size_t floats) { return (floats + 63) / 64 * 64; };  // 256-byte steps
     const size_t n_enc = al((size_t)e->encpart_floats);
@@ -1906,6 +2061,7 @@ int pvae_train_epoch(pvae_engine* e, const int32_t* perm, int32_t n_train, const
     if (n_val > 0)
         HIPCHK(hipMemcpyAsync(e->d_rows + n_train, val_rows, (size_t)n_val * sizeof(int), hipMemcpyHostToDevice, e->stream));
     bool fwd_done = false;
+    const bool clip = e->clip_norm > 0;  // training passes dump their gradients, one update per batch
     const int tp = (B + 31) / 32;  // 32-row tiles per batch
     // batches above 32 rows: every loss slot of the epoch starts at zero (tiles a short batch does not reach stay there) -- one
     // fill per epoch, and the per-step scalars share a launch with the first noise draw of the step (three launch slots per
@@ -1931,10 +2087,11 @@ int pvae_train_epoch(pvae_engine* e, const int32_t* perm, int32_t n_train, const
                 for (int c = 0; c < nc; ++c) {
                     begin_eps(R * e->K);
                     if ((rc = launch_check(e, "step_begin/gen_eps"))) return rc;
-                    if (nc == 1) rc = multi_tile_train(e, base + s * B, slot);
-                    else rc = run_chunk(e, base + s * B + R * c, std::min(R, nb - R * c), nb, c, c == nc - 1, slot + 3 * c);
+                    if (nc == 1) rc = multi_tile_train(e, base + s * B, slot, clip ? 2 : 0);
+                    else rc = run_chunk(e, base + s * B + R * c, std::min(R, nb - R * c), nb, c, c == nc - 1 && !clip, slot + 3 * c);
                     if (rc) return rc;
                 }
+                if (clip && (rc = clipped_update(e))) return rc;
                 continue;
             }
             if (phase == 1 && e->T > 1 && nb > 32 && e->fused_narrow) {  // validation: one read of the wide weights per 32 T rows
@@ -1951,9 +2108,10 @@ int pvae_train_epoch(pvae_engine* e, const int32_t* perm, int32_t n_train, const
                 if ((rc = launch_check(e, "step_begin/gen_eps"))) return rc;
                 // a short last batch of at most 32 rows is ONE tile: a plain train step (TRAIN_ACC would add the gradient
                 // dump the previous batch's tiles left behind, or find none at all when n_train <= 32 < batch_size)
-                const int tm = phase == 1 ? 1 : nb <= 32 ? 0 : (t + 1) * 32 >= nb ? 4 : 2;
+                const int tm = phase == 1 ? 1 : clip ? 2 : nb <= 32 ? 0 : (t + 1) * 32 >= nb ? 4 : 2;
                 if ((rc = run_tile(e, base + s * B + 32 * t, std::min(32, nb - 32 * t), nb, t, tm, slot + 3 * t))) return rc;
             }
+            if (clip && phase == 0 && (rc = clipped_update(e))) return rc;
         }
     }
     // batch size 32: the validation batches go through the read-only kernels T at a time, each with its own loss (one read
@@ -1987,7 +2145,7 @@ int pvae_train_epoch(pvae_engine* e, const int32_t* perm, int32_t n_train, const
             // the first-layer forward of the NEXT batch rides on this step's wide encoder backward
             int next_off = 0, next_n = 0;
             bool fuse = false;
-            if (phase == 0 && e->fuse_fwd) {
+            if (phase == 0 && e->fuse_fwd && !clip) {
                 if (s + 1 < st_tr) { next_off = (s + 1) * B; next_n = std::min(B, n_train - next_off); fuse = true; }
                 else if (st_va > 0 && !mt_val) { next_off = n_train; next_n = std::min(B, (int)n_val); fuse = true; }
             }
@@ -2023,11 +2181,13 @@ int pvae_train_epoch(pvae_engine* e, const int32_t* perm, int32_t n_train, const
             if ((rc = launch_check(e, "step_begin/gen_eps/gather"))) return rc;
             if ((rc = stage_a(e, base + s * B, false, fwd_done, fwd_done))) return rc;
             if ((rc = shard_allreduce(e, 0))) return rc;
-            if ((rc = stage_b(e, phase == 0 ? 0 : 1))) return rc;
+            const int pass = phase == 1 ? 1 : clip ? 2 : 0;
+            if ((rc = stage_b(e, pass))) return rc;
             if ((rc = shard_allreduce(e, 1))) return rc;
             if ((rc = join_gather(e))) return rc;  // the fused forward of the wide encoder backward reads the next batch's words
-            if ((rc = stage_c(e, phase == 0 ? 0 : 1, e->d_loss + 3 * ((phase == 0 ? 0 : st_tr) + s), fuse, next_off, next_n, xrn)))
+            if ((rc = stage_c(e, pass, e->d_loss + 3 * ((phase == 0 ? 0 : st_tr) + s), fuse, next_off, next_n, xrn)))
                 return rc;
+            if (clip && phase == 0 && (rc = clipped_update(e))) return rc;
             fwd_done = fuse;
         }
     }
@@ -2273,9 +2433,16 @@ int pvae_stage_a(pvae_engine* e, const int32_t* rows, int32_t n, const float* ep
     e->promised_rows.clear();
     return stage_a(e, 0, mode != 3, fwd_done);
 }
-int pvae_stage_b(pvae_engine* e, int mode) { return stage_b(e, mode); }
+static int staged_unclipped(pvae_engine* e, int mode) {
+    return mode == 0 && e->clip_norm > 0 ? set_err(e, -5, "staged train steps do not clip (pvae_set_clip_norm): the norm spans all shards") : 0;
+}
+int pvae_stage_b(pvae_engine* e, int mode) {
+    const int rc = staged_unclipped(e, mode);
+    return rc ? rc : stage_b(e, mode);
+}
 int pvae_stage_c(pvae_engine* e, int mode, float* out3) {
     int rc;
+    if ((rc = staged_unclipped(e, mode))) return rc;
     e->promised_rows.clear();
     if ((rc = ensure_loss(e, 1))) return rc;
     if ((rc = stage_c(e, mode, e->d_loss))) return rc;
@@ -2284,6 +2451,7 @@ int pvae_stage_c(pvae_engine* e, int mode, float* out3) {
 int pvae_stage_c_next(pvae_engine* e, int mode, float* out3, const int32_t* next_rows, int32_t next_n) {
     int rc;
     e->promised_rows.clear();
+    if ((rc = staged_unclipped(e, mode))) return rc;
     if (mode != 0 || !e->fuse_fwd || !next_rows || next_n <= 0) return pvae_stage_c(e, mode, out3);
     if (next_n > 32) return set_err(e, -2, "a device pass takes at most 32 rows (got %d)", next_n);
     if ((rc = check_rows(e, next_rows, next_n))) return rc;
