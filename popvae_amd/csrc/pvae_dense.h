@@ -36,28 +36,46 @@ template <int DT> __device__ __forceinline__ typename PvdType<DT>::T pvd_from_f3
 __device__ __forceinline__ float pvd_sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
 __device__ __forceinline__ float pvd_phi(float z) { return __expf(-0.5f * z * z) * 0.3989422804014327f; }
 __device__ __forceinline__ float pvd_Phi(float z) { return 0.5f * (1.f + erff(z * 0.7071067811865476f)); }
-__device__ __forceinline__ float pvd_act(float z, int act) {
+// the kind is the same for the whole launch: one branch for four values
+__device__ __forceinline__ pvd_f32x4 pvd_act4(pvd_f32x4 z, int act) {
+#define PVD_EACH(EXPR)                                  \
+    _Pragma("unroll") for (int e = 0; e < 4; ++e) {     \
+        const float x = z[e];                           \
+        z[e] = EXPR;                                    \
+    }                                                   \
+    return z;
     switch (act) {
-        case PVD_RELU: return z > 0.f ? z : z != z ? z : 0.f;
-        case PVD_ELU: return z > 0.f ? z : expm1f(z);
-        case PVD_SIGMOID: return pvd_sigmoid(z);
-        case PVD_TANH: return tanhf(z);
-        case PVD_SILU: return z * pvd_sigmoid(z);
-        case PVD_GELU: return z * pvd_Phi(z);
+        case PVD_RELU: PVD_EACH(x > 0.f ? x : x != x ? x : 0.f)
+        case PVD_ELU: PVD_EACH(x > 0.f ? x : expm1f(x))
+        case PVD_SIGMOID: PVD_EACH(pvd_sigmoid(x))
+        case PVD_TANH: PVD_EACH(tanhf(x))
+        case PVD_SILU: PVD_EACH(x * pvd_sigmoid(x))
+        case PVD_GELU: PVD_EACH(x * pvd_Phi(x))
         default: return z;
     }
 }
-__device__ __forceinline__ float pvd_act_grad(float z, int act) {
-    switch (act) {
-        case PVD_RELU: return z > 0.f ? 1.f : 0.f;
-        case PVD_ELU: return z > 0.f ? 1.f : __expf(z);
-        case PVD_SIGMOID: { const float s = pvd_sigmoid(z); return s * (1.f - s); }
-        case PVD_TANH: { const float t = tanhf(z); return 1.f - t * t; }
-        case PVD_SILU: { const float s = pvd_sigmoid(z); return s * (1.f + z * (1.f - s)); }
-        case PVD_GELU: return pvd_Phi(z) + z * pvd_phi(z);
-        default: return 1.f;
-    }
+__device__ __forceinline__ float pvd_silu_grad(float z) {
+    const float s = pvd_sigmoid(z);
+    return s * (1.f + z * (1.f - s));
 }
+__device__ __forceinline__ float pvd_tanh_grad(float z) {
+    const float t = tanhf(z);
+    return 1.f - t * t;
+}
+__device__ __forceinline__ pvd_f32x4 pvd_act_grad4(pvd_f32x4 z, int act) {
+    switch (act) {
+        case PVD_RELU: PVD_EACH(x > 0.f ? 1.f : 0.f)
+        case PVD_ELU: PVD_EACH(x > 0.f ? 1.f : __expf(x))
+        case PVD_SIGMOID: PVD_EACH(pvd_sigmoid(x) * pvd_sigmoid(-x))
+        case PVD_TANH: PVD_EACH(pvd_tanh_grad(x))
+        case PVD_SILU: PVD_EACH(pvd_silu_grad(x))
+        case PVD_GELU: PVD_EACH(pvd_Phi(x) + x * pvd_phi(x))
+        default: return (pvd_f32x4){1.f, 1.f, 1.f, 1.f};
+    }
+#undef PVD_EACH
+}
+__device__ __forceinline__ float pvd_act(float z, int act) { return pvd_act4((pvd_f32x4){z, z, z, z}, act)[0]; }
+__device__ __forceinline__ float pvd_act_grad(float z, int act) { return pvd_act_grad4((pvd_f32x4){z, z, z, z}, act)[0]; }
 
 // ---------------------------------------------------------------------------------------------
 // what follows the product
@@ -84,23 +102,22 @@ template <int DT> __device__ __forceinline__ void pvd_finish4(const PvdOut& O, i
     if (O.vec && n + 3 < O.cols) {
         if (bias) z += pvm_load4(bias, DT, n);
         if (O.pre) *reinterpret_cast<pvd_f32x4*>(O.pre + m * O.ldp + n) = z;
-        pvd_f32x4 o;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = pvd_act(z[e], O.act);
+        pvd_f32x4 o = pvd_act4(z, O.act);
         if (res) o += pvm_load4(res, DT, m * O.ldr + n);
         pvm_store4(y, DT, 0, o);
         return;
     }
+    const int left = (int)min((int64_t)4, O.cols - n);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        if (n + e >= O.cols) return;
-        float a = z[e];
-        if (bias) a += pvd_to_f32<DT>(bias[n + e]);
-        if (O.pre) O.pre[m * O.ldp + n + e] = a;
-        a = pvd_act(a, O.act);
-        if (res) a += pvd_to_f32<DT>(res[m * O.ldr + n + e]);
-        y[e] = pvd_from_f32<DT>(a);
-    }
+    for (int e = 0; e < 4; ++e)
+        if (e < left) {
+            if (bias) z[e] += pvd_to_f32<DT>(bias[n + e]);
+            if (O.pre) O.pre[m * O.ldp + n + e] = z[e];
+        }
+    const pvd_f32x4 o = pvd_act4(z, O.act);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (e < left) y[e] = pvd_from_f32<DT>(res ? o[e] + pvd_to_f32<DT>(res[m * O.ldr + n + e]) : o[e]);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -139,9 +156,9 @@ template <int DT, bool GRAD> struct PvdStage {
             if (GRAD && P.act != PVD_LINEAR) {
 #pragma unroll
                 for (int e = 0; e < VEC; e += 4) {
-                    const pvd_f32x4 z4 = *reinterpret_cast<const pvd_f32x4*>(z + e);
+                    const pvd_f32x4 d4 = pvd_act_grad4(*reinterpret_cast<const pvd_f32x4*>(z + e), P.act);
 #pragma unroll
-                    for (int f = 0; f < 4; ++f) o[e + f] = pvd_from_f32<DT>(pvd_to_f32<DT>(o[e + f]) * pvd_act_grad(z4[f], P.act));
+                    for (int f = 0; f < 4; ++f) o[e + f] = pvd_from_f32<DT>(pvd_to_f32<DT>(o[e + f]) * d4[f]);
                 }
             }
             return;
@@ -332,4 +349,259 @@ template <int DT> __global__ __launch_bounds__(256) void pvk_dense_bwd_tile(cons
     __syncthreads();
     if (g == 0 && n < J.n && J.dbias)
         static_cast<T*>(J.dbias)[n] = pvd_from_f32<DT>((red[c] + red[64 + c]) + (red[128 + c] + red[192 + c]));
+}
+
+// ---------------------------------------------------------------------------------------------
+// Large products, step 1: operands that the product kernel below cannot read as they are -- rows not contiguous along the
+// contraction, not aligned to sixteen bytes, or a contraction that is no multiple of 128 bytes -- are laid out anew, and g is
+// formed from dy and z, once instead of once per tile: a source of R rows of C contiguous elements becomes [R][pad(C)]
+// and / or its transpose [C][pad(R)], zeros behind the end.  One launch for up to three sources; bound by memory.
+// ---------------------------------------------------------------------------------------------
+struct PvdPack {
+    const void* p;
+    int64_t R, C, ld;
+    const float* pre;  // g = p * act'(pre)
+    int64_t ldp;
+    int act, vec;      // vec: sixteen bytes of p (and of pre) at multiples of them can be read at once
+    void* same;        // [R][ld_same] or NULL
+    int64_t ld_same;
+    void* tran;        // [C][ld_tran] or NULL
+    int64_t ld_tran;
+    float* sums;       // [row tiles][C]: column sums of 64 rows each, or NULL
+    float* g32;        // [R][C] float32: g unrounded, or NULL
+    int rt, ct;        // tiles of 64 x 64
+};
+struct PvdPacks {
+    int n, first[4];
+    PvdPack job[3];
+};
+
+template <int DT> __global__ __launch_bounds__(256) void pvk_dense_pack(const PvdPacks P) {
+    typedef typename PvdType<DT>::T T;
+    enum { VEC = PvdType<DT>::VEC, PER = 64 / VEC, LD = 64 + (DT == PVD_F32 ? 1 : 2) };
+    __shared__ T tile[64 * LD];
+    __shared__ float colsum[4][64];
+    int j = 0;
+    while (j + 1 < P.n && (int)blockIdx.x >= P.first[j + 1]) ++j;
+    const PvdPack& J = P.job[j];
+    const int b = blockIdx.x - P.first[j], tid = threadIdx.x;
+    const int64_t r0 = (int64_t)(b / J.ct) * 64, c0 = (int64_t)(b % J.ct) * 64;
+    const T* p = static_cast<const T*>(J.p);
+    T* same = static_cast<T*>(J.same);
+    // runs of VEC columns: PER runs a row, 256 / PER rows at a time
+    const int run = tid % PER, row = tid / PER;
+    float sum[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) sum[e] = 0.f;
+#pragma unroll 2
+    for (int rr = row; rr < 64; rr += 256 / PER) {
+        const int64_t r = r0 + rr, c = c0 + run * VEC;
+        alignas(16) T v[VEC];
+        float f[VEC];
+        const bool whole = r < J.R && c + VEC <= J.C;
+        if (whole && J.vec) {
+            *reinterpret_cast<pvd_u32x4*>(v) = *reinterpret_cast<const pvd_u32x4*>(p + r * J.ld + c);
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[e] = r < J.R && c + e < J.C ? p[r * J.ld + c + e] : T(0);
+        }
+        if (J.sums || J.g32 || (J.pre && J.act != PVD_LINEAR)) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) f[e] = pvd_to_f32<DT>(v[e]);
+            if (J.pre && J.act != PVD_LINEAR) {
+                alignas(16) float z[VEC];
+                if (whole && J.vec) {
+#pragma unroll
+                    for (int e = 0; e < VEC; e += 4) *reinterpret_cast<pvd_f32x4*>(z + e) = *reinterpret_cast<const pvd_f32x4*>(J.pre + r * J.ldp + c + e);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) z[e] = r < J.R && c + e < J.C ? J.pre[r * J.ldp + c + e] : 0.f;
+                }
+#pragma unroll
+                for (int e = 0; e < VEC; e += 4) {
+                    const pvd_f32x4 d4 = pvd_act_grad4(*reinterpret_cast<const pvd_f32x4*>(z + e), J.act);
+#pragma unroll
+                    for (int i = e; i < e + 4; ++i) {
+                        f[i] = r < J.R && c + i < J.C ? f[i] * d4[i - e] : 0.f;
+                        v[i] = pvd_from_f32<DT>(f[i]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) sum[e] += f[e];
+            if (J.g32)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e)
+                    if (r < J.R && c + e < J.C) J.g32[r * J.C + c + e] = f[e];
+        }
+        if (same && r < J.R && c < J.ld_same) *reinterpret_cast<pvd_u32x4*>(same + r * J.ld_same + c) = *reinterpret_cast<const pvd_u32x4*>(v);
+        if (J.tran)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) tile[rr * LD + run * VEC + e] = v[e];
+    }
+    if (J.tran) {
+        T* tran = static_cast<T*>(J.tran);
+        __syncthreads();
+        for (int cc = row; cc < 64; cc += 256 / PER) {  // here a run is VEC rows of one column
+            const int64_t c = c0 + cc, r = r0 + run * VEC;
+            alignas(16) T v[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[e] = tile[(run * VEC + e) * LD + cc];
+            if (c < J.C && r < J.ld_tran) *reinterpret_cast<pvd_u32x4*>(tran + c * J.ld_tran + r) = *reinterpret_cast<const pvd_u32x4*>(v);
+        }
+    }
+    if (J.sums) {
+        // lanes of a wave that hold the same columns are PER apart
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            for (int o = PER; o < 64; o *= 2) sum[e] += __shfl_xor(sum[e], o);
+            if ((tid & 63) < PER) colsum[tid >> 6][run * VEC + e] = sum[e];
+        }
+        __syncthreads();
+        if (tid < 64 && c0 + tid < J.C)
+            J.sums[(r0 / 64) * J.C + c0 + tid] = (colsum[0][tid] + colsum[1][tid]) + (colsum[2][tid] + colsum[3][tid]);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Large products, step 2: both operands as rows of contraction, 128 bytes of every row a step.  LDS holds two steps: while the
+// matrix instructions work on one, the next arrives from memory (global_load_lds, no registers in between).  A row of 128
+// bytes is eight pieces of sixteen; piece c of row r lies at slot c ^ ((r >> 1) & 7), which spreads the sixteen rows a
+// quarter wave reads over all banks.  The direct loads write lane after lane, so the lanes choose their source accordingly.
+// Tiles are numbered so that the workgroups of one XCD (blockIdx % 8) work on neighbouring tiles and find each other's
+// operands in their L2.
+// ---------------------------------------------------------------------------------------------
+struct PvdNtJob {
+    const char *x, *w;      // [x_rows][steps * 128 bytes], row strides ldx, ldw in bytes
+    int64_t ldx, ldw;
+    int x_rows, w_rows;
+    int steps, per, splits; // steps of 128 bytes; of each piece; pieces
+    int mt, nt, band;       // tiles; rows of tiles that go together
+    PvdOut O;
+    float* part;            // splits > 1: [piece][rows][cols] float32
+};
+struct PvdNtJobs {
+    int n, first[3];        // first workgroup of each product; of the column sums behind them
+    PvdNtJob job[2];
+    const float* sums;      // [sum_tiles][sum_cols] -> dbias
+    int sum_tiles;
+    int64_t sum_cols;
+    void* dbias;
+};
+
+typedef const __attribute__((address_space(1))) void* pvd_gptr;
+typedef __attribute__((address_space(3))) void* pvd_lptr;
+
+template <int DT, int TM, int TN, int WM, int WN> struct PvdNt {
+    enum { WAVES = WM * WN, THREADS = 64 * WAVES, BUF = (TM + TN) * 128, LDS = 2 * BUF, FM = TM / WM / 16, FN = TN / WN / 16 };
+    enum { FITS = LDS / WAVES / 256, EPR = FITS < TM / WM ? FITS : TM / WM };  // rows of a wave's result that its share of LDS holds
+    static_assert(TM % (8 * WAVES) == 0 && TN % (8 * WAVES) == 0, "rows are loaded eight per wave");
+    static_assert(FN == 4 && EPR % 16 == 0 && (TM / WM) % EPR == 0, "a wave's result is 64 columns wide");
+
+    // rows [row0, row0 + ROWS) of one step into LDS; rows behind the end repeat the last one (their results are dropped)
+    template <int ROWS> static __device__ __forceinline__ void fetch(const char* p, int64_t ld, int rows, int row0, int64_t at, char* lds) {
+        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+#pragma unroll
+        for (int u = 0; u < ROWS / (8 * WM * WN); ++u) {
+            const int i = u * WM * WN + wave, r = min(row0 + 8 * i + (lane >> 3), rows - 1);
+            const int piece = (lane & 7) ^ (4 * (i & 1) | (lane >> 4));
+            __builtin_amdgcn_global_load_lds((pvd_gptr)(p + r * ld + at + piece * 16), (pvd_lptr)(lds + i * 1024), 16, 0, 0);
+        }
+    }
+    // every wave's direct loads are in LDS, and every wave is done reading what they replaced
+    static __device__ __forceinline__ void arrived() {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+    }
+    static __device__ __forceinline__ void same_wave() {  // LDS written by lanes of this wave is read by others of it
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+    static __device__ __forceinline__ pvd_u32x4 piece(const char* lds, int r, int c) {
+        return *reinterpret_cast<const pvd_u32x4*>(lds + r * 128 + ((c ^ ((r >> 1) & 7)) << 4));
+    }
+
+    static __device__ __forceinline__ void run(const PvdNtJob& J, int block, char* smem) {
+        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r16 = lane & 15, q = lane >> 4;
+        const int tiles = J.mt * J.nt, total = tiles * J.splits;
+        // an XCD's workgroups, block % 8 apart, take consecutive tiles
+        const int xcd = block & 7, each = total >> 3, more = total & 7;
+        int t = xcd * each + min(xcd, more) + (block >> 3);
+        const int pc = t / tiles;
+        t -= pc * tiles;
+        const int per_band = J.band * J.nt, bi = t / per_band, in = t - bi * per_band, bh = min(J.band, J.mt - bi * J.band);
+        const int m0 = (bi * J.band + in % bh) * TM, n0 = in / bh * TN;
+        const int s0 = pc * J.per, s1 = min(J.steps, s0 + J.per);
+        const int wm = (wave % WM) * (TM / WM), wn = (wave / WM) * (TN / WN);
+        pvd_f32x4 acc[FN][FM];
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+#pragma unroll
+            for (int k = 0; k < FM; ++k) acc[i][k] = (pvd_f32x4){0.f, 0.f, 0.f, 0.f};
+        fetch<TM>(J.x, J.ldx, J.x_rows, m0, (int64_t)s0 * 128, smem);
+        fetch<TN>(J.w, J.ldw, J.w_rows, n0, (int64_t)s0 * 128, smem + TM * 128);
+        arrived();
+        for (int s = s0; s < s1; ++s) {
+            const char* cur = smem + ((s - s0) & 1) * BUF;
+            if (s + 1 < s1) {
+                char* next = smem + ((s + 1 - s0) & 1) * BUF;
+                fetch<TM>(J.x, J.ldx, J.x_rows, m0, (int64_t)(s + 1) * 128, next);
+                fetch<TN>(J.w, J.ldw, J.w_rows, n0, (int64_t)(s + 1) * 128, next + TM * 128);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                pvd_u32x4 a[FN], b[FM];
+#pragma unroll
+                for (int i = 0; i < FN; ++i) a[i] = piece(cur + TM * 128, wn + 16 * i + r16, 4 * h + q);
+#pragma unroll
+                for (int k = 0; k < FM; ++k) b[k] = piece(cur, wm + 16 * k + r16, 4 * h + q);
+#pragma unroll
+                for (int k = 0; k < FM; ++k)
+#pragma unroll
+                    for (int i = 0; i < FN; ++i) acc[i][k] = pvd_mfma16<DT>(a[i], b[k], acc[i][k]);
+            }
+            arrived();
+        }
+        // through LDS, as many rows at a time as fit, so that sixteen lanes read and write 64 consecutive columns of a row; the
+        // sixteen pieces of a row of 64 floats are spread by the row's number
+        float* ep = reinterpret_cast<float*>(smem) + wave * EPR * 64;
+        const int er = lane >> 4, eu = lane & 15;
+#pragma unroll
+        for (int k0 = 0; k0 < FM; k0 += EPR / 16) {
+#pragma unroll
+            for (int k = 0; k < EPR / 16; ++k)
+#pragma unroll
+                for (int i = 0; i < FN; ++i)
+                    *reinterpret_cast<pvd_f32x4*>(ep + (16 * k + r16) * 64 + (((4 * i + q) ^ r16) << 2)) = acc[i][k0 + k];
+            same_wave();
+#pragma unroll 2
+            for (int row = er; row < EPR; row += 4) {
+                const pvd_f32x4 z = *reinterpret_cast<const pvd_f32x4*>(ep + row * 64 + ((eu ^ (row & 15)) << 2));
+                const int64_t m = m0 + wm + 16 * k0 + row, n = n0 + wn + 4 * eu;
+                if (J.splits == 1) pvd_finish4<DT>(J.O, m, n, z);
+                else if (m < J.O.rows)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (n + e < J.O.cols) J.part[(pc * J.O.rows + m) * J.O.cols + n + e] = z[e];
+            }
+            same_wave();
+        }
+    }
+};
+
+template <int DT, int TM, int TN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void pvk_dense_nt(const PvdNtJobs P) {
+    extern __shared__ __attribute__((aligned(1024))) char pvd_smem[];
+    typedef typename PvdType<DT>::T T;
+    const int b = blockIdx.x;
+    if (b < P.first[2]) {
+        const int j = b >= P.first[1];
+        return PvdNt<DT, TM, TN, WM, WN>::run(P.job[j], b - P.first[j], pvd_smem);
+    }
+    const int64_t c = (int64_t)(b - P.first[2]) * blockDim.x + threadIdx.x;
+    if (c >= P.sum_cols) return;
+    float s = 0.f;
+    for (int i = 0; i < P.sum_tiles; ++i) s += P.sums[i * P.sum_cols + c];
+    static_cast<T*>(P.dbias)[c] = pvd_from_f32<DT>(s);
 }

@@ -58,6 +58,17 @@ int check_weights(const void* w, int64_t k, int64_t n, int64_t sk, int64_t sn, i
     return refuse(-2, "w: neither rows nor columns are contiguous (strides %lld, %lld)", (long long)sk, (long long)sn);
 }
 
+int check_workspace(const char* what, const void* p, int64_t have, int64_t need) {
+    if (need == 0) return 0;
+    if (!p || have < need) return refuse(-8, "%s needs a workspace of %lld bytes (got %lld)", what, (long long)need, (long long)(p ? have : 0));
+    if (!aligned(p, 16)) return refuse(-2, "the workspace is not aligned to 16 bytes");
+    return 0;
+}
+int check_grid(int64_t blocks) {
+    if (blocks > 0x7fffffff) return refuse(-2, "%lld workgroups: the operands are too large for one launch", (long long)blocks);
+    return 0;
+}
+
 // an operand of the tile kernel: rows x K, and whether sixteen bytes along its unit stride can be read at once
 PvdOperand operand(const void* p, int64_t rows, int64_t cols_k, int64_t sr, int64_t sk, int size) {
     PvdOperand o{};
@@ -113,6 +124,183 @@ int launch_join(int dt, const PvdTileJob& J, hipStream_t s) {
     PVD_BY_TYPE(dt, hipLaunchKernelGGL(pvk_dense_join<D_>, dim3((unsigned)ceil_div(quads, 256)), dim3(256), 0, s, J.O, (const float*)J.part, J.splits));
     return launched("dense_join");
 }
+
+// ---- large products: operands laid out (pvk_dense_pack) where they have to be, then pvk_dense_nt ----
+// A product goes this way when both its sides fill most of a tile, its contraction gives the pipeline some steps, and the
+// whole is large enough to pay for the launches.
+bool is_large(int64_t m, int64_t n, int64_t k) { return m >= 96 && n >= 96 && k >= 64 && (double)m * n * k >= 1 << 25; }
+
+int64_t pad_k(int64_t k, int size) { return ceil_div(k, 128 / size) * (128 / size); }
+int64_t round256(int64_t b) { return ceil_div(b, 256) * 256; }
+
+// [rows][K] as the product kernel reads it: where it lies, or laid out in the workspace at `at`
+struct NtOperand {
+    const void* p;
+    int64_t ld;  // elements
+    int rows;
+};
+
+struct NtPlan {
+    PvdPacks packs{};
+    PvdNtJobs jobs{};
+    int64_t bytes = 0;     // workspace
+    int tm = 0;            // tile edge
+    bool need_pack = false;
+};
+
+struct NtBuilder {
+    int dt, size;
+    char* base;            // the workspace (NULL when only its size is asked for)
+    NtPlan plan;
+    NtBuilder(int dt_, void* ws) : dt(dt_), size(esize(dt_)), base(static_cast<char*>(ws)) {}
+
+    void* take(int64_t bytes) {
+        char* p = base + plan.bytes;
+        plan.bytes += round256(bytes);
+        return p;
+    }
+    PvdPack& source(const void* p, int64_t R, int64_t C, int64_t ld, const float* pre, int64_t ldp, int act) {
+        PvdPack& J = plan.packs.job[plan.packs.n++];
+        J = PvdPack{};
+        J.p = p; J.R = R; J.C = C; J.ld = ld;
+        J.pre = act == PVD_LINEAR ? nullptr : pre;
+        J.ldp = ldp; J.act = act;
+        J.vec = aligned(p, 16) && (R <= 1 || ld * size % 16 == 0) && (!J.pre || (aligned(pre, 16) && (R <= 1 || ldp % 4 == 0)));
+        return J;
+    }
+    NtOperand same(PvdPack& J) {
+        J.ld_same = pad_k(J.C, size);
+        J.same = take(J.R * J.ld_same * size);
+        return {J.same, J.ld_same, (int)J.R};
+    }
+    NtOperand transposed(PvdPack& J) {
+        J.ld_tran = pad_k(J.R, size);
+        J.tran = take(J.C * J.ld_tran * size);
+        return {J.tran, J.ld_tran, (int)J.C};
+    }
+    // an operand given as memory rows (R rows of C contiguous elements): by_rows: its rows are the product's, else its columns
+    NtOperand operand(const void* p, int64_t R, int64_t C, int64_t ld, bool by_rows) {
+        if (by_rows && C * size % 128 == 0 && aligned(p, 16) && (R <= 1 || ld * size % 16 == 0)) return {p, ld, (int)R};
+        PvdPack& J = source(p, R, C, ld, nullptr, 0, PVD_LINEAR);
+        return by_rows ? same(J) : transposed(J);
+    }
+    void product(const NtOperand& x, const NtOperand& w, int64_t K, const PvdOut& O) {
+        PvdNtJob& J = plan.jobs.job[plan.jobs.n++];
+        J = PvdNtJob{};
+        J.x = static_cast<const char*>(x.p); J.ldx = x.ld * size; J.x_rows = x.rows;
+        J.w = static_cast<const char*>(w.p); J.ldw = w.ld * size; J.w_rows = w.rows;
+        J.steps = (int)ceil_div(K * size, 128);
+        J.O = O;
+    }
+    // tile edge, pieces, numbering; call when all products are in
+    void finish() {
+        // 256 x 256 (two waves on a SIMD, the fewest LDS reads per product) when that leaves most of the chip's CUs a tile, else
+        // 128 x 128, two workgroups to a CU
+        int64_t big = 0;
+        for (int i = 0; i < plan.jobs.n; ++i) big += ceil_div(plan.jobs.job[i].O.rows, 256) * ceil_div(plan.jobs.job[i].O.cols, 256);
+        plan.tm = size == 2 && big >= 192 ? 256 : 128;
+        int64_t tiles = 0;
+        for (int i = 0; i < plan.jobs.n; ++i) {
+            PvdNtJob& J = plan.jobs.job[i];
+            J.mt = (int)ceil_div(J.O.rows, plan.tm);
+            J.nt = (int)ceil_div(J.O.cols, plan.tm);
+            tiles += (int64_t)J.mt * J.nt;
+        }
+        for (int i = 0; i < plan.jobs.n; ++i) {
+            PvdNtJob& J = plan.jobs.job[i];
+            // pieces of the contraction, eight steps at least, while the launch would leave CUs without a tile
+            const int64_t pieces = std::max<int64_t>(1, std::min<int64_t>(J.steps / 8, 512 / std::max<int64_t>(1, tiles)));
+            J.per = (int)ceil_div(J.steps, pieces);
+            J.splits = (int)ceil_div(J.steps, J.per);
+            // a band's rows of tiles keep their operand in an XCD's L2 while the columns pass by
+            J.band = (int)std::min<int64_t>(J.mt, std::max<int64_t>(4, (2 << 20) / ((int64_t)plan.tm * J.per * 128)));
+            if (J.splits > 1) J.part = static_cast<float*>(take((int64_t)J.splits * J.O.rows * J.O.cols * 4));
+        }
+        int at = 0;
+        for (int i = 0; i < plan.packs.n; ++i) {
+            PvdPack& J = plan.packs.job[i];
+            J.rt = (int)ceil_div(J.tran ? std::max(J.R, J.ld_tran) : J.R, 64);
+            J.ct = (int)ceil_div(J.same ? std::max(J.C, J.ld_same) : J.C, 64);
+            plan.packs.first[i] = at;
+            at += J.rt * J.ct;
+        }
+        plan.packs.first[plan.packs.n] = at;
+    }
+};
+
+template <int DT, int TM, int WM, int WN> int launch_nt(const PvdNtJobs& P, int blocks, hipStream_t s) {
+    typedef PvdNt<DT, TM, TM, WM, WN> K;
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(pvk_dense_nt<DT, TM, TM, WM, WN>),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, K::LDS);
+    if (e != hipSuccess) return refuse(-10, "%d bytes of LDS: %s", (int)K::LDS, hipGetErrorString(e));
+    hipLaunchKernelGGL((pvk_dense_nt<DT, TM, TM, WM, WN>), dim3(blocks), dim3(K::THREADS), K::LDS, s, P);
+    return launched("dense_nt");
+}
+int launch_large(int dt, NtPlan& plan, hipStream_t s) {
+    if (plan.packs.n) {
+        PVD_BY_TYPE(dt, hipLaunchKernelGGL(pvk_dense_pack<D_>, dim3(plan.packs.first[plan.packs.n]), dim3(256), 0, s, plan.packs));
+        if (int rc = launched("dense_pack")) return rc;
+    }
+    PvdNtJobs& P = plan.jobs;
+    int64_t at = 0;
+    for (int i = 0; i < 2; ++i) {
+        P.first[i] = (int)at;
+        if (i < P.n) at += (int64_t)P.job[i].mt * P.job[i].nt * P.job[i].splits;
+    }
+    P.first[2] = (int)at;
+    if (P.dbias) at += ceil_div(P.sum_cols, plan.tm == 256 ? 512 : 256);
+    if (int rc = check_grid(at)) return rc;
+    int rc;
+    if (dt == PVAE_F32) rc = launch_nt<PVD_F32, 128, 2, 2>(P, (int)at, s);
+    else if (dt == PVAE_BF16) rc = plan.tm == 256 ? launch_nt<PVD_BF16, 256, 2, 4>(P, (int)at, s) : launch_nt<PVD_BF16, 128, 2, 2>(P, (int)at, s);
+    else rc = plan.tm == 256 ? launch_nt<PVD_F16, 256, 2, 4>(P, (int)at, s) : launch_nt<PVD_F16, 128, 2, 2>(P, (int)at, s);
+    if (rc) return rc;
+    for (int i = 0; i < P.n; ++i)
+        if (P.job[i].splits > 1) {
+            PvdTileJob J{};
+            J.O = P.job[i].O;
+            J.part = P.job[i].part;
+            J.splits = P.job[i].splits;
+            if ((rc = launch_join(dt, J, s))) return rc;
+        }
+    return 0;
+}
+
+NtPlan large_dense(const pvae_dense_args& a, void* ws) {
+    NtBuilder B(a.dtype, ws);
+    const NtOperand x = B.operand(a.x, a.m, a.k, a.ldx, true);
+    const NtOperand w = a.w_sk == 1 ? B.operand(a.w, a.n, a.k, a.w_sn, true) : B.operand(a.w, a.k, a.n, a.w_sk, false);
+    B.product(x, w, a.k, output(a.m, a.n, a.y, a.ldy, a.bias, a.residual, a.ldr, a.pre, a.ldp, a.act, B.size));
+    B.finish();
+    return B.plan;
+}
+NtPlan large_bwd(const pvae_dense_bwd_args& a, void* ws) {
+    NtBuilder B(a.dtype, ws);
+    // g: as it lies for dx (contraction over n), transposed for dw (over m), its column sums, and unrounded if asked for
+    PvdPack& g = B.source(a.dy, a.m, a.n, a.lddy, a.pre, a.ldp, a.act);
+    NtOperand gx{}, gw{};
+    if (a.dx) gx = B.same(g);
+    if (a.dw) gw = B.transposed(g);
+    g.g32 = a.dpre;
+    if (a.dbias) {
+        g.sums = static_cast<float*>(B.take(ceil_div(a.m, 64) * a.n * 4));
+        B.plan.jobs.sums = g.sums;
+        B.plan.jobs.sum_tiles = (int)ceil_div(a.m, 64);
+        B.plan.jobs.sum_cols = a.n;
+        B.plan.jobs.dbias = a.dbias;
+    }
+    if (a.dx) {
+        const NtOperand w = a.w_sn == 1 ? B.operand(a.w, a.k, a.n, a.w_sk, true) : B.operand(a.w, a.n, a.k, a.w_sn, false);
+        B.product(gx, w, a.n, output(a.m, a.k, a.dx, a.lddx, nullptr, a.dx_add, a.ldadd, nullptr, 0, PVD_LINEAR, B.size));
+    }
+    if (a.dw) {
+        const NtOperand x = B.operand(a.x, a.m, a.k, a.ldx, false);
+        B.product(x, gw, a.m, output(a.k, a.n, a.dw, a.n, nullptr, nullptr, 0, nullptr, 0, PVD_LINEAR, B.size));
+    }
+    B.finish();
+    return B.plan;
+}
+bool bwd_is_large(const pvae_dense_bwd_args& a) { return (a.dx || a.dw) && is_large(a.m, a.n, a.k) && a.k >= 96; }
 
 PvdTileJob dense_job(const pvae_dense_args& a) {
     const int size = esize(a.dtype);
@@ -187,17 +375,6 @@ int check_dense_bwd(const pvae_dense_bwd_args* a) {
     if (a->dpre && !aligned(a->dpre, 4)) return refuse(-2, "dpre is not aligned to its elements");
     return 0;
 }
-int check_workspace(const char* what, const void* p, int64_t have, int64_t need) {
-    if (need == 0) return 0;
-    if (!p || have < need) return refuse(-8, "%s needs a workspace of %lld bytes (got %lld)", what, (long long)need, (long long)(p ? have : 0));
-    if (!aligned(p, 16)) return refuse(-2, "the workspace is not aligned to 16 bytes");
-    return 0;
-}
-int check_grid(int64_t blocks) {
-    if (blocks > 0x7fffffff) return refuse(-2, "%lld workgroups: the operands are too large for one launch", (long long)blocks);
-    return 0;
-}
-
 // ---- many tensors ----
 int check_tensors(const char* name, const pvae_tensor* t, int64_t count, bool tiles) {
     if (count < 0 || count > 65536) return refuse(-2, "%lld tensors: 0 .. 65536", (long long)count);
@@ -302,6 +479,7 @@ const char* pvae_ops_last_error(void) { return g_err; }
 
 int64_t pvae_dense_workspace(const pvae_dense_args* a) {
     if (check_dense(a) || a->m == 0 || a->n == 0) return 0;
+    if (is_large(a->m, a->n, a->k)) return large_dense(*a, nullptr).bytes;
     return tile_job_bytes(dense_job(*a));
 }
 
@@ -309,6 +487,11 @@ int pvae_dense(const pvae_dense_args* a, void* workspace, int64_t workspace_byte
     if (int rc = check_dense(a)) return rc;
     if (a->m == 0 || a->n == 0) return 0;
     hipStream_t s = static_cast<hipStream_t>(hip_stream);
+    if (is_large(a->m, a->n, a->k)) {
+        NtPlan plan = large_dense(*a, workspace);
+        if (int rc = check_workspace("pvae_dense", workspace, workspace_bytes, plan.bytes)) return rc;
+        return launch_large(a->dtype, plan, s);
+    }
     PvdTileJob J = dense_job(*a);
     if (int rc = check_workspace("pvae_dense", workspace, workspace_bytes, tile_job_bytes(J))) return rc;
     const int64_t blocks = (int64_t)J.mt * J.nt * J.splits;
@@ -321,12 +504,18 @@ int pvae_dense(const pvae_dense_args* a, void* workspace, int64_t workspace_byte
 
 int64_t pvae_dense_bwd_workspace(const pvae_dense_bwd_args* a) {
     if (check_dense_bwd(a)) return 0;
+    if (bwd_is_large(*a)) return large_bwd(*a, nullptr).bytes;
     return bwd_bytes(bwd_plan(*a));
 }
 
 int pvae_dense_bwd(const pvae_dense_bwd_args* a, void* workspace, int64_t workspace_bytes, void* hip_stream) {
     if (int rc = check_dense_bwd(a)) return rc;
     hipStream_t s = static_cast<hipStream_t>(hip_stream);
+    if (bwd_is_large(*a)) {
+        NtPlan plan = large_bwd(*a, workspace);
+        if (int rc = check_workspace("pvae_dense_bwd", workspace, workspace_bytes, plan.bytes)) return rc;
+        return launch_large(a->dtype, plan, s);
+    }
     BwdPlan p = bwd_plan(*a);
     if (int rc = check_workspace("pvae_dense_bwd", workspace, workspace_bytes, bwd_bytes(p))) return rc;
     const int64_t blocks = p.J.n_dx + p.J.n_dw + p.n_db;
