@@ -302,10 +302,15 @@ template <int DT> __global__ __launch_bounds__(256) void pvk_dense_join(const Pv
     if (i >= O.rows * quads) return;
     const int64_t m = i / quads, n = i % quads * 4;
     pvd_f32x4 z = {0.f, 0.f, 0.f, 0.f};
-    for (int p = 0; p < pieces; ++p)
+    if (O.cols % 4 == 0) {
+#pragma unroll 4
+        for (int p = 0; p < pieces; ++p) z += *reinterpret_cast<const pvd_f32x4*>(part + (p * O.rows + m) * O.cols + n);
+    } else {
+        for (int p = 0; p < pieces; ++p)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (n + e < O.cols) z[e] += part[(p * O.rows + m) * O.cols + n + e];
+            for (int e = 0; e < 4; ++e)
+                if (n + e < O.cols) z[e] += part[(p * O.rows + m) * O.cols + n + e];
+    }
     pvd_finish4<DT>(O, m, n, z);
 }
 
@@ -363,10 +368,10 @@ struct PvdPack {
     const float* pre;  // g = p * act'(pre)
     int64_t ldp;
     int act, vec;      // vec: sixteen bytes of p (and of pre) at multiples of them can be read at once
-    void* same;        // [R][ld_same] or NULL
-    int64_t ld_same;
-    void* tran;        // [C][ld_tran] or NULL
-    int64_t ld_tran;
+    void* same;        // [R][ld_same], the first w_same elements of a row filled, or NULL
+    int64_t ld_same, w_same;
+    void* tran;        // [C][ld_tran], w_tran of a row filled, or NULL
+    int64_t ld_tran, w_tran;
     float* sums;       // [row tiles][C]: column sums of 64 rows each, or NULL
     float* g32;        // [R][C] float32: g unrounded, or NULL
     int rt, ct;        // tiles of 64 x 64
@@ -434,7 +439,7 @@ template <int DT> __global__ __launch_bounds__(256) void pvk_dense_pack(const Pv
                 for (int e = 0; e < VEC; ++e)
                     if (r < J.R && c + e < J.C) J.g32[r * J.C + c + e] = f[e];
         }
-        if (same && r < J.R && c < J.ld_same) *reinterpret_cast<pvd_u32x4*>(same + r * J.ld_same + c) = *reinterpret_cast<const pvd_u32x4*>(v);
+        if (same && r < J.R && c < J.w_same) *reinterpret_cast<pvd_u32x4*>(same + r * J.ld_same + c) = *reinterpret_cast<const pvd_u32x4*>(v);
         if (J.tran)
 #pragma unroll
             for (int e = 0; e < VEC; ++e) tile[rr * LD + run * VEC + e] = v[e];
@@ -447,7 +452,7 @@ template <int DT> __global__ __launch_bounds__(256) void pvk_dense_pack(const Pv
             alignas(16) T v[VEC];
 #pragma unroll
             for (int e = 0; e < VEC; ++e) v[e] = tile[(run * VEC + e) * LD + cc];
-            if (c < J.C && r < J.ld_tran) *reinterpret_cast<pvd_u32x4*>(tran + c * J.ld_tran + r) = *reinterpret_cast<const pvd_u32x4*>(v);
+            if (c < J.C && r < J.w_tran) *reinterpret_cast<pvd_u32x4*>(tran + c * J.ld_tran + r) = *reinterpret_cast<const pvd_u32x4*>(v);
         }
     }
     if (J.sums) {
@@ -492,26 +497,98 @@ struct PvdNtJobs {
 typedef const __attribute__((address_space(1))) void* pvd_gptr;
 typedef __attribute__((address_space(3))) void* pvd_lptr;
 
-template <int DT, int TM, int TN, int WM, int WN> struct PvdNt {
-    enum { WAVES = WM * WN, THREADS = 64 * WAVES, BUF = (TM + TN) * 128, LDS = 2 * BUF, FM = TM / WM / 16, FN = TN / WN / 16 };
+// What follows the product for ROWS x 64 products of one wave in LDS (row r's piece u of four floats at slot u ^ (r & 15)):
+// rows m .., columns n ..; the residuals of several rows are asked for together.
+template <int DT, int ROWS> __device__ __forceinline__ void pvd_finish_rows(const PvdOut& O, int64_t m, int64_t n, const float* ep) {
+    typedef typename PvdType<DT>::T T;
+    const int lane = threadIdx.x & 63;
+    const T *bias = static_cast<const T*>(O.bias), *res = static_cast<const T*>(O.res);
+    T* y = static_cast<T*>(O.y);
+    const int rows = (int)max((int64_t)0, min((int64_t)ROWS, O.rows - m));
+    if (O.vec && (O.cols & 3) == 0) {  // sixteen lanes, four columns each, on a row
+        enum { G = ROWS / 4 < 8 ? ROWS / 4 : 8 };
+        const int er = lane >> 4, eu = lane & 15;
+        const int64_t c = n + 4 * eu;
+        if (c >= O.cols) return;
+        pvd_f32x4 b4 = {0.f, 0.f, 0.f, 0.f};
+        if (bias) b4 = pvm_load4(bias, DT, c);
+#pragma unroll 1
+        for (int r0 = er; r0 < rows; r0 += 4 * G) {
+            pvd_f32x4 r4[G];
+            if (res)
+#pragma unroll
+                for (int g = 0; g < G; ++g)
+                    if (r0 + 4 * g < rows) r4[g] = pvm_load4(res, DT, (m + r0 + 4 * g) * O.ldr + c);
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const int r = r0 + 4 * g;
+                if (r >= rows) break;
+                pvd_f32x4 z = *reinterpret_cast<const pvd_f32x4*>(ep + r * 64 + ((eu ^ (r & 15)) << 2));
+                z += b4;
+                if (O.pre) *reinterpret_cast<pvd_f32x4*>(O.pre + (m + r) * O.ldp + c) = z;
+                pvd_f32x4 o = pvd_act4(z, O.act);
+                if (res) o += r4[g];
+                pvm_store4(y, DT, (m + r) * O.ldy + c, o);
+            }
+        }
+        return;
+    }
+    // a lane per column: a row's 64 columns lie together whatever their alignment
+    const int64_t c = n + lane;
+    if (c >= O.cols) return;
+    const float b1 = bias ? pvd_to_f32<DT>(bias[c]) : 0.f;
+#pragma unroll 1
+    for (int r0 = 0; r0 < rows; r0 += 8) {
+        float r1[8];
+        if (res)
+#pragma unroll
+            for (int g = 0; g < 8; ++g)
+                if (r0 + g < rows) r1[g] = pvd_to_f32<DT>(res[(m + r0 + g) * O.ldr + c]);
+#pragma unroll
+        for (int g4 = 0; g4 < 8; g4 += 4) {
+            pvd_f32x4 z;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int r = r0 + g4 + g;
+                z[g] = ep[r * 64 + (((lane >> 2) ^ (r & 15)) << 2) + (lane & 3)] + b1;
+                if (O.pre && r < rows) O.pre[(m + r) * O.ldp + c] = z[g];
+            }
+            const pvd_f32x4 o = pvd_act4(z, O.act);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int r = r0 + g4 + g;
+                if (r < rows) y[(m + r) * O.ldy + c] = pvd_from_f32<DT>(res ? o[g] + r1[g4 + g] : o[g]);
+            }
+        }
+    }
+}
+
+// TM x TN: tile (x's rows, the weights' columns); WM x WN: waves; ST: steps that LDS holds
+template <int DT, int TM, int TN, int WM, int WN, int ST> struct PvdNt {
+    enum { WAVES = WM * WN, THREADS = 64 * WAVES, BUF = (TM + TN) * 128, LDS = ST * BUF, FM = TM / WM / 16, FN = TN / WN / 16 };
+    enum { LOADS = (TM + TN) / (8 * WAVES) };                          // direct loads of a wave per step
+    enum { GB = FM * FN <= 16 ? FM : 16 / FN, GROUPS = 2 * FM / GB };  // a step's matrix work: groups of FN x GB fragments
     enum { FITS = LDS / WAVES / 256, EPR = FITS < TM / WM ? FITS : TM / WM };  // rows of a wave's result that its share of LDS holds
     static_assert(TM % (8 * WAVES) == 0 && TN % (8 * WAVES) == 0, "rows are loaded eight per wave");
-    static_assert(FN == 4 && EPR % 16 == 0 && (TM / WM) % EPR == 0, "a wave's result is 64 columns wide");
+    static_assert(FN % 4 == 0 && EPR % 16 == 0 && (TM / WM) % EPR == 0, "a wave's result goes out in pieces 64 columns wide");
 
     // rows [row0, row0 + ROWS) of one step into LDS; rows behind the end repeat the last one (their results are dropped)
     template <int ROWS> static __device__ __forceinline__ void fetch(const char* p, int64_t ld, int rows, int row0, int64_t at, char* lds) {
         const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
 #pragma unroll
-        for (int u = 0; u < ROWS / (8 * WM * WN); ++u) {
-            const int i = u * WM * WN + wave, r = min(row0 + 8 * i + (lane >> 3), rows - 1);
+        for (int u = 0; u < ROWS / (8 * WAVES); ++u) {
+            const int i = u * WAVES + wave, r = min(row0 + 8 * i + (lane >> 3), rows - 1);
             const int piece = (lane & 7) ^ (4 * (i & 1) | (lane >> 4));
             __builtin_amdgcn_global_load_lds((pvd_gptr)(p + r * ld + at + piece * 16), (pvd_lptr)(lds + i * 1024), 16, 0, 0);
         }
     }
-    // every wave's direct loads are in LDS, and every wave is done reading what they replaced
-    static __device__ __forceinline__ void arrived() {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
+    // all but the last `steps` steps that this wave has asked for have arrived, its own reads of LDS too; then every wave's
+    static __device__ __forceinline__ void arrived(int steps) {
+        if (ST > 3 && steps >= 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * LOADS) : "memory");
+        else if (ST > 2 && steps >= 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
     }
     static __device__ __forceinline__ void same_wave() {  // LDS written by lanes of this wave is read by others of it
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -539,65 +616,101 @@ template <int DT, int TM, int TN, int WM, int WN> struct PvdNt {
         for (int i = 0; i < FN; ++i)
 #pragma unroll
             for (int k = 0; k < FM; ++k) acc[i][k] = (pvd_f32x4){0.f, 0.f, 0.f, 0.f};
-        fetch<TM>(J.x, J.ldx, J.x_rows, m0, (int64_t)s0 * 128, smem);
-        fetch<TN>(J.w, J.ldw, J.w_rows, n0, (int64_t)s0 * 128, smem + TM * 128);
-        arrived();
+        auto get = [&](int s, int slot) {
+            char* lds = smem + slot * BUF;
+            fetch<TM>(J.x, J.ldx, J.x_rows, m0, (int64_t)s * 128, lds);
+            fetch<TN>(J.w, J.ldw, J.w_rows, n0, (int64_t)s * 128, lds + TM * 128);
+        };
+        // The fragments of a group are read from LDS while the group before them is multiplied, a quarter into it -- across
+        // steps too: behind the first quarter of a step's last group the waves meet, and the next step's first fragments come
+        // in under the rest.
+        pvd_u32x4 a[2][FN], b[2][GB];
+        auto read = [&](const char* lds, int g) {
+            const int h = g / (FM / GB), k0 = g % (FM / GB) * GB;
+            if (k0 == 0)
+#pragma unroll
+                for (int i = 0; i < FN; ++i) a[h][i] = piece(lds + TM * 128, wn + 16 * i + r16, 4 * h + q);
+#pragma unroll
+            for (int k = 0; k < GB; ++k) b[g & 1][k] = piece(lds, wm + 16 * (k0 + k) + r16, 4 * h + q);
+        };
+        auto multiply = [&](int g, int from, int to) {
+            const int h = g / (FM / GB), k0 = g % (FM / GB) * GB;
+#pragma unroll
+            for (int u = from; u < to; ++u) {
+                const int k = u / FN, i = u % FN;
+                acc[i][k0 + k] = pvd_mfma16<DT>(a[h][i], b[g & 1][k], acc[i][k0 + k]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        enum { EACH = FN * GB, FIRST = EACH / 4 };
+#pragma unroll
+        for (int j = 0; j < ST - 1; ++j)
+            if (s0 + j < s1) get(s0 + j, j);
+        arrived(min(ST - 2, s1 - 1 - s0));
+        read(smem, 0);
+        int cur = 0;
         for (int s = s0; s < s1; ++s) {
-            const char* cur = smem + ((s - s0) & 1) * BUF;
+            const char* lds = smem + cur * BUF;
+            if (s + ST - 1 < s1) get(s + ST - 1, cur == 0 ? ST - 1 : cur - 1);
+#pragma unroll
+            for (int g = 0; g + 1 < GROUPS; ++g) {
+                multiply(g, 0, FIRST);
+                read(lds, g + 1);
+                __builtin_amdgcn_sched_barrier(0);
+                multiply(g, FIRST, EACH);
+            }
+            multiply(GROUPS - 1, 0, FIRST);
+            cur = cur + 1 == ST ? 0 : cur + 1;
             if (s + 1 < s1) {
-                char* next = smem + ((s + 1 - s0) & 1) * BUF;
-                fetch<TM>(J.x, J.ldx, J.x_rows, m0, (int64_t)(s + 1) * 128, next);
-                fetch<TN>(J.w, J.ldw, J.w_rows, n0, (int64_t)(s + 1) * 128, next + TM * 128);
+                arrived(min(ST - 2, s1 - 2 - s));
+                read(smem + cur * BUF, 0);
+                __builtin_amdgcn_sched_barrier(0);
             }
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                pvd_u32x4 a[FN], b[FM];
-#pragma unroll
-                for (int i = 0; i < FN; ++i) a[i] = piece(cur + TM * 128, wn + 16 * i + r16, 4 * h + q);
-#pragma unroll
-                for (int k = 0; k < FM; ++k) b[k] = piece(cur, wm + 16 * k + r16, 4 * h + q);
-#pragma unroll
-                for (int k = 0; k < FM; ++k)
-#pragma unroll
-                    for (int i = 0; i < FN; ++i) acc[i][k] = pvd_mfma16<DT>(a[i], b[k], acc[i][k]);
-            }
-            arrived();
+            multiply(GROUPS - 1, FIRST, EACH);
         }
+        arrived(0);
         // through LDS, as many rows at a time as fit, so that sixteen lanes read and write 64 consecutive columns of a row; the
         // sixteen pieces of a row of 64 floats are spread by the row's number
         float* ep = reinterpret_cast<float*>(smem) + wave * EPR * 64;
-        const int er = lane >> 4, eu = lane & 15;
 #pragma unroll
-        for (int k0 = 0; k0 < FM; k0 += EPR / 16) {
+        for (int kc = 0; kc < FM * 16 / EPR * (FN / 4); ++kc) {
+            const int k0 = kc / (FN / 4) * (EPR / 16), i0 = kc % (FN / 4) * 4;
 #pragma unroll
             for (int k = 0; k < EPR / 16; ++k)
 #pragma unroll
-                for (int i = 0; i < FN; ++i)
-                    *reinterpret_cast<pvd_f32x4*>(ep + (16 * k + r16) * 64 + (((4 * i + q) ^ r16) << 2)) = acc[i][k0 + k];
+                for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<pvd_f32x4*>(ep + (16 * k + r16) * 64 + (((4 * i + q) ^ r16) << 2)) = acc[i0 + i][k0 + k];
             same_wave();
-#pragma unroll 2
-            for (int row = er; row < EPR; row += 4) {
-                const pvd_f32x4 z = *reinterpret_cast<const pvd_f32x4*>(ep + row * 64 + ((eu ^ (row & 15)) << 2));
-                const int64_t m = m0 + wm + 16 * k0 + row, n = n0 + wn + 4 * eu;
-                if (J.splits == 1) pvd_finish4<DT>(J.O, m, n, z);
-                else if (m < J.O.rows)
+            const int64_t m = m0 + wm + 16 * k0, n = n0 + wn + 16 * i0;
+            if (J.splits == 1) {
+                pvd_finish_rows<DT, EPR>(J.O, m, n, ep);
+            } else {
+                for (int row = lane >> 4; row < EPR && m + row < J.O.rows; row += 4) {
+                    const int u = lane & 15;
+                    const pvd_f32x4 z = *reinterpret_cast<const pvd_f32x4*>(ep + row * 64 + ((u ^ (row & 15)) << 2));
+                    float* d = J.part + (pc * J.O.rows + m + row) * J.O.cols + n + 4 * u;
+                    if (J.O.cols % 4 == 0) {
+                        if (n + 4 * u < J.O.cols) *reinterpret_cast<pvd_f32x4*>(d) = z;
+                    } else {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (n + e < J.O.cols) J.part[(pc * J.O.rows + m) * J.O.cols + n + e] = z[e];
+                        for (int e = 0; e < 4; ++e)
+                            if (n + 4 * u + e < J.O.cols) d[e] = z[e];
+                    }
+                }
             }
             same_wave();
         }
     }
 };
 
-template <int DT, int TM, int TN, int WM, int WN>
+template <int DT, int TM, int TN, int WM, int WN, int ST>
 __global__ __launch_bounds__(64 * WM * WN) void pvk_dense_nt(const PvdNtJobs P) {
     extern __shared__ __attribute__((aligned(1024))) char pvd_smem[];
     typedef typename PvdType<DT>::T T;
     const int b = blockIdx.x;
     if (b < P.first[2]) {
         const int j = b >= P.first[1];
-        return PvdNt<DT, TM, TN, WM, WN>::run(P.job[j], b - P.first[j], pvd_smem);
+        return PvdNt<DT, TM, TN, WM, WN, ST>::run(P.job[j], b - P.first[j], pvd_smem);
     }
     const int64_t c = (int64_t)(b - P.first[2]) * blockDim.x + threadIdx.x;
     if (c >= P.sum_cols) return;

@@ -16,6 +16,7 @@
 enum { PVM_MAXT = 48, PVM_THREADS = 256, PVM_CHUNK = 8192, PVM_PARTS = 2048 };
 
 typedef float pvm_f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned short pvm_u16x8 __attribute__((ext_vector_type(8)));
 typedef unsigned short pvm_u16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 pvm_f16x4 __attribute__((ext_vector_type(4)));
 
@@ -29,7 +30,7 @@ struct PvmTab {  // elements [0, n) of tensor t are chunks first[t] .. first[t +
     int64_t n[PVM_MAXT];
     int tile[PVM_MAXT];            // pvae_tensor.tile of b, m and v
     unsigned char dt[PVM_MAXT];    // type of a
-    unsigned char vec[PVM_MAXT];   // every pointer is aligned for four elements
+    unsigned char vec[PVM_MAXT];   // every pointer is aligned to sixteen bytes
 };
 
 __device__ __forceinline__ float pvm_bf16(unsigned short u) { return __uint_as_float((unsigned)u << 16); }
@@ -68,6 +69,26 @@ __device__ __forceinline__ void pvm_store4(void* p, int dt, int64_t i, pvm_f32x4
             (pvm_f16x4){(_Float16)x.x, (_Float16)x.y, (_Float16)x.z, (_Float16)x.w};
 }
 
+// sixteen bytes of a tensor and what they hold
+template <int DT> struct PvmVec { enum { N = 8 }; typedef pvm_u16x8 V; };
+template <> struct PvmVec<0> { enum { N = 4 }; typedef pvm_f32x4 V; };
+template <int DT> __device__ __forceinline__ float pvm_get(typename PvmVec<DT>::V v, int e) {
+    if constexpr (DT == 0) return v[e];
+    else if constexpr (DT == 1) return pvm_bf16(v[e]);
+    else return (float)__builtin_bit_cast(_Float16, (unsigned short)v[e]);
+}
+template <int DT> __device__ __forceinline__ void pvm_set(typename PvmVec<DT>::V& v, int e, float x) {
+    if constexpr (DT == 0) v[e] = x;
+    else if constexpr (DT == 1) v[e] = pvm_to_bf16(x);
+    else v[e] = __builtin_bit_cast(unsigned short, (_Float16)x);
+}
+#define PVM_BY_TYPE(dt, CALL)                                   \
+    switch (dt) {                                               \
+        case 0: { constexpr int D_ = 0; CALL; } break;          \
+        case 1: { constexpr int D_ = 1; CALL; } break;          \
+        default: { constexpr int D_ = 2; CALL; } break;         \
+    }
+
 __device__ __forceinline__ int pvm_find(const PvmTab& T, int chunk) {  // the tensor of a chunk: first[t] <= chunk < first[t + 1]
     int lo = 0, hi = T.count - 1;
     while (lo < hi) {
@@ -90,26 +111,52 @@ __device__ __forceinline__ double pvm_block_sum(double s) {
     return a;
 }
 
+// the sum of squares of a whole chunk (all its loads under way together) or of the end of a tensor
+template <int DT> __device__ __forceinline__ double pvm_sumsq_chunk(const void* a, int64_t i0, int64_t i1, bool vec) {
+    typedef typename PvmVec<DT>::V V;
+    enum { N = PvmVec<DT>::N, LOADS = PVM_CHUNK / N / PVM_THREADS };
+    double s = 0.0;
+    int64_t i = i0 + threadIdx.x;
+    if (vec) {
+        const V* p = reinterpret_cast<const V*>(static_cast<const char*>(a) + i0 * (16 / N)) + threadIdx.x;
+        if (i1 - i0 == PVM_CHUNK) {
+            V v[LOADS];
+#pragma unroll
+            for (int u = 0; u < LOADS; ++u) v[u] = p[u * PVM_THREADS];
+#pragma unroll
+            for (int u = 0; u < LOADS; ++u)
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    const double x = pvm_get<DT>(v[u], e);
+                    s = fma(x, x, s);
+                }
+            return s;
+        }
+        const int whole = (int)(i1 - i0) / N;
+        for (int u = threadIdx.x; u < whole; u += PVM_THREADS, p += PVM_THREADS) {
+            const V v = *p;
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const double x = pvm_get<DT>(v, e);
+                s = fma(x, x, s);
+            }
+        }
+        i += (int64_t)whole * N;
+    }
+    for (; i < i1; i += PVM_THREADS) {
+        const double x = pvm_load1(a, DT, i);
+        s = fma(x, x, s);
+    }
+    return s;
+}
+
 __global__ __launch_bounds__(PVM_THREADS) void pvk_sumsq(const PvmTab T, double* __restrict__ part) {
     const int chunks = T.first[T.count];
     double s = 0.0;
     for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
-        const int t = pvm_find(T, c), dt = T.dt[t];
-        const void* a = T.a[t];
+        const int t = pvm_find(T, c);
         const int64_t i0 = (int64_t)(c - T.first[t]) * PVM_CHUNK, i1 = min(T.n[t], i0 + PVM_CHUNK);
-        int64_t i = i0;
-        if (T.vec[t]) {
-            for (i = i0 + 4 * threadIdx.x; i + 3 < i1; i += 4 * PVM_THREADS) {
-                const pvm_f32x4 x = pvm_load4(a, dt, i);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s = fma((double)x[e], (double)x[e], s);
-            }
-            i = i0 + ((i1 - i0) & ~(int64_t)3);
-        }
-        for (i += threadIdx.x; i < i1; i += PVM_THREADS) {
-            const double x = pvm_load1(a, dt, i);
-            s = fma(x, x, s);
-        }
+        PVM_BY_TYPE(T.dt[t], s += pvm_sumsq_chunk<D_>(T.a[t], i0, i1, T.vec[t]));
     }
     s = pvm_block_sum(s);
     if (threadIdx.x == 0) part[blockIdx.x] = s;
@@ -132,6 +179,34 @@ __global__ __launch_bounds__(PVM_THREADS) void pvk_norm_final(const double* __re
     if (threadIdx.x == 0) *norm = (float)n;
 }
 
+template <int DT> __device__ __forceinline__ void pvm_scale_chunk(const void* a, void* b, int64_t i0, int64_t i1, bool vec, float s) {
+    typedef typename PvmVec<DT>::V V;
+    enum { N = PvmVec<DT>::N, LOADS = PVM_CHUNK / N / PVM_THREADS };
+    int64_t i = i0 + threadIdx.x;
+    if (vec) {
+        const V* p = reinterpret_cast<const V*>(static_cast<const char*>(a) + i0 * (16 / N)) + threadIdx.x;
+        V* q = reinterpret_cast<V*>(static_cast<char*>(b) + i0 * (16 / N)) + threadIdx.x;
+        auto scaled = [&](V v) {
+            V o;
+#pragma unroll
+            for (int e = 0; e < N; ++e) pvm_set<DT>(o, e, pvm_get<DT>(v, e) * s);
+            return o;
+        };
+        if (i1 - i0 == PVM_CHUNK) {
+            V v[LOADS];
+#pragma unroll
+            for (int u = 0; u < LOADS; ++u) v[u] = p[u * PVM_THREADS];
+#pragma unroll
+            for (int u = 0; u < LOADS; ++u) q[u * PVM_THREADS] = scaled(v[u]);
+            return;
+        }
+        const int whole = (int)(i1 - i0) / N;
+        for (int u = threadIdx.x; u < whole; u += PVM_THREADS, p += PVM_THREADS, q += PVM_THREADS) *q = scaled(*p);
+        i += (int64_t)whole * N;
+    }
+    for (; i < i1; i += PVM_THREADS) pvm_store1(b, DT, i, pvm_load1(a, DT, i) * s);
+}
+
 __global__ __launch_bounds__(PVM_THREADS) void pvk_clip_apply(const PvmTab T, const double* __restrict__ part, int nparts, double max_norm,
                                                               float* __restrict__ norm) {
     const double n = pvm_norm(part, nparts);
@@ -139,17 +214,10 @@ __global__ __launch_bounds__(PVM_THREADS) void pvk_clip_apply(const PvmTab T, co
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
     const int chunks = T.first[T.count];
     for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
-        const int t = pvm_find(T, c), dt = T.dt[t];
-        const void* a = T.a[t];
-        void* b = T.b[t];
-        if (s == 1.f && a == b) continue;  // in place and within the bound: every value stays as it is
+        const int t = pvm_find(T, c);
+        if (s == 1.f && T.a[t] == T.b[t]) continue;  // in place and within the bound: every value stays as it is
         const int64_t i0 = (int64_t)(c - T.first[t]) * PVM_CHUNK, i1 = min(T.n[t], i0 + PVM_CHUNK);
-        int64_t i = i0;
-        if (T.vec[t]) {
-            for (i = i0 + 4 * threadIdx.x; i + 3 < i1; i += 4 * PVM_THREADS) pvm_store4(b, dt, i, pvm_load4(a, dt, i) * s);
-            i = i0 + ((i1 - i0) & ~(int64_t)3);
-        }
-        for (i += threadIdx.x; i < i1; i += PVM_THREADS) pvm_store1(b, dt, i, pvm_load1(a, dt, i) * s);
+        PVM_BY_TYPE(T.dt[t], pvm_scale_chunk<D_>(T.a[t], T.b[t], i0, i1, T.vec[t], s));
     }
 }
 
@@ -178,6 +246,45 @@ __device__ __forceinline__ void pvm_adam1(float& p, float& m, float& v, float g,
     p -= alpha * m / (sqrtf(v) + eps);
 }
 
+// four elements at a time, two groups under way: parameters and moments pass once, past the caches
+template <int DT> __device__ __forceinline__ void pvm_adam_chunk(const void* a, float* p, float* m, float* v, int tile, int64_t i0, int64_t i1, bool vec,
+                                                                 float s, float alpha, float c1, float c2, float eps) {
+    auto at = [&](int64_t i) { return tile ? i + i / tile * 2 * tile : i; };  // i / tile * 3 tile + i % tile
+    int64_t i = i0 + threadIdx.x;
+    if (vec) {
+        const int whole = (int)(i1 - i0) / 4;
+        auto step = [&](pvm_f32x4 g, int64_t j, pvm_f32x4 p4, pvm_f32x4 m4, pvm_f32x4 v4) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float pe = p4[e], me = m4[e], ve = v4[e];
+                pvm_adam1(pe, me, ve, g[e] * s, alpha, c1, c2, eps);
+                p4[e] = pe; m4[e] = me; v4[e] = ve;
+            }
+            __builtin_nontemporal_store(p4, reinterpret_cast<pvm_f32x4*>(p + j));
+            __builtin_nontemporal_store(m4, reinterpret_cast<pvm_f32x4*>(m + j));
+            __builtin_nontemporal_store(v4, reinterpret_cast<pvm_f32x4*>(v + j));
+        };
+        auto ld = [](const float* q) { return __builtin_nontemporal_load(reinterpret_cast<const pvm_f32x4*>(q)); };
+        int u = threadIdx.x;
+        for (; u + PVM_THREADS < whole; u += 2 * PVM_THREADS) {
+            const int64_t e0 = i0 + 4 * u, e1 = e0 + 4 * PVM_THREADS, j0 = at(e0), j1 = at(e1);
+            const pvm_f32x4 g0 = pvm_load4(a, DT, e0), p0 = ld(p + j0), m0 = ld(m + j0), v0 = ld(v + j0);
+            const pvm_f32x4 g1 = pvm_load4(a, DT, e1), p1 = ld(p + j1), m1 = ld(m + j1), v1 = ld(v + j1);
+            step(g0, j0, p0, m0, v0);
+            step(g1, j1, p1, m1, v1);
+        }
+        for (; u < whole; u += PVM_THREADS) {
+            const int64_t e0 = i0 + 4 * u, j0 = at(e0);
+            step(pvm_load4(a, DT, e0), j0, ld(p + j0), ld(m + j0), ld(v + j0));
+        }
+        i += (int64_t)whole * 4;
+    }
+    for (; i < i1; i += PVM_THREADS) {
+        const int64_t j = at(i);
+        pvm_adam1(p[j], m[j], v[j], pvm_load1(a, DT, i) * s, alpha, c1, c2, eps);
+    }
+}
+
 __global__ __launch_bounds__(PVM_THREADS) void pvk_adam_apply(const PvmTab T, const double* __restrict__ part, int nparts, double clip_norm,
                                                               float* __restrict__ norm, const PvmAdam A) {
     float s = 1.f;
@@ -189,33 +296,8 @@ __global__ __launch_bounds__(PVM_THREADS) void pvk_adam_apply(const PvmTab T, co
     const float alpha = pvm_alpha(A), c1 = (float)(1.0 - A.b1), c2 = (float)(1.0 - A.b2), eps = A.eps;
     const int chunks = T.first[T.count];
     for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
-        const int t = pvm_find(T, c), dt = T.dt[t], tile = T.tile[t];
-        const void* a = T.a[t];
-        float *p = static_cast<float*>(T.b[t]), *m = T.m[t], *v = T.v[t];
+        const int t = pvm_find(T, c);
         const int64_t i0 = (int64_t)(c - T.first[t]) * PVM_CHUNK, i1 = min(T.n[t], i0 + PVM_CHUNK);
-        auto at = [&](int64_t i) { return tile ? i + i / tile * 2 * tile : i; };  // i / tile * 3 tile + i % tile
-        int64_t i = i0;
-        if (T.vec[t]) {
-            for (i = i0 + 4 * threadIdx.x; i + 3 < i1; i += 4 * PVM_THREADS) {
-                const pvm_f32x4 g = pvm_load4(a, dt, i) * s;
-                const int64_t j = at(i);
-                pvm_f32x4 p4 = *reinterpret_cast<pvm_f32x4*>(p + j), m4 = *reinterpret_cast<pvm_f32x4*>(m + j),
-                          v4 = *reinterpret_cast<pvm_f32x4*>(v + j);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float pe = p4[e], me = m4[e], ve = v4[e];
-                    pvm_adam1(pe, me, ve, g[e], alpha, c1, c2, eps);
-                    p4[e] = pe; m4[e] = me; v4[e] = ve;
-                }
-                *reinterpret_cast<pvm_f32x4*>(p + j) = p4;
-                *reinterpret_cast<pvm_f32x4*>(m + j) = m4;
-                *reinterpret_cast<pvm_f32x4*>(v + j) = v4;
-            }
-            i = i0 + ((i1 - i0) & ~(int64_t)3);
-        }
-        for (i += threadIdx.x; i < i1; i += PVM_THREADS) {
-            const int64_t j = at(i);
-            pvm_adam1(p[j], m[j], v[j], pvm_load1(a, dt, i) * s, alpha, c1, c2, eps);
-        }
+        PVM_BY_TYPE(T.dt[t], pvm_adam_chunk<D_>(T.a[t], static_cast<float*>(T.b[t]), T.m[t], T.v[t], T.tile[t], i0, i1, T.vec[t], s, alpha, c1, c2, eps));
     }
 }

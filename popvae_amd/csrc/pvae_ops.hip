@@ -5,6 +5,7 @@
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
+#include <cstdlib>
 #include <new>
 #include <string>
 #include <utility>
@@ -145,7 +146,7 @@ struct NtPlan {
     PvdNtJobs jobs{};
     int64_t bytes = 0;     // workspace
     int tm = 0;            // tile edge
-    bool need_pack = false;
+    bool deep = false;
 };
 
 struct NtBuilder {
@@ -168,13 +169,17 @@ struct NtBuilder {
         J.vec = aligned(p, 16) && (R <= 1 || ld * size % 16 == 0) && (!J.pre || (aligned(pre, 16) && (R <= 1 || ldp % 4 == 0)));
         return J;
     }
+    // a row stride of a laid-out operand: an odd multiple of 128 bytes, so that a tile's rows lie in all of the L2's channels
+    int64_t spread(int64_t k) const { return k * size / 128 % 2 ? k : k + 128 / size; }
     NtOperand same(PvdPack& J) {
-        J.ld_same = pad_k(J.C, size);
+        J.w_same = pad_k(J.C, size);
+        J.ld_same = spread(J.w_same);
         J.same = take(J.R * J.ld_same * size);
         return {J.same, J.ld_same, (int)J.R};
     }
     NtOperand transposed(PvdPack& J) {
-        J.ld_tran = pad_k(J.R, size);
+        J.w_tran = pad_k(J.R, size);
+        J.ld_tran = spread(J.w_tran);
         J.tran = take(J.C * J.ld_tran * size);
         return {J.tran, J.ld_tran, (int)J.C};
     }
@@ -194,33 +199,37 @@ struct NtBuilder {
     }
     // tile edge, pieces, numbering; call when all products are in
     void finish() {
-        // 256 x 256 (two waves on a SIMD, the fewest LDS reads per product) when that leaves most of the chip's CUs a tile, else
-        // 128 x 128, two workgroups to a CU
-        int64_t big = 0;
-        for (int i = 0; i < plan.jobs.n; ++i) big += ceil_div(plan.jobs.job[i].O.rows, 256) * ceil_div(plan.jobs.job[i].O.cols, 256);
-        plan.tm = size == 2 && big >= 192 ? 256 : 128;
-        int64_t tiles = 0;
+        auto tile_steps = [&](int tm) {
+            int64_t n = 0;
+            for (int i = 0; i < plan.jobs.n; ++i) {
+                const PvdNtJob& J = plan.jobs.job[i];
+                n += ceil_div(J.O.rows, tm) * ceil_div(J.O.cols, tm) * J.steps;
+            }
+            return n;
+        };
+        // 128 x 128 with eight waves, two workgroups to a CU.  float32 takes 64 x 64 (five to a CU) where 128 x 128 would give the
+        // CUs less than 40 steps each: matrix work is sixteen times slower there, and an uneven last round counts.
+        plan.tm = size == 4 && tile_steps(128) < 256 * 40 ? 64 : 128;
+        const int64_t per = std::max<int64_t>(8, ceil_div(tile_steps(plan.tm), plan.tm == 64 ? 1024 : 512));
+        int64_t wgs = 0;
         for (int i = 0; i < plan.jobs.n; ++i) {
             PvdNtJob& J = plan.jobs.job[i];
             J.mt = (int)ceil_div(J.O.rows, plan.tm);
             J.nt = (int)ceil_div(J.O.cols, plan.tm);
-            tiles += (int64_t)J.mt * J.nt;
-        }
-        for (int i = 0; i < plan.jobs.n; ++i) {
-            PvdNtJob& J = plan.jobs.job[i];
-            // pieces of the contraction, eight steps at least, while the launch would leave CUs without a tile
-            const int64_t pieces = std::max<int64_t>(1, std::min<int64_t>(J.steps / 8, 512 / std::max<int64_t>(1, tiles)));
-            J.per = (int)ceil_div(J.steps, pieces);
-            J.splits = (int)ceil_div(J.steps, J.per);
+            // a contraction much longer than a CU's fair share is cut into pieces (each costs a write and a read of the result)
+            J.per = J.steps > 2 * per ? (int)ceil_div(J.steps, ceil_div(J.steps, per)) : std::max(1, J.steps);
+            J.splits = std::max(1, (int)ceil_div(J.steps, J.per));
             // a band's rows of tiles keep their operand in an XCD's L2 while the columns pass by
-            J.band = (int)std::min<int64_t>(J.mt, std::max<int64_t>(4, (2 << 20) / ((int64_t)plan.tm * J.per * 128)));
+            J.band = (int)std::min<int64_t>(J.mt, std::max<int64_t>(4, (1 << 20) / ((int64_t)plan.tm * J.per * 128)));
             if (J.splits > 1) J.part = static_cast<float*>(take((int64_t)J.splits * J.O.rows * J.O.cols * 4));
+            wgs += (int64_t)J.mt * J.nt * J.splits;
         }
+        plan.deep = plan.tm == 128 && wgs <= 256;  // one workgroup to a CU: four steps in LDS instead of two
         int at = 0;
         for (int i = 0; i < plan.packs.n; ++i) {
             PvdPack& J = plan.packs.job[i];
-            J.rt = (int)ceil_div(J.tran ? std::max(J.R, J.ld_tran) : J.R, 64);
-            J.ct = (int)ceil_div(J.same ? std::max(J.C, J.ld_same) : J.C, 64);
+            J.rt = (int)ceil_div(J.tran ? J.w_tran : J.R, 64);
+            J.ct = (int)ceil_div(J.same ? J.w_same : J.C, 64);
             plan.packs.first[i] = at;
             at += J.rt * J.ct;
         }
@@ -228,12 +237,12 @@ struct NtBuilder {
     }
 };
 
-template <int DT, int TM, int WM, int WN> int launch_nt(const PvdNtJobs& P, int blocks, hipStream_t s) {
-    typedef PvdNt<DT, TM, TM, WM, WN> K;
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(pvk_dense_nt<DT, TM, TM, WM, WN>),
+template <int DT, int TM, int WM, int WN, int ST> int launch_nt(const PvdNtJobs& P, int blocks, hipStream_t s) {
+    typedef PvdNt<DT, TM, TM, WM, WN, ST> K;
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(pvk_dense_nt<DT, TM, TM, WM, WN, ST>),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, K::LDS);
     if (e != hipSuccess) return refuse(-10, "%d bytes of LDS: %s", (int)K::LDS, hipGetErrorString(e));
-    hipLaunchKernelGGL((pvk_dense_nt<DT, TM, TM, WM, WN>), dim3(blocks), dim3(K::THREADS), K::LDS, s, P);
+    hipLaunchKernelGGL((pvk_dense_nt<DT, TM, TM, WM, WN, ST>), dim3(blocks), dim3(K::THREADS), K::LDS, s, P);
     return launched("dense_nt");
 }
 int launch_large(int dt, NtPlan& plan, hipStream_t s) {
@@ -248,12 +257,12 @@ int launch_large(int dt, NtPlan& plan, hipStream_t s) {
         if (i < P.n) at += (int64_t)P.job[i].mt * P.job[i].nt * P.job[i].splits;
     }
     P.first[2] = (int)at;
-    if (P.dbias) at += ceil_div(P.sum_cols, plan.tm == 256 ? 512 : 256);
+    if (P.dbias) at += ceil_div(P.sum_cols, plan.tm == 128 ? 512 : 256);
     if (int rc = check_grid(at)) return rc;
-    int rc;
-    if (dt == PVAE_F32) rc = launch_nt<PVD_F32, 128, 2, 2>(P, (int)at, s);
-    else if (dt == PVAE_BF16) rc = plan.tm == 256 ? launch_nt<PVD_BF16, 256, 2, 4>(P, (int)at, s) : launch_nt<PVD_BF16, 128, 2, 2>(P, (int)at, s);
-    else rc = plan.tm == 256 ? launch_nt<PVD_F16, 256, 2, 4>(P, (int)at, s) : launch_nt<PVD_F16, 128, 2, 2>(P, (int)at, s);
+    int rc = 0;
+    const int blocks = (int)at;
+    if (plan.tm == 64) rc = launch_nt<PVD_F32, 64, 4, 1, 2>(P, blocks, s);
+    else PVD_BY_TYPE(dt, (rc = plan.deep ? launch_nt<D_, 128, 4, 2, 4>(P, blocks, s) : launch_nt<D_, 128, 4, 2, 2>(P, blocks, s)));
     if (rc) return rc;
     for (int i = 0; i < P.n; ++i)
         if (P.job[i].splits > 1) {
@@ -427,7 +436,7 @@ template <typename Fill, typename Launch> int for_tables(const pvae_tensor* g, i
         T.a[c] = g[i].data;
         T.n[c] = g[i].n;
         T.dt[c] = (unsigned char)g[i].dtype;
-        T.vec[c] = aligned(g[i].data, 4 * esize(g[i].dtype));
+        T.vec[c] = aligned(g[i].data, 16);
         T.b[c] = nullptr;
         T.m[c] = T.v[c] = nullptr;
         T.tile[c] = 0;
@@ -571,7 +580,7 @@ int pvae_clip_by_global_norm(const pvae_tensor* g, const pvae_tensor* out, int64
             g, count,
             [&](PvmTab& T, int c, int64_t i) {
                 T.b[c] = out[i].data;
-                T.vec[c] = T.vec[c] && aligned(out[i].data, 4 * esize(out[i].dtype));
+                T.vec[c] = T.vec[c] && aligned(out[i].data, 16);
             },
             [&](PvmTab& T) {
                 hipLaunchKernelGGL(pvk_clip_apply, dim3(std::min(2048, T.first[T.count])), dim3(PVM_THREADS), 0, s, T, (const double*)part,
