@@ -296,22 +296,280 @@ template <int DT> __global__ __launch_bounds__(256) void pvk_dense_tile(const Pv
     pvd_tile_job<DT, false, false>(J, blockIdx.x, smem);
 }
 
-// the pieces of a split contraction, added in order, and what follows the product
-template <int DT> __global__ __launch_bounds__(256) void pvk_dense_join(const PvdOut O, const float* __restrict__ part, int pieces) {
-    const int64_t quads = (O.cols + 3) / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= O.rows * quads) return;
-    const int64_t m = i / quads, n = i % quads * 4;
+// ---------------------------------------------------------------------------------------------
+// The slim kernel, for few rows or results too small to give the chip 64 x 64 tiles: a workgroup of eight waves makes 32 rows
+// x 16 columns.  The waves take runs of the contraction in turn and read both operands straight from memory into the matrix
+// instruction's registers -- one round trip instead of one per LDS step, which is what such a call spends its time on --
+// and the eight partial results meet in LDS, added in order.
+// ---------------------------------------------------------------------------------------------
+enum { PVD_SM = 32, PVD_SN = 16, PVD_SW = 8 };
+
+// VEC elements of row `row` from k on, as a lane of the matrix instruction holds them; zeros outside
+template <int DT, bool GRAD> __device__ __forceinline__ pvd_u32x4 pvd_slim_load(const PvdOperand& P, int64_t row, int64_t k, int64_t k1) {
+    typedef typename PvdType<DT>::T T;
+    enum { VEC = PvdType<DT>::VEC };
+    alignas(16) T v[VEC];
+    const T* p = static_cast<const T*>(P.p) + row * P.sr + k * P.sk;
+    const bool grad = GRAD && P.act != PVD_LINEAR;
+    const float* z = grad ? P.pre + row * P.pr + k * P.pk : nullptr;
+    const bool in = row < P.rows;
+    if (P.sk == 1 && P.vec && in && k + VEC <= k1) {
+        *reinterpret_cast<pvd_u32x4*>(v) = *reinterpret_cast<const pvd_u32x4*>(p);
+    } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] = in && k + e < k1 ? p[e * P.sk] : T(0);
+    }
+    if (grad) {
+        alignas(16) float zz[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) zz[e] = in && k + e < k1 ? z[e * P.pk] : 0.f;
+#pragma unroll
+        for (int e = 0; e < VEC; e += 4) {
+            const pvd_f32x4 d = pvd_act_grad4(*reinterpret_cast<const pvd_f32x4*>(zz + e), P.act);
+#pragma unroll
+            for (int f = 0; f < 4; ++f) v[e + f] = pvd_from_f32<DT>(pvd_to_f32<DT>(v[e + f]) * d[f]);
+        }
+    }
+    return *reinterpret_cast<const pvd_u32x4*>(v);
+}
+
+template <int DT, bool GX, bool GW> __device__ __forceinline__ void pvd_slim_job(const PvdTileJob& J, int64_t block, float* red) {
+    enum { KS = 4 * PvdType<DT>::VEC, RUN = 2 };  // contraction of one matrix instruction group; groups under way per wave
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 15, q = lane >> 4;
+    const int64_t tiles = (int64_t)J.mt * J.nt;
+    const int piece = (int)(block / tiles);
+    const int64_t t = block % tiles, m0 = t / J.nt * PVD_SM, n0 = t % J.nt * PVD_SN;
+    const int64_t k0 = piece * J.kper, k1 = min(J.K, k0 + J.kper);
+    pvd_f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    for (int64_t k = k0 + wave * (RUN * KS); k < k1; k += PVD_SW * RUN * KS) {
+        pvd_u32x4 a[RUN], b[RUN][2];
+#pragma unroll
+        for (int u = 0; u < RUN; ++u) {
+            const int64_t kk = k + u * KS + q * PvdType<DT>::VEC;
+            a[u] = pvd_slim_load<DT, GW>(J.W, n0 + r, kk, k1);
+            b[u][0] = pvd_slim_load<DT, GX>(J.X, m0 + r, kk, k1);
+            b[u][1] = pvd_slim_load<DT, GX>(J.X, m0 + 16 + r, kk, k1);
+        }
+#pragma unroll
+        for (int u = 0; u < RUN; ++u)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) acc[j] = pvd_mfma16<DT>(a[u], b[u][j], acc[j]);
+    }
+    // red[wave][row][16 columns]
+#pragma unroll
+    for (int j = 0; j < 2; ++j) *reinterpret_cast<pvd_f32x4*>(red + ((wave * PVD_SM + 16 * j + r) * PVD_SN + 4 * q)) = acc[j];
+    __syncthreads();
+    if (tid >= PVD_SM * PVD_SN / 4) return;
+    const int row = tid >> 2, c = (tid & 3) * 4;
+    pvd_f32x4 z = *reinterpret_cast<const pvd_f32x4*>(red + row * PVD_SN + c);
+#pragma unroll
+    for (int w = 1; w < PVD_SW; ++w) z += *reinterpret_cast<const pvd_f32x4*>(red + (w * PVD_SM + row) * PVD_SN + c);
+    const int64_t m = m0 + row, n = n0 + c;
+    if (J.splits == 1) pvd_finish4<DT>(J.O, m, n, z);
+    else if (m < J.O.rows)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (n + e < J.O.cols) J.part[(piece * J.O.rows + m) * J.O.cols + n + e] = z[e];
+}
+
+template <int DT> __global__ __launch_bounds__(512) void pvk_dense_slim(const PvdTileJob J) {
+    __shared__ __attribute__((aligned(16))) float red[PVD_SW * PVD_SM * PVD_SN];
+    pvd_slim_job<DT, false, false>(J, blockIdx.x, red);
+}
+
+// ---------------------------------------------------------------------------------------------
+// The rows kernel, for up to eight rows (one point asked for an answer): the weights are read once, and that is its time.  A
+// lane holds sixteen bytes of a row of w -- or, unaligned, as many columns 64 apart -- and all rows' sums of those columns in
+// registers; x, as float32, comes from LDS.  The workgroup's eight waves, and pieces of the grid, split the contraction.
+// w^T (contiguous along the contraction): sixteen lanes share a column instead and add up at the end.
+// ---------------------------------------------------------------------------------------------
+struct PvdRowsJob {
+    const void* x;
+    int64_t ldx;
+    const void* w;
+    int64_t ldw;    // row stride of w, or of w^T
+    int64_t K;
+    PvdOut O;
+    int splits;
+    int64_t kper;   // contraction of a piece, at most PVD_RK
+    int blocks;     // workgroups of a piece
+    int vec;
+    float* part;
+};
+enum { PVD_RK = 1024, PVD_RW = 8 };
+
+// x's rows of [k0, k1) to LDS as float32, [row][k]; rows and k behind the end are zeros
+template <int DT, int R> __device__ __forceinline__ void pvd_rows_x(const PvdRowsJob& J, int64_t k0, int64_t k1, float* xs) {
+    typedef typename PvdType<DT>::T T;
+    const T* x = static_cast<const T*>(J.x);
+    for (int i = threadIdx.x; i < R * PVD_RK; i += 64 * PVD_RW) {
+        const int r = i / PVD_RK, k = i % PVD_RK;
+        if (k < ((k1 - k0 + 31) & ~31)) xs[i] = r < J.O.rows && k0 + k < k1 ? pvd_to_f32<DT>(x[r * J.ldx + k0 + k]) : 0.f;
+    }
+    __syncthreads();
+}
+
+template <int DT, int R> __global__ __launch_bounds__(512) void pvk_dense_rows(const PvdRowsJob J) {
+    typedef typename PvdType<DT>::T T;
+    enum { VEC = PvdType<DT>::VEC, COLS = 64 * VEC };
+    __shared__ __attribute__((aligned(16))) float xs[R * PVD_RK];
+    __shared__ __attribute__((aligned(16))) float red[PVD_RW * COLS];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const int piece = blockIdx.x / J.blocks;
+    const int64_t n0 = (int64_t)(blockIdx.x % J.blocks) * COLS, k0 = piece * J.kper, k1 = min(J.K, k0 + J.kper);
+    pvd_rows_x<DT, R>(J, k0, k1, xs);
+    float acc[R][VEC];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[r][e] = 0.f;
+    const int K = (int)(k1 - k0);
+    const T* w = static_cast<const T*>(J.w) + k0 * J.ldw + n0;
+    // wave after wave four rows of w, eight of a lane's loads under way
+    auto add = [&](const T (&v)[4][VEC], int k) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const pvd_f32x4 x4 = *reinterpret_cast<const pvd_f32x4*>(xs + r * PVD_RK + k);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) acc[r][e] = fmaf(x4[j], pvd_to_f32<DT>(v[j][e]), acc[r][e]);
+        }
+    };
+    if (J.vec) {
+        const bool in = n0 + lane * VEC < J.O.cols;
+#pragma unroll 2
+        for (int k = 4 * wave; k < K; k += 4 * PVD_RW) {
+            alignas(16) T v[4][VEC];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (in && k + j < K) *reinterpret_cast<pvd_u32x4*>(v[j]) = *reinterpret_cast<const pvd_u32x4*>(w + (int64_t)(k + j) * J.ldw + lane * VEC);
+                else *reinterpret_cast<pvd_u32x4*>(v[j]) = (pvd_u32x4){0, 0, 0, 0};
+            }
+            add(v, k);
+        }
+    } else {
+        for (int k = 4 * wave; k < K; k += 4 * PVD_RW) {
+            T v[4][VEC];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const int64_t c = lane + 64 * e;
+                    v[j][e] = k + j < K && n0 + c < J.O.cols ? w[(int64_t)(k + j) * J.ldw + c] : T(0);
+                }
+            add(v, k);
+        }
+    }
+    // the waves' sums, one row of the result at a time
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        if (r >= J.O.rows) break;
+        if (J.vec) {
+#pragma unroll
+            for (int e = 0; e < VEC; e += 4)
+                *reinterpret_cast<pvd_f32x4*>(red + wave * COLS + lane * VEC + e) = (pvd_f32x4){acc[r][e], acc[r][e + 1], acc[r][e + 2], acc[r][e + 3]};
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) red[wave * COLS + lane + 64 * e] = acc[r][e];
+        }
+        __syncthreads();
+        if (tid < COLS / 4) {
+            pvd_f32x4 z = *reinterpret_cast<const pvd_f32x4*>(red + 4 * tid);
+#pragma unroll
+            for (int v = 1; v < PVD_RW; ++v) z += *reinterpret_cast<const pvd_f32x4*>(red + v * COLS + 4 * tid);
+            const int64_t n = n0 + 4 * tid;
+            if (J.splits == 1) pvd_finish4<DT>(J.O, r, n, z);
+            else
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (n + e < J.O.cols) J.part[(piece * J.O.rows + r) * J.O.cols + n + e] = z[e];
+        }
+        __syncthreads();
+    }
+}
+
+// w^T: a wave's four groups of sixteen lanes take a column each, COLS columns to a workgroup
+template <int DT, int R> __global__ __launch_bounds__(512) void pvk_dense_rows_t(const PvdRowsJob J) {
+    typedef typename PvdType<DT>::T T;
+    enum { VEC = PvdType<DT>::VEC, COLS = 128 };
+    __shared__ __attribute__((aligned(16))) float xs[R * PVD_RK];
+    __shared__ __attribute__((aligned(16))) float out[R * COLS];
+    const int tid = threadIdx.x, lane = tid & 15, group = tid >> 4;
+    const int piece = blockIdx.x / J.blocks;
+    const int64_t n0 = (int64_t)(blockIdx.x % J.blocks) * COLS, k0 = piece * J.kper, k1 = min(J.K, k0 + J.kper);
+    pvd_rows_x<DT, R>(J, k0, k1, xs);
+    const int K = (int)(k1 - k0);
+    float acc[4][R];
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int r = 0; r < R; ++r) acc[c][r] = 0.f;
+    // four columns of a group side by side: their loads are under way together
+    for (int k = lane * VEC; k < K; k += 16 * VEC) {
+        alignas(16) T v[4][VEC];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const int64_t n = n0 + group + 32 * c;
+            const T* p = static_cast<const T*>(J.w) + n * J.ldw + k0 + k;
+            if (J.vec && n < J.O.cols && k + VEC <= K) *reinterpret_cast<pvd_u32x4*>(v[c]) = *reinterpret_cast<const pvd_u32x4*>(p);
+            else
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) v[c][e] = n < J.O.cols && k + e < K ? p[e] : T(0);
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int e = 0; e < VEC; e += 4) {
+                const pvd_f32x4 x4 = *reinterpret_cast<const pvd_f32x4*>(xs + r * PVD_RK + k + e);
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[c][r] = fmaf(x4[j], pvd_to_f32<DT>(v[c][e + j]), acc[c][r]);
+            }
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float s = acc[c][r];
+            for (int o = 8; o; o /= 2) s += __shfl_xor(s, o);
+            if (lane == 0) out[r * COLS + group + 32 * c] = s;
+        }
+    __syncthreads();
+    for (int i = tid; i < R * COLS / 4; i += 512) {
+        const int r = i / (COLS / 4), c = i % (COLS / 4) * 4;
+        if (r >= J.O.rows) return;
+        const pvd_f32x4 z = *reinterpret_cast<const pvd_f32x4*>(out + r * COLS + c);
+        if (J.splits == 1) pvd_finish4<DT>(J.O, r, n0 + c, z);
+        else
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (n0 + c + e < J.O.cols) J.part[(piece * J.O.rows + r) * J.O.cols + n0 + c + e] = z[e];
+    }
+}
+
+// The pieces of a split contraction, added in a fixed order, and what follows the product.  G lanes share four columns when
+// there are many pieces of a small result: lane g adds pieces g, g + G, ..., the G sums are added in turn.
+template <int DT, int G> __global__ __launch_bounds__(256) void pvk_dense_join(const PvdOut O, const float* __restrict__ part, int pieces) {
+    const int64_t quads = (O.cols + 3) / 4, i = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+    const bool in = i < O.rows * quads;
+    const int64_t m = in ? i / quads : 0, n = in ? i % quads * 4 : 0;
     pvd_f32x4 z = {0.f, 0.f, 0.f, 0.f};
     if (O.cols % 4 == 0) {
 #pragma unroll 4
-        for (int p = 0; p < pieces; ++p) z += *reinterpret_cast<const pvd_f32x4*>(part + (p * O.rows + m) * O.cols + n);
+        for (int p = threadIdx.x % G; p < pieces; p += G) z += *reinterpret_cast<const pvd_f32x4*>(part + (p * O.rows + m) * O.cols + n);
     } else {
-        for (int p = 0; p < pieces; ++p)
+        for (int p = threadIdx.x % G; p < pieces; p += G)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 if (n + e < O.cols) z[e] += part[(p * O.rows + m) * O.cols + n + e];
     }
-    pvd_finish4<DT>(O, m, n, z);
+#pragma unroll
+    for (int o = G / 2; o; o /= 2)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z[e] += __shfl_down(z[e], o, G);
+    if (in && threadIdx.x % G == 0) pvd_finish4<DT>(O, m, n, z);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -331,29 +589,45 @@ struct PvdBwdJob {
     float* dpre;
 };
 
-template <int DT> __global__ __launch_bounds__(256) void pvk_dense_bwd_tile(const PvdBwdJob J) {
-    __shared__ __attribute__((aligned(16))) char smem[2 * PVD_T * PVD_LDB];
+// 64 columns of dbias (and of dpre): the workgroup's waves take rows in turn
+template <int DT, int WAVES> __device__ __forceinline__ void pvd_bias_job(const PvdBwdJob& J, int64_t block, float* red) {
     typedef typename PvdType<DT>::T T;
-    int64_t b = blockIdx.x;
-    if (b < J.n_dx) return pvd_tile_job<DT, true, false>(J.dx, b, smem);
-    b -= J.n_dx;
-    if (b < J.n_dw) return pvd_tile_job<DT, false, true>(J.dw, b, smem);
-    b -= J.n_dw;
     const int c = threadIdx.x & 63, g = threadIdx.x >> 6;
-    const int64_t n = b * 64 + c;
+    const int64_t n = block * 64 + c;
     float s = 0.f;
-    if (n < J.n)
-        for (int64_t m = g; m < J.m; m += 4) {
+    if (n < J.n) {
+#pragma unroll 4
+        for (int64_t m = g; m < J.m; m += WAVES) {
             float v = pvd_to_f32<DT>(static_cast<const T*>(J.dy)[m * J.lddy + n]);
             if (J.act != PVD_LINEAR) v *= pvd_act_grad(J.pre[m * J.ldp + n], J.act);
             if (J.dpre) J.dpre[m * J.n + n] = v;
             s += v;
         }
-    float* red = reinterpret_cast<float*>(smem);
+    }
     red[threadIdx.x] = s;
     __syncthreads();
-    if (g == 0 && n < J.n && J.dbias)
-        static_cast<T*>(J.dbias)[n] = pvd_from_f32<DT>((red[c] + red[64 + c]) + (red[128 + c] + red[192 + c]));
+    if (g == 0 && n < J.n && J.dbias) {
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) s += red[64 * w + c];
+        static_cast<T*>(J.dbias)[n] = pvd_from_f32<DT>(s);
+    }
+}
+
+template <int DT> __global__ __launch_bounds__(256) void pvk_dense_bwd_tile(const PvdBwdJob J) {
+    __shared__ __attribute__((aligned(16))) char smem[2 * PVD_T * PVD_LDB];
+    int64_t b = blockIdx.x;
+    if (b < J.n_dx) return pvd_tile_job<DT, true, false>(J.dx, b, smem);
+    b -= J.n_dx;
+    if (b < J.n_dw) return pvd_tile_job<DT, false, true>(J.dw, b, smem);
+    pvd_bias_job<DT, 4>(J, b - J.n_dw, reinterpret_cast<float*>(smem));
+}
+template <int DT> __global__ __launch_bounds__(512) void pvk_dense_bwd_slim(const PvdBwdJob J) {
+    __shared__ __attribute__((aligned(16))) float red[PVD_SW * PVD_SM * PVD_SN];
+    int64_t b = blockIdx.x;
+    if (b < J.n_dx) return pvd_slim_job<DT, true, false>(J.dx, b, red);
+    b -= J.n_dx;
+    if (b < J.n_dw) return pvd_slim_job<DT, false, true>(J.dw, b, red);
+    pvd_bias_job<DT, PVD_SW>(J, b - J.n_dw, red);
 }
 
 // ---------------------------------------------------------------------------------------------

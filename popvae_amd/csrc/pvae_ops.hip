@@ -98,32 +98,76 @@ PvdOut output(int64_t rows, int64_t cols, void* y, int64_t ldy, const void* bias
     return o;
 }
 
-// pieces of the contraction: enough workgroups for the chip when the result has few tiles, each with at least 512 bytes of
-// every row
-void split_tile_job(PvdTileJob& J, int size, int64_t wanted) {
-    const int64_t step = 128 / size, tiles = (int64_t)J.mt * J.nt, most = std::max<int64_t>(1, J.K / (4 * step));
-    const int64_t pieces = tiles ? std::min(most, std::max<int64_t>(1, wanted / tiles)) : 1;
-    J.kper = std::max<int64_t>(step, ceil_div(ceil_div(J.K, pieces), step) * step);
-    J.splits = (int)std::max<int64_t>(1, ceil_div(J.K, J.kper));
-}
-PvdTileJob tile_job(const PvdOperand& X, const PvdOperand& W, const PvdOut& O, int64_t K, int size) {
-    PvdTileJob J{X, W, O, K, (int)ceil_div(O.rows, PVD_T), (int)ceil_div(O.cols, PVD_T), 1, 0, nullptr};
-    split_tile_job(J, size, 512);
+// A product through the slim kernel (32 x 16 a workgroup) or the tile kernel (64 x 64), and the pieces of its contraction.
+// Slim while its workgroups find room on the chip at once: what counts then is one round trip to memory, not bytes.
+bool is_slim(int64_t rows, int64_t cols) { return ceil_div(rows, PVD_SM) * ceil_div(cols, PVD_SN) <= 1024; }
+PvdTileJob tile_job(const PvdOperand& X, const PvdOperand& W, const PvdOut& O, int64_t K, int size, bool slim) {
+    PvdTileJob J{X, W, O, K, (int)ceil_div(O.rows, slim ? PVD_SM : PVD_T), (int)ceil_div(O.cols, slim ? PVD_SN : PVD_T), 1, 0, nullptr};
+    // pieces: while CUs would be left without work, each with a few steps of the kernel's loop at least
+    const int64_t step = slim ? PVD_SW * 2 * 64 / size : 128 / size, tiles = (int64_t)J.mt * J.nt;
+    const int64_t most = std::max<int64_t>(1, K / ((slim ? 2 : 4) * step));
+    const int64_t pieces = tiles ? std::min(most, std::max<int64_t>(1, (slim ? 256 : 512) / tiles)) : 1;
+    J.kper = std::max<int64_t>(step, ceil_div(ceil_div(K, pieces), step) * step);
+    J.splits = (int)std::max<int64_t>(1, ceil_div(K, J.kper));
     return J;
 }
 int64_t tile_job_bytes(const PvdTileJob& J) { return J.splits > 1 ? (int64_t)J.splits * J.O.rows * J.O.cols * 4 : 0; }
 
-#define PVD_BY_TYPE(dt, CALL)                                          \
+#define PVD_BY_TYPE(dt, ...)                                           \
     switch (dt) {                                                      \
-        case PVAE_F32: { constexpr int D_ = PVD_F32; CALL; } break;    \
-        case PVAE_BF16: { constexpr int D_ = PVD_BF16; CALL; } break;  \
-        default: { constexpr int D_ = PVD_F16; CALL; } break;          \
+        case PVAE_F32: { constexpr int D_ = PVD_F32; __VA_ARGS__; } break;    \
+        case PVAE_BF16: { constexpr int D_ = PVD_BF16; __VA_ARGS__; } break;  \
+        default: { constexpr int D_ = PVD_F16; __VA_ARGS__; } break;          \
     }
 
-int launch_join(int dt, const PvdTileJob& J, hipStream_t s) {
-    const int64_t quads = J.O.rows * ceil_div(J.O.cols, 4);
-    PVD_BY_TYPE(dt, hipLaunchKernelGGL(pvk_dense_join<D_>, dim3((unsigned)ceil_div(quads, 256)), dim3(256), 0, s, J.O, (const float*)J.part, J.splits));
+int launch_join(int dt, const PvdOut& O, const float* part, int pieces, hipStream_t s) {
+    const int64_t quads = O.rows * ceil_div(O.cols, 4);
+    // sixteen lanes to four columns where a lane of its own would leave the chip empty and walk a long way
+    if (pieces >= 16 && quads < 64 * 1024) {
+        PVD_BY_TYPE(dt, hipLaunchKernelGGL((pvk_dense_join<D_, 16>), dim3((unsigned)ceil_div(quads, 16)), dim3(256), 0, s, O, part, pieces));
+    } else {
+        PVD_BY_TYPE(dt, hipLaunchKernelGGL((pvk_dense_join<D_, 1>), dim3((unsigned)ceil_div(quads, 256)), dim3(256), 0, s, O, part, pieces));
+    }
     return launched("dense_join");
+}
+
+// ---- up to eight rows: the weights read once ----
+bool is_rows(const pvae_dense_args& a) { return a.m <= 8 && a.k > 0; }
+bool rows_transposed(const pvae_dense_args& a) { return a.n > 1 ? a.w_sn != 1 : a.w_sk == 1; }  // w's columns are contiguous
+PvdRowsJob rows_job(const pvae_dense_args& a) {
+    const int size = esize(a.dtype);
+    const bool t = rows_transposed(a);
+    PvdRowsJob J{};
+    J.x = a.x; J.ldx = a.ldx;
+    J.w = a.w; J.ldw = t ? a.w_sn : a.w_sk;
+    J.K = a.k;
+    J.O = output(a.m, a.n, a.y, a.ldy, a.bias, a.residual, a.ldr, a.pre, a.ldp, a.act, size);
+    J.vec = aligned(a.w, 16) && J.ldw * size % 16 == 0 && (t || a.n * size % 16 == 0);
+    J.blocks = (int)ceil_div(a.n, t ? 128 : 64 * 16 / size);
+    // pieces of the contraction: to fill the chip, of 64 at least and of PVD_RK, what LDS holds of x, at most
+    const int64_t pieces = std::max(ceil_div(a.k, PVD_RK), std::min<int64_t>(std::max<int64_t>(1, a.k / 64), std::max<int64_t>(1, 512 / J.blocks)));
+    J.kper = ceil_div(ceil_div(a.k, pieces), 32) * 32;
+    J.splits = (int)ceil_div(a.k, J.kper);
+    return J;
+}
+int64_t rows_bytes(const PvdRowsJob& J) { return J.splits > 1 ? (int64_t)J.splits * J.O.rows * J.O.cols * 4 : 0; }
+template <int DT, int R> void launch_rows(const PvdRowsJob& J, bool t, hipStream_t s) {
+    const dim3 grid((unsigned)(J.blocks * (int64_t)J.splits));
+    if (t) hipLaunchKernelGGL((pvk_dense_rows_t<DT, R>), grid, dim3(512), 0, s, J);
+    else hipLaunchKernelGGL((pvk_dense_rows<DT, R>), grid, dim3(512), 0, s, J);
+}
+int run_rows(const pvae_dense_args& a, PvdRowsJob J, void* workspace, hipStream_t s) {
+    if (int rc = check_grid(J.blocks * (int64_t)J.splits)) return rc;
+    J.part = static_cast<float*>(workspace);
+    const bool t = rows_transposed(a);
+    PVD_BY_TYPE(a.dtype, {
+        if (a.m == 1) launch_rows<D_, 1>(J, t, s);
+        else if (a.m == 2) launch_rows<D_, 2>(J, t, s);
+        else if (a.m <= 4) launch_rows<D_, 4>(J, t, s);
+        else launch_rows<D_, 8>(J, t, s);
+    });
+    if (int rc = launched("dense_rows")) return rc;
+    return J.splits > 1 ? launch_join(a.dtype, J.O, J.part, J.splits, s) : 0;
 }
 
 // ---- large products: operands laid out (pvk_dense_pack) where they have to be, then pvk_dense_nt ----
@@ -265,13 +309,7 @@ int launch_large(int dt, NtPlan& plan, hipStream_t s) {
     else PVD_BY_TYPE(dt, (rc = plan.deep ? launch_nt<D_, 128, 4, 2, 4>(P, blocks, s) : launch_nt<D_, 128, 4, 2, 2>(P, blocks, s)));
     if (rc) return rc;
     for (int i = 0; i < P.n; ++i)
-        if (P.job[i].splits > 1) {
-            PvdTileJob J{};
-            J.O = P.job[i].O;
-            J.part = P.job[i].part;
-            J.splits = P.job[i].splits;
-            if ((rc = launch_join(dt, J, s))) return rc;
-        }
+        if (P.job[i].splits > 1 && (rc = launch_join(dt, P.job[i].O, P.job[i].part, P.job[i].splits, s))) return rc;
     return 0;
 }
 
@@ -314,7 +352,7 @@ bool bwd_is_large(const pvae_dense_bwd_args& a) { return (a.dx || a.dw) && is_la
 PvdTileJob dense_job(const pvae_dense_args& a) {
     const int size = esize(a.dtype);
     return tile_job(operand(a.x, a.m, a.k, a.ldx, 1, size), operand(a.w, a.n, a.k, a.w_sn, a.w_sk, size),
-                    output(a.m, a.n, a.y, a.ldy, a.bias, a.residual, a.ldr, a.pre, a.ldp, a.act, size), a.k, size);
+                    output(a.m, a.n, a.y, a.ldy, a.bias, a.residual, a.ldr, a.pre, a.ldp, a.act, size), a.k, size, is_slim(a.m, a.n));
 }
 int check_dense(const pvae_dense_args* a) {
     if (!a) return refuse(-1, "no arguments");
@@ -335,20 +373,22 @@ int check_dense(const pvae_dense_args* a) {
 struct BwdPlan {
     PvdBwdJob J;
     int64_t n_db;
+    bool slim;  // both products through the slim kernel
 };
 BwdPlan bwd_plan(const pvae_dense_bwd_args& a) {
     const int size = esize(a.dtype);
     BwdPlan p{};
+    p.slim = is_slim(a.dx ? a.m : 0, a.k) && is_slim(a.dw ? a.k : 0, a.n);
     PvdOperand gx = operand(a.dy, a.m, a.n, a.lddy, 1, size), gw = operand(a.dy, a.n, a.m, 1, a.lddy, size);
     with_grad(gx, a.pre, a.ldp, 1, a.act);
     with_grad(gw, a.pre, 1, a.ldp, a.act);
     // w as an operand of dx: rows are the k of the layer, the contraction its n
     if (a.dx)
         p.J.dx = tile_job(gx, operand(a.w, a.k, a.n, a.w_sk, a.w_sn, size),
-                          output(a.m, a.k, a.dx, a.lddx, nullptr, a.dx_add, a.ldadd, nullptr, 0, PVD_LINEAR, size), a.n, size);
+                          output(a.m, a.k, a.dx, a.lddx, nullptr, a.dx_add, a.ldadd, nullptr, 0, PVD_LINEAR, size), a.n, size, p.slim);
     if (a.dw)
         p.J.dw = tile_job(operand(a.x, a.k, a.m, 1, a.ldx, size), gw,
-                          output(a.k, a.n, a.dw, a.n, nullptr, nullptr, 0, nullptr, 0, PVD_LINEAR, size), a.m, size);
+                          output(a.k, a.n, a.dw, a.n, nullptr, nullptr, 0, nullptr, 0, PVD_LINEAR, size), a.m, size, p.slim);
     p.J.n_dx = a.dx ? (int64_t)p.J.dx.mt * p.J.dx.nt * p.J.dx.splits : 0;
     p.J.n_dw = a.dw ? (int64_t)p.J.dw.mt * p.J.dw.nt * p.J.dw.splits : 0;
     p.J.dy = a.dy;
@@ -488,6 +528,7 @@ const char* pvae_ops_last_error(void) { return g_err; }
 
 int64_t pvae_dense_workspace(const pvae_dense_args* a) {
     if (check_dense(a) || a->m == 0 || a->n == 0) return 0;
+    if (is_rows(*a)) return rows_bytes(rows_job(*a));
     if (is_large(a->m, a->n, a->k)) return large_dense(*a, nullptr).bytes;
     return tile_job_bytes(dense_job(*a));
 }
@@ -496,6 +537,11 @@ int pvae_dense(const pvae_dense_args* a, void* workspace, int64_t workspace_byte
     if (int rc = check_dense(a)) return rc;
     if (a->m == 0 || a->n == 0) return 0;
     hipStream_t s = static_cast<hipStream_t>(hip_stream);
+    if (is_rows(*a)) {
+        const PvdRowsJob J = rows_job(*a);
+        if (int rc = check_workspace("pvae_dense", workspace, workspace_bytes, rows_bytes(J))) return rc;
+        return run_rows(*a, J, workspace, s);
+    }
     if (is_large(a->m, a->n, a->k)) {
         NtPlan plan = large_dense(*a, workspace);
         if (int rc = check_workspace("pvae_dense", workspace, workspace_bytes, plan.bytes)) return rc;
@@ -506,9 +552,13 @@ int pvae_dense(const pvae_dense_args* a, void* workspace, int64_t workspace_byte
     const int64_t blocks = (int64_t)J.mt * J.nt * J.splits;
     if (int rc = check_grid(blocks)) return rc;
     J.part = static_cast<float*>(workspace);
-    PVD_BY_TYPE(a->dtype, hipLaunchKernelGGL(pvk_dense_tile<D_>, dim3((unsigned)blocks), dim3(256), 0, s, J));
+    if (is_slim(a->m, a->n)) {
+        PVD_BY_TYPE(a->dtype, hipLaunchKernelGGL(pvk_dense_slim<D_>, dim3((unsigned)blocks), dim3(512), 0, s, J));
+    } else {
+        PVD_BY_TYPE(a->dtype, hipLaunchKernelGGL(pvk_dense_tile<D_>, dim3((unsigned)blocks), dim3(256), 0, s, J));
+    }
     if (int rc = launched("dense_tile")) return rc;
-    return J.splits > 1 ? launch_join(a->dtype, J, s) : 0;
+    return J.splits > 1 ? launch_join(a->dtype, J.O, J.part, J.splits, s) : 0;
 }
 
 int64_t pvae_dense_bwd_workspace(const pvae_dense_bwd_args* a) {
@@ -532,12 +582,16 @@ int pvae_dense_bwd(const pvae_dense_bwd_args* a, void* workspace, int64_t worksp
     if (blocks == 0) return 0;
     p.J.dx.part = static_cast<float*>(workspace);
     p.J.dw.part = static_cast<float*>(workspace) + (p.J.n_dx ? tile_job_bytes(p.J.dx) / 4 : 0);
-    PVD_BY_TYPE(a->dtype, hipLaunchKernelGGL(pvk_dense_bwd_tile<D_>, dim3((unsigned)blocks), dim3(256), 0, s, p.J));
+    if (p.slim) {
+        PVD_BY_TYPE(a->dtype, hipLaunchKernelGGL(pvk_dense_bwd_slim<D_>, dim3((unsigned)blocks), dim3(512), 0, s, p.J));
+    } else {
+        PVD_BY_TYPE(a->dtype, hipLaunchKernelGGL(pvk_dense_bwd_tile<D_>, dim3((unsigned)blocks), dim3(256), 0, s, p.J));
+    }
     if (int rc = launched("dense_bwd_tile")) return rc;
     if (p.J.n_dx && p.J.dx.splits > 1)
-        if (int rc = launch_join(a->dtype, p.J.dx, s)) return rc;
+        if (int rc = launch_join(a->dtype, p.J.dx.O, p.J.dx.part, p.J.dx.splits, s)) return rc;
     if (p.J.n_dw && p.J.dw.splits > 1)
-        if (int rc = launch_join(a->dtype, p.J.dw, s)) return rc;
+        if (int rc = launch_join(a->dtype, p.J.dw.O, p.J.dw.part, p.J.dw.splits, s)) return rc;
     return 0;
 }
 
