@@ -15,6 +15,7 @@ typedef float pvd_f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 pvd_bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 pvd_f16x8 __attribute__((ext_vector_type(8)));
 typedef unsigned pvd_u32x4 __attribute__((ext_vector_type(4)));
+typedef pvd_u32x4 pvd_u32x4_any __attribute__((aligned(2)));  // sixteen bytes at any address of an element
 
 template <int DT> struct PvdType { typedef unsigned short T; enum { SIZE = 2, VEC = 8 }; };
 template <> struct PvdType<PVD_F32> { typedef float T; enum { SIZE = 4, VEC = 4 }; };
@@ -90,34 +91,34 @@ struct PvdOut {
     float* pre;
     int64_t ldp;
     int act;
-    int vec;  // four columns at a multiple of four may be read and written as one access everywhere
 };
+
+// four elements from p[i] on, `left` of which are there (zeros, and nothing stored, behind them)
+__device__ __forceinline__ pvd_f32x4 pvd_load_some(const void* p, int dt, int64_t i, int left) {
+    if (left >= 4) return pvm_load4(p, dt, i);
+    pvd_f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+        if (e < left) v[e] = pvm_load1(p, dt, i + e);
+    return v;
+}
+__device__ __forceinline__ void pvd_store_some(void* p, int dt, int64_t i, pvd_f32x4 v, int left) {
+    if (left >= 4) return pvm_store4(p, dt, i, v);
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+        if (e < left) pvm_store1(p, dt, i + e, v[e]);
+}
+__device__ __forceinline__ int pvd_left(int64_t n, int64_t cols) { return (int)min((int64_t)4, cols - n); }
 
 // z = the products of columns n .. n + 3 of row m
 template <int DT> __device__ __forceinline__ void pvd_finish4(const PvdOut& O, int64_t m, int64_t n, pvd_f32x4 z) {
-    typedef typename PvdType<DT>::T T;
     if (m >= O.rows || n >= O.cols) return;
-    const T *bias = static_cast<const T*>(O.bias), *res = static_cast<const T*>(O.res);
-    T* y = static_cast<T*>(O.y) + m * O.ldy + n;
-    if (O.vec && n + 3 < O.cols) {
-        if (bias) z += pvm_load4(bias, DT, n);
-        if (O.pre) *reinterpret_cast<pvd_f32x4*>(O.pre + m * O.ldp + n) = z;
-        pvd_f32x4 o = pvd_act4(z, O.act);
-        if (res) o += pvm_load4(res, DT, m * O.ldr + n);
-        pvm_store4(y, DT, 0, o);
-        return;
-    }
-    const int left = (int)min((int64_t)4, O.cols - n);
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (e < left) {
-            if (bias) z[e] += pvd_to_f32<DT>(bias[n + e]);
-            if (O.pre) O.pre[m * O.ldp + n + e] = z[e];
-        }
-    const pvd_f32x4 o = pvd_act4(z, O.act);
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (e < left) y[e] = pvd_from_f32<DT>(res ? o[e] + pvd_to_f32<DT>(res[m * O.ldr + n + e]) : o[e]);
+    const int left = pvd_left(n, O.cols);
+    if (O.bias) z += pvd_load_some(O.bias, DT, n, left);
+    if (O.pre) pvd_store_some(O.pre, 0, m * O.ldp + n, z, left);
+    pvd_f32x4 o = pvd_act4(z, O.act);
+    if (O.res) o += pvd_load_some(O.res, DT, m * O.ldr + n, left);
+    pvd_store_some(O.y, DT, m * O.ldy + n, o, left);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -131,7 +132,6 @@ struct PvdOperand {  // element (row, k) at p[row * sr + k * sk]; one of the str
     const float* pre;  // gradient operand: p is dy and the element dy * f'(pre); pre's strides
     int64_t pr, pk;
     int act;
-    int vec;  // sixteen bytes along the unit stride may be read as one access where they start at a multiple
 };
 
 enum { PVD_T = 64, PVD_LDB = 144 };  // tile edge; bytes of an LDS row: 128 and 16 that spread the rows over the banks
@@ -151,12 +151,12 @@ template <int DT, bool GRAD> struct PvdStage {
             for (int e = 0; e < VEC; ++e) o[e] = T(0);
             return;
         }
-        if (P.vec && left >= VEC) {
-            *reinterpret_cast<pvd_u32x4*>(o) = *reinterpret_cast<const pvd_u32x4*>(p);
+        if (left >= VEC) {
+            *reinterpret_cast<pvd_u32x4*>(o) = *reinterpret_cast<const pvd_u32x4_any*>(p);
             if (GRAD && P.act != PVD_LINEAR) {
 #pragma unroll
                 for (int e = 0; e < VEC; e += 4) {
-                    const pvd_f32x4 d4 = pvd_act_grad4(*reinterpret_cast<const pvd_f32x4*>(z + e), P.act);
+                    const pvd_f32x4 d4 = pvd_act_grad4(pvm_load4(z, 0, e), P.act);
 #pragma unroll
                     for (int f = 0; f < 4; ++f) o[e + f] = pvd_from_f32<DT>(pvd_to_f32<DT>(o[e + f]) * d4[f]);
                 }
@@ -284,10 +284,7 @@ template <int DT, bool GX, bool GW> __device__ __forceinline__ void pvd_tile_job
         for (int i = 0; i < 2; ++i) {
             const int64_t mm = m + 16 * j, nn = n + 16 * i;
             if (J.splits == 1) pvd_finish4<DT>(J.O, mm, nn, acc[i][j]);
-            else if (mm < J.O.rows)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (nn + e < J.O.cols) J.part[(piece * J.O.rows + mm) * J.O.cols + nn + e] = acc[i][j][e];
+            else if (mm < J.O.rows) pvd_store_some(J.part, 0, (piece * J.O.rows + mm) * J.O.cols + nn, acc[i][j], pvd_left(nn, J.O.cols));
         }
 }
 
@@ -313,8 +310,8 @@ template <int DT, bool GRAD> __device__ __forceinline__ pvd_u32x4 pvd_slim_load(
     const bool grad = GRAD && P.act != PVD_LINEAR;
     const float* z = grad ? P.pre + row * P.pr + k * P.pk : nullptr;
     const bool in = row < P.rows;
-    if (P.sk == 1 && P.vec && in && k + VEC <= k1) {
-        *reinterpret_cast<pvd_u32x4*>(v) = *reinterpret_cast<const pvd_u32x4*>(p);
+    if (P.sk == 1 && in && k + VEC <= k1) {
+        *reinterpret_cast<pvd_u32x4*>(v) = *reinterpret_cast<const pvd_u32x4_any*>(p);
     } else {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) v[e] = in && k + e < k1 ? p[e * P.sk] : T(0);
@@ -366,10 +363,7 @@ template <int DT, bool GX, bool GW> __device__ __forceinline__ void pvd_slim_job
     for (int w = 1; w < PVD_SW; ++w) z += *reinterpret_cast<const pvd_f32x4*>(red + (w * PVD_SM + row) * PVD_SN + c);
     const int64_t m = m0 + row, n = n0 + c;
     if (J.splits == 1) pvd_finish4<DT>(J.O, m, n, z);
-    else if (m < J.O.rows)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (n + e < J.O.cols) J.part[(piece * J.O.rows + m) * J.O.cols + n + e] = z[e];
+    else if (m < J.O.rows) pvd_store_some(J.part, 0, (piece * J.O.rows + m) * J.O.cols + n, z, pvd_left(n, J.O.cols));
 }
 
 template <int DT> __global__ __launch_bounds__(512) void pvk_dense_slim(const PvdTileJob J) {
@@ -379,8 +373,7 @@ template <int DT> __global__ __launch_bounds__(512) void pvk_dense_slim(const Pv
 
 // ---------------------------------------------------------------------------------------------
 // The rows kernel, for up to eight rows (one point asked for an answer): the weights are read once, and that is its time.  A
-// lane holds sixteen bytes of a row of w -- or, unaligned, as many columns 64 apart -- and all rows' sums of those columns in
-// registers; x, as float32, comes from LDS.  The workgroup's eight waves, and pieces of the grid, split the contraction.
+// lane holds sixteen bytes of a row of w and all rows' sums of those columns in registers; x, as float32, comes from LDS.  The workgroup's eight waves, and pieces of the grid, split the contraction.
 // w^T (contiguous along the contraction): sixteen lanes share a column instead and add up at the end.
 // ---------------------------------------------------------------------------------------------
 struct PvdRowsJob {
@@ -393,7 +386,6 @@ struct PvdRowsJob {
     int splits;
     int64_t kper;   // contraction of a piece, at most PVD_RK
     int blocks;     // workgroups of a piece
-    int vec;
     float* part;
 };
 enum { PVD_RK = 1024, PVD_RW = 8 };
@@ -436,28 +428,25 @@ template <int DT, int R> __global__ __launch_bounds__(512) void pvk_dense_rows(c
                 for (int e = 0; e < VEC; ++e) acc[r][e] = fmaf(x4[j], pvd_to_f32<DT>(v[j][e]), acc[r][e]);
         }
     };
-    if (J.vec) {
-        const bool in = n0 + lane * VEC < J.O.cols;
+    const int left = (int)min((int64_t)VEC, J.O.cols - n0 - lane * VEC);
+    if (left >= VEC) {
 #pragma unroll 2
         for (int k = 4 * wave; k < K; k += 4 * PVD_RW) {
             alignas(16) T v[4][VEC];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                if (in && k + j < K) *reinterpret_cast<pvd_u32x4*>(v[j]) = *reinterpret_cast<const pvd_u32x4*>(w + (int64_t)(k + j) * J.ldw + lane * VEC);
+                if (k + j < K) *reinterpret_cast<pvd_u32x4*>(v[j]) = *reinterpret_cast<const pvd_u32x4_any*>(w + (int64_t)(k + j) * J.ldw + lane * VEC);
                 else *reinterpret_cast<pvd_u32x4*>(v[j]) = (pvd_u32x4){0, 0, 0, 0};
             }
             add(v, k);
         }
-    } else {
+    } else if (left > 0) {  // the lane with the last columns
         for (int k = 4 * wave; k < K; k += 4 * PVD_RW) {
             T v[4][VEC];
 #pragma unroll
             for (int j = 0; j < 4; ++j)
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const int64_t c = lane + 64 * e;
-                    v[j][e] = k + j < K && n0 + c < J.O.cols ? w[(int64_t)(k + j) * J.ldw + c] : T(0);
-                }
+                for (int e = 0; e < VEC; ++e) v[j][e] = k + j < K && e < left ? w[(int64_t)(k + j) * J.ldw + lane * VEC + e] : T(0);
             add(v, k);
         }
     }
@@ -465,14 +454,9 @@ template <int DT, int R> __global__ __launch_bounds__(512) void pvk_dense_rows(c
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         if (r >= J.O.rows) break;
-        if (J.vec) {
 #pragma unroll
-            for (int e = 0; e < VEC; e += 4)
-                *reinterpret_cast<pvd_f32x4*>(red + wave * COLS + lane * VEC + e) = (pvd_f32x4){acc[r][e], acc[r][e + 1], acc[r][e + 2], acc[r][e + 3]};
-        } else {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) red[wave * COLS + lane + 64 * e] = acc[r][e];
-        }
+        for (int e = 0; e < VEC; e += 4)
+            *reinterpret_cast<pvd_f32x4*>(red + wave * COLS + lane * VEC + e) = (pvd_f32x4){acc[r][e], acc[r][e + 1], acc[r][e + 2], acc[r][e + 3]};
         __syncthreads();
         if (tid < COLS / 4) {
             pvd_f32x4 z = *reinterpret_cast<const pvd_f32x4*>(red + 4 * tid);
@@ -480,10 +464,7 @@ template <int DT, int R> __global__ __launch_bounds__(512) void pvk_dense_rows(c
             for (int v = 1; v < PVD_RW; ++v) z += *reinterpret_cast<const pvd_f32x4*>(red + v * COLS + 4 * tid);
             const int64_t n = n0 + 4 * tid;
             if (J.splits == 1) pvd_finish4<DT>(J.O, r, n, z);
-            else
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (n + e < J.O.cols) J.part[(piece * J.O.rows + r) * J.O.cols + n + e] = z[e];
+            else if (n < J.O.cols) pvd_store_some(J.part, 0, (piece * J.O.rows + r) * J.O.cols + n, z, pvd_left(n, J.O.cols));
         }
         __syncthreads();
     }
@@ -512,7 +493,7 @@ template <int DT, int R> __global__ __launch_bounds__(512) void pvk_dense_rows_t
         for (int c = 0; c < 4; ++c) {
             const int64_t n = n0 + group + 32 * c;
             const T* p = static_cast<const T*>(J.w) + n * J.ldw + k0 + k;
-            if (J.vec && n < J.O.cols && k + VEC <= K) *reinterpret_cast<pvd_u32x4*>(v[c]) = *reinterpret_cast<const pvd_u32x4*>(p);
+            if (n < J.O.cols && k + VEC <= K) *reinterpret_cast<pvd_u32x4*>(v[c]) = *reinterpret_cast<const pvd_u32x4_any*>(p);
             else
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) v[c][e] = n < J.O.cols && k + e < K ? p[e] : T(0);
@@ -542,10 +523,7 @@ template <int DT, int R> __global__ __launch_bounds__(512) void pvk_dense_rows_t
         if (r >= J.O.rows) return;
         const pvd_f32x4 z = *reinterpret_cast<const pvd_f32x4*>(out + r * COLS + c);
         if (J.splits == 1) pvd_finish4<DT>(J.O, r, n0 + c, z);
-        else
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (n0 + c + e < J.O.cols) J.part[(piece * J.O.rows + r) * J.O.cols + n0 + c + e] = z[e];
+        else if (n0 + c < J.O.cols) pvd_store_some(J.part, 0, (piece * J.O.rows + r) * J.O.cols + n0 + c, z, pvd_left(n0 + c, J.O.cols));
     }
 }
 
@@ -556,15 +534,9 @@ template <int DT, int G> __global__ __launch_bounds__(256) void pvk_dense_join(c
     const bool in = i < O.rows * quads;
     const int64_t m = in ? i / quads : 0, n = in ? i % quads * 4 : 0;
     pvd_f32x4 z = {0.f, 0.f, 0.f, 0.f};
-    if (O.cols % 4 == 0) {
+    const int left = pvd_left(n, O.cols);
 #pragma unroll 4
-        for (int p = threadIdx.x % G; p < pieces; p += G) z += *reinterpret_cast<const pvd_f32x4*>(part + (p * O.rows + m) * O.cols + n);
-    } else {
-        for (int p = threadIdx.x % G; p < pieces; p += G)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (n + e < O.cols) z[e] += part[(p * O.rows + m) * O.cols + n + e];
-    }
+    for (int p = threadIdx.x % G; p < pieces; p += G) z += pvd_load_some(part, 0, (p * O.rows + m) * O.cols + n, left);
 #pragma unroll
     for (int o = G / 2; o; o /= 2)
 #pragma unroll
@@ -641,7 +613,7 @@ struct PvdPack {
     int64_t R, C, ld;
     const float* pre;  // g = p * act'(pre)
     int64_t ldp;
-    int act, vec;      // vec: sixteen bytes of p (and of pre) at multiples of them can be read at once
+    int act;
     void* same;        // [R][ld_same], the first w_same elements of a row filled, or NULL
     int64_t ld_same, w_same;
     void* tran;        // [C][ld_tran], w_tran of a row filled, or NULL
@@ -678,8 +650,8 @@ template <int DT> __global__ __launch_bounds__(256) void pvk_dense_pack(const Pv
         alignas(16) T v[VEC];
         float f[VEC];
         const bool whole = r < J.R && c + VEC <= J.C;
-        if (whole && J.vec) {
-            *reinterpret_cast<pvd_u32x4*>(v) = *reinterpret_cast<const pvd_u32x4*>(p + r * J.ld + c);
+        if (whole) {
+            *reinterpret_cast<pvd_u32x4*>(v) = *reinterpret_cast<const pvd_u32x4_any*>(p + r * J.ld + c);
         } else {
 #pragma unroll
             for (int e = 0; e < VEC; ++e) v[e] = r < J.R && c + e < J.C ? p[r * J.ld + c + e] : T(0);
@@ -689,9 +661,9 @@ template <int DT> __global__ __launch_bounds__(256) void pvk_dense_pack(const Pv
             for (int e = 0; e < VEC; ++e) f[e] = pvd_to_f32<DT>(v[e]);
             if (J.pre && J.act != PVD_LINEAR) {
                 alignas(16) float z[VEC];
-                if (whole && J.vec) {
+                if (whole) {
 #pragma unroll
-                    for (int e = 0; e < VEC; e += 4) *reinterpret_cast<pvd_f32x4*>(z + e) = *reinterpret_cast<const pvd_f32x4*>(J.pre + r * J.ldp + c + e);
+                    for (int e = 0; e < VEC; e += 4) *reinterpret_cast<pvd_f32x4*>(z + e) = pvm_load4(J.pre, 0, r * J.ldp + c + e);
                 } else {
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) z[e] = r < J.R && c + e < J.C ? J.pre[r * J.ldp + c + e] : 0.f;
@@ -774,65 +746,31 @@ typedef __attribute__((address_space(3))) void* pvd_lptr;
 // What follows the product for ROWS x 64 products of one wave in LDS (row r's piece u of four floats at slot u ^ (r & 15)):
 // rows m .., columns n ..; the residuals of several rows are asked for together.
 template <int DT, int ROWS> __device__ __forceinline__ void pvd_finish_rows(const PvdOut& O, int64_t m, int64_t n, const float* ep) {
-    typedef typename PvdType<DT>::T T;
-    const int lane = threadIdx.x & 63;
-    const T *bias = static_cast<const T*>(O.bias), *res = static_cast<const T*>(O.res);
-    T* y = static_cast<T*>(O.y);
+    enum { G = ROWS / 4 < 8 ? ROWS / 4 : 8 };
+    const int lane = threadIdx.x & 63, er = lane >> 4, eu = lane & 15;  // sixteen lanes, four columns each, on a row
     const int rows = (int)max((int64_t)0, min((int64_t)ROWS, O.rows - m));
-    if (O.vec && (O.cols & 3) == 0) {  // sixteen lanes, four columns each, on a row
-        enum { G = ROWS / 4 < 8 ? ROWS / 4 : 8 };
-        const int er = lane >> 4, eu = lane & 15;
-        const int64_t c = n + 4 * eu;
-        if (c >= O.cols) return;
-        pvd_f32x4 b4 = {0.f, 0.f, 0.f, 0.f};
-        if (bias) b4 = pvm_load4(bias, DT, c);
-#pragma unroll 1
-        for (int r0 = er; r0 < rows; r0 += 4 * G) {
-            pvd_f32x4 r4[G];
-            if (res)
-#pragma unroll
-                for (int g = 0; g < G; ++g)
-                    if (r0 + 4 * g < rows) r4[g] = pvm_load4(res, DT, (m + r0 + 4 * g) * O.ldr + c);
-#pragma unroll
-            for (int g = 0; g < G; ++g) {
-                const int r = r0 + 4 * g;
-                if (r >= rows) break;
-                pvd_f32x4 z = *reinterpret_cast<const pvd_f32x4*>(ep + r * 64 + ((eu ^ (r & 15)) << 2));
-                z += b4;
-                if (O.pre) *reinterpret_cast<pvd_f32x4*>(O.pre + (m + r) * O.ldp + c) = z;
-                pvd_f32x4 o = pvd_act4(z, O.act);
-                if (res) o += r4[g];
-                pvm_store4(y, DT, (m + r) * O.ldy + c, o);
-            }
-        }
-        return;
-    }
-    // a lane per column: a row's 64 columns lie together whatever their alignment
-    const int64_t c = n + lane;
+    const int64_t c = n + 4 * eu;
     if (c >= O.cols) return;
-    const float b1 = bias ? pvd_to_f32<DT>(bias[c]) : 0.f;
+    const int left = pvd_left(c, O.cols);
+    pvd_f32x4 b4 = {0.f, 0.f, 0.f, 0.f};
+    if (O.bias) b4 = pvd_load_some(O.bias, DT, c, left);
 #pragma unroll 1
-    for (int r0 = 0; r0 < rows; r0 += 8) {
-        float r1[8];
-        if (res)
+    for (int r0 = er; r0 < rows; r0 += 4 * G) {
+        pvd_f32x4 r4[G];
+        if (O.res)
 #pragma unroll
-            for (int g = 0; g < 8; ++g)
-                if (r0 + g < rows) r1[g] = pvd_to_f32<DT>(res[(m + r0 + g) * O.ldr + c]);
+            for (int g = 0; g < G; ++g)
+                if (r0 + 4 * g < rows) r4[g] = pvd_load_some(O.res, DT, (m + r0 + 4 * g) * O.ldr + c, left);
 #pragma unroll
-        for (int g4 = 0; g4 < 8; g4 += 4) {
-            pvd_f32x4 z;
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int r = r0 + g4 + g;
-                z[g] = ep[r * 64 + (((lane >> 2) ^ (r & 15)) << 2) + (lane & 3)] + b1;
-                if (O.pre && r < rows) O.pre[(m + r) * O.ldp + c] = z[g];
-            }
-            const pvd_f32x4 o = pvd_act4(z, O.act);
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int r = r0 + g4 + g;
-                if (r < rows) y[(m + r) * O.ldy + c] = pvd_from_f32<DT>(res ? o[g] + r1[g4 + g] : o[g]);
-            }
+        for (int g = 0; g < G; ++g) {
+            const int r = r0 + 4 * g;
+            if (r >= rows) break;
+            pvd_f32x4 z = *reinterpret_cast<const pvd_f32x4*>(ep + r * 64 + ((eu ^ (r & 15)) << 2));
+            z += b4;
+            if (O.pre) pvd_store_some(O.pre, 0, (m + r) * O.ldp + c, z, left);
+            pvd_f32x4 o = pvd_act4(z, O.act);
+            if (O.res) o += r4[g];
+            pvd_store_some(O.y, DT, (m + r) * O.ldy + c, o, left);
         }
     }
 }
@@ -962,14 +900,8 @@ template <int DT, int TM, int TN, int WM, int WN, int ST> struct PvdNt {
                 for (int row = lane >> 4; row < EPR && m + row < J.O.rows; row += 4) {
                     const int u = lane & 15;
                     const pvd_f32x4 z = *reinterpret_cast<const pvd_f32x4*>(ep + row * 64 + ((u ^ (row & 15)) << 2));
-                    float* d = J.part + (pc * J.O.rows + m + row) * J.O.cols + n + 4 * u;
-                    if (J.O.cols % 4 == 0) {
-                        if (n + 4 * u < J.O.cols) *reinterpret_cast<pvd_f32x4*>(d) = z;
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (n + 4 * u + e < J.O.cols) d[e] = z[e];
-                    }
+                    if (n + 4 * u < J.O.cols)
+                        pvd_store_some(J.part, 0, (pc * J.O.rows + m + row) * J.O.cols + n + 4 * u, z, pvd_left(n + 4 * u, J.O.cols));
                 }
             }
             same_wave();

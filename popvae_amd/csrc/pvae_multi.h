@@ -19,6 +19,12 @@ typedef float pvm_f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned short pvm_u16x8 __attribute__((ext_vector_type(8)));
 typedef unsigned short pvm_u16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 pvm_f16x4 __attribute__((ext_vector_type(4)));
+// the same where nothing but the elements' own alignment is known (a view, an odd row stride): memory is read and written 8 and
+// 16 bytes at a time all the same, the hardware takes any address
+typedef pvm_f32x4 pvm_f32x4_any __attribute__((aligned(4)));
+typedef pvm_u16x4 pvm_u16x4_any __attribute__((aligned(2)));
+typedef pvm_f16x4 pvm_f16x4_any __attribute__((aligned(2)));
+typedef pvm_u16x8 pvm_u16x8_any __attribute__((aligned(2)));
 
 struct PvmTab {  // elements [0, n) of tensor t are chunks first[t] .. first[t + 1) of PVM_CHUNK elements
     int count;
@@ -30,7 +36,6 @@ struct PvmTab {  // elements [0, n) of tensor t are chunks first[t] .. first[t +
     int64_t n[PVM_MAXT];
     int tile[PVM_MAXT];            // pvae_tensor.tile of b, m and v
     unsigned char dt[PVM_MAXT];    // type of a
-    unsigned char vec[PVM_MAXT];   // every pointer is aligned to sixteen bytes
 };
 
 __device__ __forceinline__ float pvm_bf16(unsigned short u) { return __uint_as_float((unsigned)u << 16); }
@@ -46,12 +51,12 @@ __device__ __forceinline__ float pvm_load1(const void* p, int dt, int64_t i) {
     return (float)static_cast<const _Float16*>(p)[i];
 }
 __device__ __forceinline__ pvm_f32x4 pvm_load4(const void* p, int dt, int64_t i) {
-    if (dt == 0) return *reinterpret_cast<const pvm_f32x4*>(static_cast<const float*>(p) + i);
+    if (dt == 0) return *reinterpret_cast<const pvm_f32x4_any*>(static_cast<const float*>(p) + i);
     if (dt == 1) {
-        const pvm_u16x4 u = *reinterpret_cast<const pvm_u16x4*>(static_cast<const unsigned short*>(p) + i);
+        const pvm_u16x4 u = *reinterpret_cast<const pvm_u16x4_any*>(static_cast<const unsigned short*>(p) + i);
         return (pvm_f32x4){pvm_bf16(u.x), pvm_bf16(u.y), pvm_bf16(u.z), pvm_bf16(u.w)};
     }
-    const pvm_f16x4 h = *reinterpret_cast<const pvm_f16x4*>(static_cast<const _Float16*>(p) + i);
+    const pvm_f16x4 h = *reinterpret_cast<const pvm_f16x4_any*>(static_cast<const _Float16*>(p) + i);
     return (pvm_f32x4){(float)h.x, (float)h.y, (float)h.z, (float)h.w};
 }
 __device__ __forceinline__ void pvm_store1(void* p, int dt, int64_t i, float x) {
@@ -60,18 +65,18 @@ __device__ __forceinline__ void pvm_store1(void* p, int dt, int64_t i, float x) 
     else static_cast<_Float16*>(p)[i] = (_Float16)x;
 }
 __device__ __forceinline__ void pvm_store4(void* p, int dt, int64_t i, pvm_f32x4 x) {
-    if (dt == 0) *reinterpret_cast<pvm_f32x4*>(static_cast<float*>(p) + i) = x;
+    if (dt == 0) *reinterpret_cast<pvm_f32x4_any*>(static_cast<float*>(p) + i) = x;
     else if (dt == 1)
-        *reinterpret_cast<pvm_u16x4*>(static_cast<unsigned short*>(p) + i) =
+        *reinterpret_cast<pvm_u16x4_any*>(static_cast<unsigned short*>(p) + i) =
             (pvm_u16x4){pvm_to_bf16(x.x), pvm_to_bf16(x.y), pvm_to_bf16(x.z), pvm_to_bf16(x.w)};
     else
-        *reinterpret_cast<pvm_f16x4*>(static_cast<_Float16*>(p) + i) =
+        *reinterpret_cast<pvm_f16x4_any*>(static_cast<_Float16*>(p) + i) =
             (pvm_f16x4){(_Float16)x.x, (_Float16)x.y, (_Float16)x.z, (_Float16)x.w};
 }
 
 // sixteen bytes of a tensor and what they hold
-template <int DT> struct PvmVec { enum { N = 8 }; typedef pvm_u16x8 V; };
-template <> struct PvmVec<0> { enum { N = 4 }; typedef pvm_f32x4 V; };
+template <int DT> struct PvmVec { enum { N = 8 }; typedef pvm_u16x8 V; typedef pvm_u16x8_any M; };
+template <> struct PvmVec<0> { enum { N = 4 }; typedef pvm_f32x4 V; typedef pvm_f32x4_any M; };
 template <int DT> __device__ __forceinline__ float pvm_get(typename PvmVec<DT>::V v, int e) {
     if constexpr (DT == 0) return v[e];
     else if constexpr (DT == 1) return pvm_bf16(v[e]);
@@ -112,38 +117,30 @@ __device__ __forceinline__ double pvm_block_sum(double s) {
 }
 
 // the sum of squares of a whole chunk (all its loads under way together) or of the end of a tensor
-template <int DT> __device__ __forceinline__ double pvm_sumsq_chunk(const void* a, int64_t i0, int64_t i1, bool vec) {
+template <int DT> __device__ __forceinline__ double pvm_sumsq_chunk(const void* a, int64_t i0, int64_t i1) {
     typedef typename PvmVec<DT>::V V;
+    typedef typename PvmVec<DT>::M M;
     enum { N = PvmVec<DT>::N, LOADS = PVM_CHUNK / N / PVM_THREADS };
     double s = 0.0;
-    int64_t i = i0 + threadIdx.x;
-    if (vec) {
-        const V* p = reinterpret_cast<const V*>(static_cast<const char*>(a) + i0 * (16 / N)) + threadIdx.x;
-        if (i1 - i0 == PVM_CHUNK) {
-            V v[LOADS];
+    auto add = [&](V v) {
 #pragma unroll
-            for (int u = 0; u < LOADS; ++u) v[u] = p[u * PVM_THREADS];
-#pragma unroll
-            for (int u = 0; u < LOADS; ++u)
-#pragma unroll
-                for (int e = 0; e < N; ++e) {
-                    const double x = pvm_get<DT>(v[u], e);
-                    s = fma(x, x, s);
-                }
-            return s;
+        for (int e = 0; e < N; ++e) {
+            const double x = pvm_get<DT>(v, e);
+            s = fma(x, x, s);
         }
-        const int whole = (int)(i1 - i0) / N;
-        for (int u = threadIdx.x; u < whole; u += PVM_THREADS, p += PVM_THREADS) {
-            const V v = *p;
+    };
+    const M* p = reinterpret_cast<const M*>(static_cast<const char*>(a) + i0 * (16 / N)) + threadIdx.x;
+    if (i1 - i0 == PVM_CHUNK) {
+        V v[LOADS];
 #pragma unroll
-            for (int e = 0; e < N; ++e) {
-                const double x = pvm_get<DT>(v, e);
-                s = fma(x, x, s);
-            }
-        }
-        i += (int64_t)whole * N;
+        for (int u = 0; u < LOADS; ++u) v[u] = p[u * PVM_THREADS];
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u) add(v[u]);
+        return s;
     }
-    for (; i < i1; i += PVM_THREADS) {
+    const int whole = (int)(i1 - i0) / N;
+    for (int u = threadIdx.x; u < whole; u += PVM_THREADS, p += PVM_THREADS) add(*p);
+    for (int64_t i = i0 + (int64_t)whole * N + threadIdx.x; i < i1; i += PVM_THREADS) {
         const double x = pvm_load1(a, DT, i);
         s = fma(x, x, s);
     }
@@ -156,7 +153,7 @@ __global__ __launch_bounds__(PVM_THREADS) void pvk_sumsq(const PvmTab T, double*
     for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
         const int t = pvm_find(T, c);
         const int64_t i0 = (int64_t)(c - T.first[t]) * PVM_CHUNK, i1 = min(T.n[t], i0 + PVM_CHUNK);
-        PVM_BY_TYPE(T.dt[t], s += pvm_sumsq_chunk<D_>(T.a[t], i0, i1, T.vec[t]));
+        PVM_BY_TYPE(T.dt[t], s += pvm_sumsq_chunk<D_>(T.a[t], i0, i1));
     }
     s = pvm_block_sum(s);
     if (threadIdx.x == 0) part[blockIdx.x] = s;
@@ -179,32 +176,29 @@ __global__ __launch_bounds__(PVM_THREADS) void pvk_norm_final(const double* __re
     if (threadIdx.x == 0) *norm = (float)n;
 }
 
-template <int DT> __device__ __forceinline__ void pvm_scale_chunk(const void* a, void* b, int64_t i0, int64_t i1, bool vec, float s) {
+template <int DT> __device__ __forceinline__ void pvm_scale_chunk(const void* a, void* b, int64_t i0, int64_t i1, float s) {
     typedef typename PvmVec<DT>::V V;
+    typedef typename PvmVec<DT>::M M;
     enum { N = PvmVec<DT>::N, LOADS = PVM_CHUNK / N / PVM_THREADS };
-    int64_t i = i0 + threadIdx.x;
-    if (vec) {
-        const V* p = reinterpret_cast<const V*>(static_cast<const char*>(a) + i0 * (16 / N)) + threadIdx.x;
-        V* q = reinterpret_cast<V*>(static_cast<char*>(b) + i0 * (16 / N)) + threadIdx.x;
-        auto scaled = [&](V v) {
-            V o;
+    const M* p = reinterpret_cast<const M*>(static_cast<const char*>(a) + i0 * (16 / N)) + threadIdx.x;
+    M* q = reinterpret_cast<M*>(static_cast<char*>(b) + i0 * (16 / N)) + threadIdx.x;
+    auto scaled = [&](V v) {
+        V o;
 #pragma unroll
-            for (int e = 0; e < N; ++e) pvm_set<DT>(o, e, pvm_get<DT>(v, e) * s);
-            return o;
-        };
-        if (i1 - i0 == PVM_CHUNK) {
-            V v[LOADS];
+        for (int e = 0; e < N; ++e) pvm_set<DT>(o, e, pvm_get<DT>(v, e) * s);
+        return o;
+    };
+    if (i1 - i0 == PVM_CHUNK) {
+        V v[LOADS];
 #pragma unroll
-            for (int u = 0; u < LOADS; ++u) v[u] = p[u * PVM_THREADS];
+        for (int u = 0; u < LOADS; ++u) v[u] = p[u * PVM_THREADS];
 #pragma unroll
-            for (int u = 0; u < LOADS; ++u) q[u * PVM_THREADS] = scaled(v[u]);
-            return;
-        }
-        const int whole = (int)(i1 - i0) / N;
-        for (int u = threadIdx.x; u < whole; u += PVM_THREADS, p += PVM_THREADS, q += PVM_THREADS) *q = scaled(*p);
-        i += (int64_t)whole * N;
+        for (int u = 0; u < LOADS; ++u) q[u * PVM_THREADS] = scaled(v[u]);
+        return;
     }
-    for (; i < i1; i += PVM_THREADS) pvm_store1(b, DT, i, pvm_load1(a, DT, i) * s);
+    const int whole = (int)(i1 - i0) / N;
+    for (int u = threadIdx.x; u < whole; u += PVM_THREADS, p += PVM_THREADS, q += PVM_THREADS) *q = scaled(*p);
+    for (int64_t i = i0 + (int64_t)whole * N + threadIdx.x; i < i1; i += PVM_THREADS) pvm_store1(b, DT, i, pvm_load1(a, DT, i) * s);
 }
 
 __global__ __launch_bounds__(PVM_THREADS) void pvk_clip_apply(const PvmTab T, const double* __restrict__ part, int nparts, double max_norm,
@@ -217,7 +211,7 @@ __global__ __launch_bounds__(PVM_THREADS) void pvk_clip_apply(const PvmTab T, co
         const int t = pvm_find(T, c);
         if (s == 1.f && T.a[t] == T.b[t]) continue;  // in place and within the bound: every value stays as it is
         const int64_t i0 = (int64_t)(c - T.first[t]) * PVM_CHUNK, i1 = min(T.n[t], i0 + PVM_CHUNK);
-        PVM_BY_TYPE(T.dt[t], pvm_scale_chunk<D_>(T.a[t], T.b[t], i0, i1, T.vec[t], s));
+        PVM_BY_TYPE(T.dt[t], pvm_scale_chunk<D_>(T.a[t], T.b[t], i0, i1, s));
     }
 }
 
@@ -247,39 +241,35 @@ __device__ __forceinline__ void pvm_adam1(float& p, float& m, float& v, float g,
 }
 
 // four elements at a time, two groups under way: parameters and moments pass once, past the caches
-template <int DT> __device__ __forceinline__ void pvm_adam_chunk(const void* a, float* p, float* m, float* v, int tile, int64_t i0, int64_t i1, bool vec,
+template <int DT> __device__ __forceinline__ void pvm_adam_chunk(const void* a, float* p, float* m, float* v, int tile, int64_t i0, int64_t i1,
                                                                  float s, float alpha, float c1, float c2, float eps) {
     auto at = [&](int64_t i) { return tile ? i + i / tile * 2 * tile : i; };  // i / tile * 3 tile + i % tile
-    int64_t i = i0 + threadIdx.x;
-    if (vec) {
-        const int whole = (int)(i1 - i0) / 4;
-        auto step = [&](pvm_f32x4 g, int64_t j, pvm_f32x4 p4, pvm_f32x4 m4, pvm_f32x4 v4) {
+    const int whole = (int)(i1 - i0) / 4;
+    auto step = [&](pvm_f32x4 g, int64_t j, pvm_f32x4 p4, pvm_f32x4 m4, pvm_f32x4 v4) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float pe = p4[e], me = m4[e], ve = v4[e];
-                pvm_adam1(pe, me, ve, g[e] * s, alpha, c1, c2, eps);
-                p4[e] = pe; m4[e] = me; v4[e] = ve;
-            }
-            __builtin_nontemporal_store(p4, reinterpret_cast<pvm_f32x4*>(p + j));
-            __builtin_nontemporal_store(m4, reinterpret_cast<pvm_f32x4*>(m + j));
-            __builtin_nontemporal_store(v4, reinterpret_cast<pvm_f32x4*>(v + j));
-        };
-        auto ld = [](const float* q) { return __builtin_nontemporal_load(reinterpret_cast<const pvm_f32x4*>(q)); };
-        int u = threadIdx.x;
-        for (; u + PVM_THREADS < whole; u += 2 * PVM_THREADS) {
-            const int64_t e0 = i0 + 4 * u, e1 = e0 + 4 * PVM_THREADS, j0 = at(e0), j1 = at(e1);
-            const pvm_f32x4 g0 = pvm_load4(a, DT, e0), p0 = ld(p + j0), m0 = ld(m + j0), v0 = ld(v + j0);
-            const pvm_f32x4 g1 = pvm_load4(a, DT, e1), p1 = ld(p + j1), m1 = ld(m + j1), v1 = ld(v + j1);
-            step(g0, j0, p0, m0, v0);
-            step(g1, j1, p1, m1, v1);
+        for (int e = 0; e < 4; ++e) {
+            float pe = p4[e], me = m4[e], ve = v4[e];
+            pvm_adam1(pe, me, ve, g[e] * s, alpha, c1, c2, eps);
+            p4[e] = pe; m4[e] = me; v4[e] = ve;
         }
-        for (; u < whole; u += PVM_THREADS) {
-            const int64_t e0 = i0 + 4 * u, j0 = at(e0);
-            step(pvm_load4(a, DT, e0), j0, ld(p + j0), ld(m + j0), ld(v + j0));
-        }
-        i += (int64_t)whole * 4;
+        __builtin_nontemporal_store(p4, reinterpret_cast<pvm_f32x4_any*>(p + j));
+        __builtin_nontemporal_store(m4, reinterpret_cast<pvm_f32x4_any*>(m + j));
+        __builtin_nontemporal_store(v4, reinterpret_cast<pvm_f32x4_any*>(v + j));
+    };
+    auto ld = [](const float* q) -> pvm_f32x4 { return __builtin_nontemporal_load(reinterpret_cast<const pvm_f32x4_any*>(q)); };
+    int u = threadIdx.x;
+    for (; u + PVM_THREADS < whole; u += 2 * PVM_THREADS) {
+        const int64_t e0 = i0 + 4 * u, e1 = e0 + 4 * PVM_THREADS, j0 = at(e0), j1 = at(e1);
+        const pvm_f32x4 g0 = pvm_load4(a, DT, e0), p0 = ld(p + j0), m0 = ld(m + j0), v0 = ld(v + j0);
+        const pvm_f32x4 g1 = pvm_load4(a, DT, e1), p1 = ld(p + j1), m1 = ld(m + j1), v1 = ld(v + j1);
+        step(g0, j0, p0, m0, v0);
+        step(g1, j1, p1, m1, v1);
     }
-    for (; i < i1; i += PVM_THREADS) {
+    for (; u < whole; u += PVM_THREADS) {
+        const int64_t e0 = i0 + 4 * u, j0 = at(e0);
+        step(pvm_load4(a, DT, e0), j0, ld(p + j0), ld(m + j0), ld(v + j0));
+    }
+    for (int64_t i = i0 + (int64_t)whole * 4 + threadIdx.x; i < i1; i += PVM_THREADS) {
         const int64_t j = at(i);
         pvm_adam1(p[j], m[j], v[j], pvm_load1(a, DT, i) * s, alpha, c1, c2, eps);
     }
@@ -298,6 +288,6 @@ __global__ __launch_bounds__(PVM_THREADS) void pvk_adam_apply(const PvmTab T, co
     for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
         const int t = pvm_find(T, c);
         const int64_t i0 = (int64_t)(c - T.first[t]) * PVM_CHUNK, i1 = min(T.n[t], i0 + PVM_CHUNK);
-        PVM_BY_TYPE(T.dt[t], pvm_adam_chunk<D_>(T.a[t], static_cast<float*>(T.b[t]), T.m[t], T.v[t], T.tile[t], i0, i1, T.vec[t], s, alpha, c1, c2, eps));
+        PVM_BY_TYPE(T.dt[t], pvm_adam_chunk<D_>(T.a[t], static_cast<float*>(T.b[t]), T.m[t], T.v[t], T.tile[t], i0, i1, s, alpha, c1, c2, eps));
     }
 }

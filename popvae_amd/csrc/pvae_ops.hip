@@ -70,17 +70,36 @@ int check_grid(int64_t blocks) {
     return 0;
 }
 
-// an operand of the tile kernel: rows x K, and whether sixteen bytes along its unit stride can be read at once
-PvdOperand operand(const void* p, int64_t rows, int64_t cols_k, int64_t sr, int64_t sk, int size) {
+// the bytes that a matrix of `rows` rows of `cols` elements reaches; an output may not meet another output or an input
+struct Extent {
+    const char* name;
+    uintptr_t lo, hi;
+};
+Extent extent(const char* name, const void* p, int64_t rows, int64_t cols, int64_t ld, int size) {
+    if (!p || rows == 0 || cols == 0) return {name, 0, 0};
+    const uintptr_t lo = reinterpret_cast<uintptr_t>(p);
+    return {name, lo, lo + (uintptr_t)(((rows - 1) * ld + cols) * size)};
+}
+int check_apart(const Extent* e, int n_out, int n) {  // e[0 .. n_out) are outputs
+    for (int i = 0; i < n_out; ++i)
+        for (int j = i + 1; j < n; ++j)
+            if (e[i].lo < e[j].hi && e[j].lo < e[i].hi) return refuse(-2, "%s overlaps %s", e[i].name, e[j].name);
+    return 0;
+}
+Extent weights_extent(const void* w, int64_t k, int64_t n, int64_t sk, int64_t sn, int size) {
+    if (!w || k == 0 || n == 0) return {"w", 0, 0};
+    const uintptr_t lo = reinterpret_cast<uintptr_t>(w);
+    return {"w", lo, lo + (uintptr_t)(((k - 1) * sk + (n - 1) * sn + 1) * size)};
+}
+
+// an operand of the tile and slim kernels: rows x K
+PvdOperand operand(const void* p, int64_t rows, int64_t cols_k, int64_t sr, int64_t sk) {
     PvdOperand o{};
     o.p = p;
     o.rows = rows;
     if (sk != 1 && sr != 1) (cols_k == 1 ? sk : sr) = 1;  // a single row or column: its stride is never used
     o.sr = sr;
     o.sk = sk;
-    const int64_t other = sk == 1 ? sr : sk;
-    const bool one = sk == 1 ? rows <= 1 : cols_k <= 1;
-    o.vec = aligned(p, 16) && (one || other * size % 16 == 0);
     return o;
 }
 void with_grad(PvdOperand& o, const float* pre, int64_t pr, int64_t pk, int act) {
@@ -88,14 +107,10 @@ void with_grad(PvdOperand& o, const float* pre, int64_t pr, int64_t pk, int act)
     o.pr = pr;
     o.pk = pk;
     o.act = act;
-    if (act != PVD_LINEAR) o.vec = o.vec && aligned(pre, 16) && (pk == 1 ? pr : pk) % 4 == 0;
 }
 PvdOut output(int64_t rows, int64_t cols, void* y, int64_t ldy, const void* bias, const void* res, int64_t ldr, float* pre, int64_t ldp,
-              int act, int size) {
-    PvdOut o{rows, cols, y, ldy, bias, res, ldr, pre, ldp, act, 0};
-    auto fits = [&](const void* p, int64_t ld, int s) { return !p || (aligned(p, 4 * s) && (rows <= 1 || ld % 4 == 0)); };
-    o.vec = fits(y, ldy, size) && fits(bias, 0, size) && fits(res, ldr, size) && fits(pre, ldp, 4);
-    return o;
+              int act) {
+    return {rows, cols, y, ldy, bias, res, ldr, pre, ldp, act};
 }
 
 // A product through the slim kernel (32 x 16 a workgroup) or the tile kernel (64 x 64), and the pieces of its contraction.
@@ -141,8 +156,7 @@ PvdRowsJob rows_job(const pvae_dense_args& a) {
     J.x = a.x; J.ldx = a.ldx;
     J.w = a.w; J.ldw = t ? a.w_sn : a.w_sk;
     J.K = a.k;
-    J.O = output(a.m, a.n, a.y, a.ldy, a.bias, a.residual, a.ldr, a.pre, a.ldp, a.act, size);
-    J.vec = aligned(a.w, 16) && J.ldw * size % 16 == 0 && (t || a.n * size % 16 == 0);
+    J.O = output(a.m, a.n, a.y, a.ldy, a.bias, a.residual, a.ldr, a.pre, a.ldp, a.act);
     J.blocks = (int)ceil_div(a.n, t ? 128 : 64 * 16 / size);
     // pieces of the contraction: to fill the chip, of 64 at least and of PVD_RK, what LDS holds of x, at most
     const int64_t pieces = std::max(ceil_div(a.k, PVD_RK), std::min<int64_t>(std::max<int64_t>(1, a.k / 64), std::max<int64_t>(1, 512 / J.blocks)));
@@ -210,7 +224,6 @@ struct NtBuilder {
         J.p = p; J.R = R; J.C = C; J.ld = ld;
         J.pre = act == PVD_LINEAR ? nullptr : pre;
         J.ldp = ldp; J.act = act;
-        J.vec = aligned(p, 16) && (R <= 1 || ld * size % 16 == 0) && (!J.pre || (aligned(pre, 16) && (R <= 1 || ldp % 4 == 0)));
         return J;
     }
     // a row stride of a laid-out operand: an odd multiple of 128 bytes, so that a tile's rows lie in all of the L2's channels
@@ -317,7 +330,7 @@ NtPlan large_dense(const pvae_dense_args& a, void* ws) {
     NtBuilder B(a.dtype, ws);
     const NtOperand x = B.operand(a.x, a.m, a.k, a.ldx, true);
     const NtOperand w = a.w_sk == 1 ? B.operand(a.w, a.n, a.k, a.w_sn, true) : B.operand(a.w, a.k, a.n, a.w_sk, false);
-    B.product(x, w, a.k, output(a.m, a.n, a.y, a.ldy, a.bias, a.residual, a.ldr, a.pre, a.ldp, a.act, B.size));
+    B.product(x, w, a.k, output(a.m, a.n, a.y, a.ldy, a.bias, a.residual, a.ldr, a.pre, a.ldp, a.act));
     B.finish();
     return B.plan;
 }
@@ -338,11 +351,11 @@ NtPlan large_bwd(const pvae_dense_bwd_args& a, void* ws) {
     }
     if (a.dx) {
         const NtOperand w = a.w_sn == 1 ? B.operand(a.w, a.k, a.n, a.w_sk, true) : B.operand(a.w, a.n, a.k, a.w_sn, false);
-        B.product(gx, w, a.n, output(a.m, a.k, a.dx, a.lddx, nullptr, a.dx_add, a.ldadd, nullptr, 0, PVD_LINEAR, B.size));
+        B.product(gx, w, a.n, output(a.m, a.k, a.dx, a.lddx, nullptr, a.dx_add, a.ldadd, nullptr, 0, PVD_LINEAR));
     }
     if (a.dw) {
         const NtOperand x = B.operand(a.x, a.m, a.k, a.ldx, false);
-        B.product(x, gw, a.m, output(a.k, a.n, a.dw, a.n, nullptr, nullptr, 0, nullptr, 0, PVD_LINEAR, B.size));
+        B.product(x, gw, a.m, output(a.k, a.n, a.dw, a.n, nullptr, nullptr, 0, nullptr, 0, PVD_LINEAR));
     }
     B.finish();
     return B.plan;
@@ -351,8 +364,8 @@ bool bwd_is_large(const pvae_dense_bwd_args& a) { return (a.dx || a.dw) && is_la
 
 PvdTileJob dense_job(const pvae_dense_args& a) {
     const int size = esize(a.dtype);
-    return tile_job(operand(a.x, a.m, a.k, a.ldx, 1, size), operand(a.w, a.n, a.k, a.w_sn, a.w_sk, size),
-                    output(a.m, a.n, a.y, a.ldy, a.bias, a.residual, a.ldr, a.pre, a.ldp, a.act, size), a.k, size, is_slim(a.m, a.n));
+    return tile_job(operand(a.x, a.m, a.k, a.ldx, 1), operand(a.w, a.n, a.k, a.w_sn, a.w_sk),
+                    output(a.m, a.n, a.y, a.ldy, a.bias, a.residual, a.ldr, a.pre, a.ldp, a.act), a.k, size, is_slim(a.m, a.n));
 }
 int check_dense(const pvae_dense_args* a) {
     if (!a) return refuse(-1, "no arguments");
@@ -367,7 +380,12 @@ int check_dense(const pvae_dense_args* a) {
         if (int rc = check_matrix("residual", a->residual, a->ldr == 0 ? 1 : a->m, a->n, a->ldr, size)) return rc;
     if (a->pre)
         if (int rc = check_matrix("pre", a->pre, a->m, a->n, a->ldp, 4)) return rc;
-    return 0;
+    const bool in_place = a->residual == a->y && (a->ldr == a->ldy || a->m <= 1);
+    const Extent e[] = {extent("y", a->y, a->m, a->n, a->ldy, size), extent("pre", a->pre, a->m, a->n, a->ldp, 4),
+                        extent("x", a->x, a->m, a->k, a->ldx, size), weights_extent(a->w, a->k, a->n, a->w_sk, a->w_sn, size),
+                        extent("bias", a->bias, 1, a->n, a->n, size),
+                        extent("residual", in_place ? nullptr : a->residual, a->m, a->n, a->ldr, size)};
+    return check_apart(e, 2, 6);
 }
 
 struct BwdPlan {
@@ -379,16 +397,16 @@ BwdPlan bwd_plan(const pvae_dense_bwd_args& a) {
     const int size = esize(a.dtype);
     BwdPlan p{};
     p.slim = is_slim(a.dx ? a.m : 0, a.k) && is_slim(a.dw ? a.k : 0, a.n);
-    PvdOperand gx = operand(a.dy, a.m, a.n, a.lddy, 1, size), gw = operand(a.dy, a.n, a.m, 1, a.lddy, size);
+    PvdOperand gx = operand(a.dy, a.m, a.n, a.lddy, 1), gw = operand(a.dy, a.n, a.m, 1, a.lddy);
     with_grad(gx, a.pre, a.ldp, 1, a.act);
     with_grad(gw, a.pre, 1, a.ldp, a.act);
     // w as an operand of dx: rows are the k of the layer, the contraction its n
     if (a.dx)
-        p.J.dx = tile_job(gx, operand(a.w, a.k, a.n, a.w_sk, a.w_sn, size),
-                          output(a.m, a.k, a.dx, a.lddx, nullptr, a.dx_add, a.ldadd, nullptr, 0, PVD_LINEAR, size), a.n, size, p.slim);
+        p.J.dx = tile_job(gx, operand(a.w, a.k, a.n, a.w_sk, a.w_sn),
+                          output(a.m, a.k, a.dx, a.lddx, nullptr, a.dx_add, a.ldadd, nullptr, 0, PVD_LINEAR), a.n, size, p.slim);
     if (a.dw)
-        p.J.dw = tile_job(operand(a.x, a.k, a.m, 1, a.ldx, size), gw,
-                          output(a.k, a.n, a.dw, a.n, nullptr, nullptr, 0, nullptr, 0, PVD_LINEAR, size), a.m, size, p.slim);
+        p.J.dw = tile_job(operand(a.x, a.k, a.m, 1, a.ldx), gw,
+                          output(a.k, a.n, a.dw, a.n, nullptr, nullptr, 0, nullptr, 0, PVD_LINEAR), a.m, size, p.slim);
     p.J.n_dx = a.dx ? (int64_t)p.J.dx.mt * p.J.dx.nt * p.J.dx.splits : 0;
     p.J.n_dw = a.dw ? (int64_t)p.J.dw.mt * p.J.dw.nt * p.J.dw.splits : 0;
     p.J.dy = a.dy;
@@ -422,7 +440,14 @@ int check_dense_bwd(const pvae_dense_bwd_args* a) {
     if (a->dw && !aligned(a->dw, size)) return refuse(-2, "dw is not aligned to its elements");
     if (a->dbias && !aligned(a->dbias, size)) return refuse(-2, "dbias is not aligned to its elements");
     if (a->dpre && !aligned(a->dpre, 4)) return refuse(-2, "dpre is not aligned to its elements");
-    return 0;
+    const bool in_place = a->dx_add == a->dx && (a->ldadd == a->lddx || a->m <= 1);
+    const Extent e[] = {extent("dx", a->dx, a->m, a->k, a->lddx, size), extent("dw", a->dw, a->k, a->n, a->n, size),
+                        extent("dbias", a->dbias, 1, a->n, a->n, size), extent("dpre", a->dpre, a->m, a->n, a->n, 4),
+                        extent("dy", a->dy, a->m, a->n, a->lddy, size), extent("pre", a->act == PVAE_LINEAR ? nullptr : a->pre, a->m, a->n, a->ldp, 4),
+                        extent("x", a->dw ? a->x : nullptr, a->m, a->k, a->ldx, size),
+                        a->dx ? weights_extent(a->w, a->k, a->n, a->w_sk, a->w_sn, size) : Extent{"w", 0, 0},
+                        extent("dx_add", in_place || !a->dx ? nullptr : a->dx_add, a->m, a->k, a->ldadd, size)};
+    return check_apart(e, 4, 9);
 }
 // ---- many tensors ----
 int check_tensors(const char* name, const pvae_tensor* t, int64_t count, bool tiles) {
@@ -476,7 +501,6 @@ template <typename Fill, typename Launch> int for_tables(const pvae_tensor* g, i
         T.a[c] = g[i].data;
         T.n[c] = g[i].n;
         T.dt[c] = (unsigned char)g[i].dtype;
-        T.vec[c] = aligned(g[i].data, 16);
         T.b[c] = nullptr;
         T.m[c] = T.v[c] = nullptr;
         T.tile[c] = 0;
@@ -632,10 +656,7 @@ int pvae_clip_by_global_norm(const pvae_tensor* g, const pvae_tensor* out, int64
         if (nparts == 0) return norm ? launch_norm(g, 0, norm, workspace, &nparts, s) : 0;
         return for_tables(
             g, count,
-            [&](PvmTab& T, int c, int64_t i) {
-                T.b[c] = out[i].data;
-                T.vec[c] = T.vec[c] && aligned(out[i].data, 16);
-            },
+            [&](PvmTab& T, int c, int64_t i) { T.b[c] = out[i].data; },
             [&](PvmTab& T) {
                 hipLaunchKernelGGL(pvk_clip_apply, dim3(std::min(2048, T.first[T.count])), dim3(PVM_THREADS), 0, s, T, (const double*)part,
                                    nparts, max_norm, norm);
@@ -694,7 +715,6 @@ int pvae_adam_step(const pvae_tensor* p, const pvae_tensor* g, const pvae_tensor
                 T.m[c] = static_cast<float*>(m[i].data);
                 T.v[c] = static_cast<float*>(v[i].data);
                 T.tile[c] = p[i].tile;
-                T.vec[c] = T.vec[c] && aligned(p[i].data, 16) && aligned(m[i].data, 16) && aligned(v[i].data, 16);
             },
             [&](PvmTab& T) {
                 hipLaunchKernelGGL(pvk_adam_apply, dim3(std::min(2048, T.first[T.count])), dim3(PVM_THREADS), 0, s, T, (const double*)part,

@@ -14,6 +14,7 @@ computed raises ValueError before anything is launched.  There is no CPU path.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import torch
 
@@ -44,6 +45,10 @@ class _Tensor(C.Structure):
     _fields_ = [("data", C.c_void_p), ("n", C.c_int64), ("dtype", C.c_int32), ("tile", C.c_int32)]
 
 
+# the same structures as bytes, which costs a call a third of what building a ctypes object does
+_pack_dense = struct.Struct("@2i3qPqP2q2PqPqPq").pack
+_pack_bwd = struct.Struct("@2i3qPqPqP2qPqPqPq3P").pack
+
 _lib = None
 
 
@@ -54,10 +59,10 @@ def lib():
         L = engine.lib()
         vp, i32, i64, f64, tp = C.c_void_p, C.c_int32, C.c_int64, C.c_double, C.POINTER(_Tensor)
         L.pvae_ops_last_error.restype = C.c_char_p
-        for name, args in (("pvae_dense", _Dense), ("pvae_dense_bwd", _DenseBwd)):
+        for name in ("pvae_dense", "pvae_dense_bwd"):
             work = getattr(L, name + "_workspace")
-            work.restype, work.argtypes = i64, [C.POINTER(args)]
-            getattr(L, name).argtypes = [C.POINTER(args), vp, i64, vp]
+            work.restype, work.argtypes = i64, [vp]
+            getattr(L, name).argtypes = [vp, vp, i64, vp]
         L.pvae_norm_workspace.restype = i64
         L.pvae_global_norm.argtypes = [tp, i64, vp, vp, i64, vp]
         L.pvae_clip_by_global_norm.argtypes = [tp, tp, i64, f64, vp, vp, i64, vp]
@@ -74,37 +79,24 @@ def _check(rc):
         raise ValueError(text)
 
 
-class _On:
-    """The tensors' device made current for a call, where it is not."""
-
-    def __init__(self, device):
-        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *a):
-        if self.guard is not None:
-            self.guard.__exit__(*a)
-
-
 def _matrix(name, t, rows, cols, dtype, device, expand=False):
     """Row stride of a [rows, cols] tensor whose rows are contiguous."""
     if t.dtype != dtype or t.device != device:
         raise ValueError(f"{name}: expected {dtype} on {device}, got {t.dtype} on {t.device}")
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
+    if t.shape != (rows, cols):
         raise ValueError(f"{name}: expected shape ({rows}, {cols}), got {tuple(t.shape)}")
-    if cols > 1 and t.stride(1) != 1:
+    ld, sn = t.stride()
+    if sn != 1 and cols > 1:
         raise ValueError(f"{name}: rows are not contiguous (strides {t.stride()})")
-    ld = t.stride(0) if rows > 1 else cols
-    if rows > 1 and ld < cols and not (expand and ld == 0):
+    if rows <= 1:
+        return cols
+    if ld < cols and not (expand and ld == 0):
         raise ValueError(f"{name}: rows overlap (strides {t.stride()})")
     return ld
 
 
 def _vector(name, t, n, dtype, device):
-    if t.dtype != dtype or t.device != device or t.dim() != 1 or t.shape[0] != n:
+    if t.dtype != dtype or t.device != device or t.shape != (n,):
         raise ValueError(f"{name}: expected {dtype} of shape ({n},) on {device}, got {t.dtype} of {tuple(t.shape)} on {t.device}")
     if n > 1 and t.stride(0) != 1:
         raise ValueError(f"{name} is not contiguous")
@@ -118,7 +110,7 @@ def _act(name):
 
 
 def _layer(x, w):
-    """Checks x [m, k] and w [k, n]; returns (type code, m, k, n, row stride of x)."""
+    """Checks x [m, k] and w [k, n]; returns (type, device, m, k, n, row stride of x)."""
     dtype, device = x.dtype, x.device
     if dtype not in DTYPES:
         raise ValueError(f"x: {dtype} is not one of float32, bfloat16, float16")
@@ -126,37 +118,32 @@ def _layer(x, w):
         raise ValueError(f"x is on {device}: the operators run on a GPU only")
     if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[0]:
         raise ValueError(f"x {tuple(x.shape)} and w {tuple(w.shape)}: expected [m, k] and [k, n]")
-    m, k = x.shape
-    n = w.shape[1]
-    ldx = _matrix("x", x, m, k, dtype, device)
     if w.dtype != dtype or w.device != device:
         raise ValueError(f"w: expected {dtype} on {device}, got {w.dtype} on {w.device}")
-    return DTYPES[dtype], m, k, n, ldx
+    m, k = x.shape
+    return dtype, device, m, k, w.shape[1], _matrix("x", x, m, k, dtype, device)
 
 
-def _spans(t):
-    """First and last byte behind a 2-D or 1-D tensor's elements."""
-    if t.numel() == 0:
-        return 0, 0
-    lo = t.data_ptr()
-    return lo, lo + (sum((s - 1) * st for s, st in zip(t.shape, t.stride())) + 1) * t.element_size()
+def _stream(device):
+    """torch's current stream of a device as a hipStream_t."""
+    return torch.cuda.current_stream(device).cuda_stream
 
 
-def _apart(outs, ins):
-    """Outputs overlap neither one another nor an input (their byte ranges)."""
-    spans = [(n, *_spans(t)) for n, t in outs if t is not None]
-    for i, (name, lo, hi) in enumerate(spans):
-        for other, t in [(o, (a, b)) for o, a, b in spans[:i]] + [(n, _spans(t)) for n, t in ins if t is not None]:
-            if lo < t[1] and t[0] < hi:
-                raise ValueError(f"{name} overlaps {other}")
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # the same without a Stream object: a microsecond less
+if _raw_stream is not None:
+    def _stream(device):  # noqa: F811
+        return _raw_stream(device.index)
 
 
-def _workspace(n, device):
-    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
+def _call(f, packed, need, device):
+    """A call whose arguments are packed; most need no workspace, and a refused one has launched nothing."""
+    rc = f(packed, None, 0, _stream(device))
+    if rc == -8:
+        n = need(packed)
+        work = torch.empty(n, dtype=torch.uint8, device=device)
+        rc = f(packed, work.data_ptr(), n, _stream(device))
+    if rc:
+        _check(rc)
 
 
 def dense(x, w, bias=None, activation="linear", residual=None, pre=None, out=None):
@@ -165,31 +152,26 @@ def dense(x, w, bias=None, activation="linear", residual=None, pre=None, out=Non
     x [m, k] (contiguous rows, any row stride), w [k, n] (a Keras kernel, or a transposed view), bias [n], residual [m, n]
     (an expanded row is fine), all of one type; sums are float32.  pre: float32 [m, n], receives ``x @ w + bias`` for
     ``dense_backward``.  out: [m, n] to write to (may be the residual), otherwise a new tensor.  Returns it."""
-    dt, m, k, n, ldx = _layer(x, w)
-    dtype, device, act = x.dtype, x.device, _act(activation)
+    dtype, device, m, k, n, ldx = _layer(x, w)
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return dense(x, w, bias, activation, residual, pre, out)
+    bp = rp = zp = ldr = ldp = 0
     if bias is not None:
         _vector("bias", bias, n, dtype, device)
-    ldr = 0 if residual is None else _matrix("residual", residual, m, n, dtype, device, expand=True)
-    ldp = 0 if pre is None else _matrix("pre", pre, m, n, torch.float32, device)
+        bp = bias.data_ptr()
+    if residual is not None:
+        ldr, rp = _matrix("residual", residual, m, n, dtype, device, expand=True), residual.data_ptr()
+    if pre is not None:
+        ldp, zp = _matrix("pre", pre, m, n, torch.float32, device), pre.data_ptr()
     if out is None:
         out, ldy = torch.empty((m, n), dtype=dtype, device=device), n
-        if pre is not None:
-            _apart([("pre", pre)], [("x", x), ("w", w), ("bias", bias), ("residual", residual)])
     else:
         ldy = _matrix("out", out, m, n, dtype, device)
-        same = residual is not None and out.data_ptr() == residual.data_ptr() and (ldr == ldy or m <= 1)
-        ins = [("x", x), ("w", w), ("bias", bias)]
-        _apart([("out", out)], ins + ([] if same else [("residual", residual)]))
-        _apart([("pre", pre), ("out", out)], ins) if pre is not None else None
-        if pre is not None and not same:
-            _apart([("pre", pre)], [("residual", residual)])
-    a = _Dense(dt, act, m, k, n, x.data_ptr(), ldx, w.data_ptr(), w.stride(0), w.stride(1), _ptr(bias), _ptr(residual), ldr,
-               out.data_ptr(), ldy, _ptr(pre), ldp)
-    L = lib()
-    with _On(device):
-        need = L.pvae_dense_workspace(a)
-        work = _workspace(need, device)
-        _check(L.pvae_dense(a, _ptr(work), need, torch.cuda.current_stream().cuda_stream))
+    sk, sn = w.stride()
+    L = _lib or lib()
+    _call(L.pvae_dense, _pack_dense(DTYPES[dtype], _act(activation), m, k, n, x.data_ptr(), ldx, w.data_ptr(), sk, sn, bp, rp, ldr,
+                                    out.data_ptr(), ldy, zp, ldp), L.pvae_dense_workspace, device)
     return out
 
 
@@ -199,24 +181,34 @@ def dense_backward(dy, x, w, pre=None, activation="linear", dx_add=None, need_dx
     dy [m, n]; x, w and activation as in the forward, pre what it left (not needed for "linear").  dx_add [m, k] is added to
     dx before its rounding: a layer whose residual is its own input passes dy.  (The gradient of the residual is dy itself;
     summed over the rows for an expanded one.)  With a 16-bit type, dy * f'(pre) is rounded to it before the two products."""
-    dt, m, k, n, ldx = _layer(x, w)
-    dtype, device, act = x.dtype, x.device, _act(activation)
+    dtype, device, m, k, n, ldx = _layer(x, w)
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return dense_backward(dy, x, w, pre, activation, dx_add, need_dx, need_dw, need_bias)
+    act = _act(activation)
     lddy = _matrix("dy", dy, m, n, dtype, device)
-    if pre is None and act:
+    zp = ldp = ap = ldadd = 0
+    if pre is not None:
+        ldp, zp = _matrix("pre", pre, m, n, torch.float32, device), pre.data_ptr()
+    elif act:
         raise ValueError(f"the gradient of {activation!r} needs pre, which dense leaves")
-    ldp = 0 if pre is None else _matrix("pre", pre, m, n, torch.float32, device)
-    ldadd = 0 if dx_add is None else _matrix("dx_add", dx_add, m, k, dtype, device, expand=True)
+    if dx_add is not None:
+        ldadd, ap = _matrix("dx_add", dx_add, m, k, dtype, device, expand=True), dx_add.data_ptr()
     dx = torch.empty((m, k), dtype=dtype, device=device) if need_dx else None
     dw = torch.empty((k, n), dtype=dtype, device=device) if need_dw else None
     db = torch.empty(n, dtype=dtype, device=device) if need_bias else None
-    a = _DenseBwd(dt, act, m, k, n, dy.data_ptr(), lddy, x.data_ptr(), ldx, w.data_ptr(), w.stride(0), w.stride(1), _ptr(pre), ldp,
-                  _ptr(dx), k, _ptr(dx_add), ldadd, _ptr(dw), _ptr(db), None)
-    L = lib()
-    with _On(device):
-        need = L.pvae_dense_bwd_workspace(a)
-        work = _workspace(need, device)
-        _check(L.pvae_dense_bwd(a, _ptr(work), need, torch.cuda.current_stream().cuda_stream))
+    sk, sn = w.stride()
+    L = _lib or lib()
+    _call(L.pvae_dense_bwd, _pack_bwd(DTYPES[dtype], act, m, k, n, dy.data_ptr(), lddy, x.data_ptr(), ldx, w.data_ptr(), sk, sn, zp, ldp,
+                                      _ptr(dx), k, ap, ldadd, _ptr(dw), _ptr(db), 0), L.pvae_dense_bwd_workspace, device)
     return dx, dw, db
+
+
+_data_ptr = torch.Tensor.data_ptr
+
+
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
 
 
 class TensorSet:
@@ -244,7 +236,7 @@ class TensorSet:
         return len(self._sizes)
 
     def _same(self):
-        if [t.data_ptr() for t in self.tensors] != self._ptrs:
+        if list(map(_data_ptr, self.tensors)) != self._ptrs:
             raise ValueError("a tensor of the set has another storage than when the set was made")
         return self._table
 
@@ -259,15 +251,22 @@ def _device_of(s):
     return s.device
 
 
+def _scratch(device):
+    """The norm that a call returns and its workspace."""
+    need = lib().pvae_norm_workspace()
+    return torch.empty((), dtype=torch.float32, device=device), torch.empty(need, dtype=torch.uint8, device=device), need
+
+
 def global_norm(tensors):
     """``sqrt(sum of squares)`` over all tensors, summed in float64: a 0-d float32 tensor."""
     s = _set(tensors)
-    device, L = _device_of(s), lib()
-    table, norm = s._same(), torch.empty((), dtype=torch.float32, device=device)
-    with _On(device):
-        need = L.pvae_norm_workspace()
-        work = _workspace(need, device)
-        _check(L.pvae_global_norm(table, len(s), norm.data_ptr(), work.data_ptr(), need, torch.cuda.current_stream().cuda_stream))
+    device = _device_of(s)
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return global_norm(s)
+    table = s._same()
+    norm, work, need = _scratch(device)
+    _check(_lib.pvae_global_norm(table, len(s), norm.data_ptr(), work.data_ptr(), need, _stream(device)))
     return norm
 
 
@@ -276,15 +275,16 @@ def clip_by_global_norm(tensors, max_norm, out=None):
     and returns the norm before clipping, a 0-d float32 tensor.  A norm that is not finite makes every output NaN."""
     s = _set(tensors)
     o = s if out is None else _set(out)
-    device, L = _device_of(s), lib()
+    device = _device_of(s)
     if len(o) != len(s) or o.device != device:
         raise ValueError("out: as many tensors as there are gradients, on their GPU")
-    table, norm = s._same(), torch.empty((), dtype=torch.float32, device=device)
-    with _On(device):
-        need = L.pvae_norm_workspace()
-        work = _workspace(need, device)
-        _check(L.pvae_clip_by_global_norm(table, o._same(), len(s), float(max_norm), norm.data_ptr(), work.data_ptr(), need,
-                                          torch.cuda.current_stream().cuda_stream))
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return clip_by_global_norm(s, max_norm, o)
+    table = s._same()
+    into = table if o is s else o._same()
+    norm, work, need = _scratch(device)
+    _check(_lib.pvae_clip_by_global_norm(table, into, len(s), float(max_norm), norm.data_ptr(), work.data_ptr(), need, _stream(device)))
     return norm
 
 
@@ -295,25 +295,23 @@ def adam_step(params, grads, m, v, step, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e
     replays read it anew).  clip_norm: the gradients enter scaled by ``min(1, clip_norm / norm)``; the norm before clipping is
     returned (a 0-d float32 tensor; None without clipping)."""
     p, g, m, v = _set(params), _set(grads), _set(m), _set(v)
-    device, L = _device_of(p), lib()
+    device = _device_of(p)
     for name, s in (("grads", g), ("m", m), ("v", v)):
         if s.device != device or s._sizes != p._sizes:
             raise ValueError(f"{name}: as many tensors of the same sizes as there are parameters, on their GPU")
-    step_dev = None
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return adam_step(p, g, m, v, step, lr, beta1, beta2, eps, clip_norm)
+    at = None
     if isinstance(step, torch.Tensor):
         if step.dtype != torch.int32 or step.numel() != 1 or step.device != device:
             raise ValueError("step: a number, or an int32 tensor of one element on the parameters' GPU")
-        step_dev, step = step.data_ptr(), 0
-    if clip_norm is not None and not clip_norm > 0:
-        raise ValueError(f"clip_norm {clip_norm}: a positive number, or None")
-    tables = [s._same() for s in (p, g, m, v)]
-    norm = work = None
-    need = 0
-    with _On(device):
-        if clip_norm is not None:
-            norm = torch.empty((), dtype=torch.float32, device=device)
-            need = L.pvae_norm_workspace()
-            work = _workspace(need, device)
-        _check(L.pvae_adam_step(*tables, len(p), lr, beta1, beta2, eps, int(step), step_dev, float(clip_norm or 0.0), _ptr(norm),
-                                _ptr(work), need, torch.cuda.current_stream().cuda_stream))
+        at, step = step.data_ptr(), 0
+    L, norm, work, need = lib(), None, None, 0
+    if clip_norm is not None:
+        if not clip_norm > 0:
+            raise ValueError(f"clip_norm {clip_norm}: a positive number, or None")
+        norm, work, need = _scratch(device)
+    _check(L.pvae_adam_step(p._same(), g._same(), m._same(), v._same(), len(p), lr, beta1, beta2, eps, int(step), at,
+                            float(clip_norm or 0.0), _ptr(norm), _ptr(work), need, _stream(device)))
     return norm

@@ -49,26 +49,55 @@ def dense_args(**kw):
     (dict(dtype=3), "type"), (dict(act=7), "activation"), (dict(m=-1), "sizes"), (dict(n=1 << 31), "sizes"), (dict(x=None), "x is NULL"),
     (dict(x=4097), "aligned"), (dict(ldx=3), "x: row stride"), (dict(ldx=1 << 60), "too large"), (dict(w_sk=7), "w: row stride"),
     (dict(w_sk=16, w_sn=2), "neither"), (dict(w_sk=1, w_sn=3), "w\\^T"), (dict(y=None), "y is NULL"), (dict(ldy=7), "y: row stride"),
-    (dict(residual=4096, ldr=5), "residual"), (dict(pre=4098, ldp=8), "pre is not aligned"), (dict(pre=4096, ldp=4), "pre: row")])
+    (dict(residual=4096, ldr=5), "residual"), (dict(pre=4098, ldp=8), "pre is not aligned"), (dict(pre=65536, ldp=4), "pre: row"), (dict(y=4096), "y overlaps x"), (dict(y=8192 + 60), "y overlaps w"),
+    (dict(pre=16384 + 32, ldp=8), "y overlaps pre"), (dict(residual=16384 + 4, ldr=8), "y overlaps residual"),
+    (dict(residual=16384, ldr=12), "y overlaps residual"), (dict(pre=4096, ldp=8, residual=16384, ldr=8), "pre overlaps x"),
+    (dict(bias=16384 + 8), "y overlaps bias")])
 def test_dense_refusals(kw, text):
     a = dense_args(**kw)
-    assert ops.lib().pvae_dense(a, None, 0, None) < 0
+    assert ops.lib().pvae_dense(C.byref(a), None, 0, None) < 0
     assert re.search(text, ops.lib().pvae_ops_last_error().decode())
-    assert ops.lib().pvae_dense_workspace(a) == 0
+    assert ops.lib().pvae_dense_workspace(C.byref(a)) == 0
+
+
+def bwd_args(**kw):
+    a = dict(dtype=0, act=2, m=2, k=4, n=8, dy=4096, lddy=8, x=8192, ldx=4, w=12288, w_sk=8, w_sn=1, pre=16384, ldp=8, dx=20480, lddx=4,
+             dx_add=None, ldadd=0, dw=24576, dbias=28672, dpre=32768)
+    a.update(kw)
+    return ops._DenseBwd(**a)
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(dtype=-1), "type"), (dict(act=9), "activation"), (dict(k=-1), "sizes"), (dict(dy=None), "dy is NULL"), (dict(lddy=7), "dy: row"),
+    (dict(pre=None), "pre is NULL"), (dict(pre=16386), "pre is not aligned"), (dict(x=None), "x is NULL"), (dict(w=None), "w is NULL"),
+    (dict(lddx=3), "dx: row"), (dict(dx_add=40960, ldadd=2), "dx_add: row"), (dict(dw=24577), "dw is not aligned"),
+    (dict(dbias=28673), "dbias is not aligned"), (dict(dpre=32769), "dpre is not aligned"), (dict(dx=4096), "dx overlaps dy"),
+    (dict(dw=8192), "dw overlaps x"), (dict(dbias=12288), "dbias overlaps w"), (dict(dpre=16384), "dpre overlaps pre"),
+    (dict(dx=24576), "dx overlaps dw"), (dict(dx_add=20484, ldadd=4), "dx overlaps dx_add")])
+def test_dense_bwd_refusals(kw, text):
+    a = bwd_args(**kw)
+    assert ops.lib().pvae_dense_bwd(C.byref(a), None, 0, None) < 0
+    assert re.search(text, ops.lib().pvae_ops_last_error().decode())
+
+
+def test_packed_arguments_are_the_structures():
+    for struct, packed in ((ops._Dense, ops._pack_dense), (ops._DenseBwd, ops._pack_bwd)):
+        values = list(range(1, len(struct._fields_) + 1))
+        assert packed(*values) == bytes(struct(*values))
 
 
 def test_empty_calls_do_nothing():
-    assert ops.lib().pvae_dense(dense_args(m=0, x=None, y=None), None, 0, None) == 0
-    assert ops.lib().pvae_dense(dense_args(n=0, w=None, y=None), None, 0, None) == 0
+    assert ops.lib().pvae_dense(C.byref(dense_args(m=0, x=None, y=None)), None, 0, None) == 0
+    assert ops.lib().pvae_dense(C.byref(dense_args(n=0, w=None, y=None)), None, 0, None) == 0
     assert ops.lib().pvae_dense(None, None, 0, None) == -1
 
 
 def test_a_missing_workspace_is_refused():
-    a = dense_args(m=64, k=100_000, n=64, ldx=100_000, w_sk=64, ldy=64)
-    need = ops.lib().pvae_dense_workspace(a)
+    a = dense_args(m=64, k=100_000, n=64, x=1 << 32, ldx=100_000, w=1 << 33, w_sk=64, y=1 << 34, ldy=64)
+    need = ops.lib().pvae_dense_workspace(C.byref(a))
     assert need > 0
     for ptr, have in ((None, need), (4096, need - 1), (4097, need)):
-        assert ops.lib().pvae_dense(a, ptr, have, None) < 0
+        assert ops.lib().pvae_dense(C.byref(a), ptr, have, None) < 0
         assert "workspace" in ops.lib().pvae_ops_last_error().decode()
 
 
