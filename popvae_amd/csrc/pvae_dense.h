@@ -603,10 +603,10 @@ template <int DT> __global__ __launch_bounds__(512) void pvk_dense_bwd_slim(cons
 }
 
 // ---------------------------------------------------------------------------------------------
-// Large products, step 1: operands that the product kernel below cannot read as they are -- rows not contiguous along the
-// contraction, not aligned to sixteen bytes, or a contraction that is no multiple of 128 bytes -- are laid out anew, and g is
-// formed from dy and z, once instead of once per tile: a source of R rows of C contiguous elements becomes [R][pad(C)]
-// and / or its transpose [C][pad(R)], zeros behind the end.  One launch for up to three sources; bound by memory.
+// Large products, step 1: operands that the product kernel below cannot read as they are -- rows not aligned to sixteen bytes,
+// or a contraction that is no multiple of 128 bytes -- are laid out anew, and g is formed from dy and z, once instead of once
+// per tile: a source of R rows of C contiguous elements becomes [pad(R)][pad(C)] or its transpose [C][pad(R)], zeros behind the
+// end.  One launch for up to three sources; bound by memory.
 // ---------------------------------------------------------------------------------------------
 struct PvdPack {
     const void* p;
@@ -614,8 +614,8 @@ struct PvdPack {
     const float* pre;  // g = p * act'(pre)
     int64_t ldp;
     int act;
-    void* same;        // [R][ld_same], the first w_same elements of a row filled, or NULL
-    int64_t ld_same, w_same;
+    void* same;        // [h_same][ld_same], the first w_same elements of a row filled, or NULL
+    int64_t ld_same, w_same, h_same;
     void* tran;        // [C][ld_tran], w_tran of a row filled, or NULL
     int64_t ld_tran, w_tran;
     float* sums;       // [row tiles][C]: column sums of 64 rows each, or NULL
@@ -685,7 +685,7 @@ template <int DT> __global__ __launch_bounds__(256) void pvk_dense_pack(const Pv
                 for (int e = 0; e < VEC; ++e)
                     if (r < J.R && c + e < J.C) J.g32[r * J.C + c + e] = f[e];
         }
-        if (same && r < J.R && c < J.w_same) *reinterpret_cast<pvd_u32x4*>(same + r * J.ld_same + c) = *reinterpret_cast<const pvd_u32x4*>(v);
+        if (same && r < J.h_same && c < J.w_same) *reinterpret_cast<pvd_u32x4*>(same + r * J.ld_same + c) = *reinterpret_cast<const pvd_u32x4*>(v);
         if (J.tran)
 #pragma unroll
             for (int e = 0; e < VEC; ++e) tile[rr * LD + run * VEC + e] = v[e];
@@ -715,17 +715,24 @@ template <int DT> __global__ __launch_bounds__(256) void pvk_dense_pack(const Pv
 }
 
 // ---------------------------------------------------------------------------------------------
-// Large products, step 2: both operands as rows of contraction, 128 bytes of every row a step.  LDS holds two steps: while the
-// matrix instructions work on one, the next arrives from memory (global_load_lds, no registers in between).  A row of 128
-// bytes is eight pieces of sixteen; piece c of row r lies at slot c ^ ((r >> 1) & 7), which spreads the sixteen rows a
-// quarter wave reads over all banks.  The direct loads write lane after lane, so the lanes choose their source accordingly.
-// Tiles are numbered so that the workgroups of one XCD (blockIdx % 8) work on neighbouring tiles and find each other's
+// Large products, step 2.  A step is 128 bytes of contraction per row of either operand.  LDS holds ST of them: while the
+// matrix instructions work on one, the next arrive from memory (global_load_lds, no registers in between).
+//   An operand whose rows run along the contraction lies in LDS row by row, a row of 128 bytes as eight pieces of sixteen; piece
+// c of row r is at slot c ^ ((r >> 1) & 7), which spreads the sixteen rows a quarter wave reads over all banks.
+//   An operand whose rows run along the other side (Keras' w in the forward, x^T and g in dw) lies there as it does in memory,
+// one line of contraction after another.  16-bit types are transposed on the way to registers (ds_read_b64_tr_b16: sixteen
+// lanes hold four lines of sixteen elements and get four lines of one element each), float32 is read element by element.
+// Pairs of pieces (float32: runs of four) of a line are exchanged by the line's number so that the lines which are read
+// together lie in different banks.
+// The direct loads write lane after lane, so the lanes choose their source accordingly.
+//   Tiles are numbered so that the workgroups of one XCD (blockIdx % 8) work on neighbouring tiles and find each other's
 // operands in their L2.
 // ---------------------------------------------------------------------------------------------
 struct PvdNtJob {
-    const char *x, *w;      // [x_rows][steps * 128 bytes], row strides ldx, ldw in bytes
+    const char *x, *w;      // [x_rows][steps * 128 bytes], row strides ldx, ldw in bytes; across: [contraction][x_rows]
     int64_t ldx, ldw;
     int x_rows, w_rows;
+    int x_across, w_across;
     int steps, per, splits; // steps of 128 bytes; of each piece; pieces
     int mt, nt, band;       // tiles; rows of tiles that go together
     PvdOut O;
@@ -740,8 +747,17 @@ struct PvdNtJobs {
     void* dbias;
 };
 
-typedef const __attribute__((address_space(1))) void* pvd_gptr;
 typedef __attribute__((address_space(3))) void* pvd_lptr;
+typedef short pvd_s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) pvd_s16x4* pvd_ltr;
+
+// Lane l's sixteen bytes at `from` go to lds + 16 l (lds: the same for the wave).  Written out because the compiler, given its
+// builtin, waits for every such load in flight before each transposing read of LDS (128 x 256 bf16 tiles: 165 us instead of
+// 121 for 4096^3); the loads are waited for in PvdNt::arrived, and write no registers.
+__device__ __forceinline__ void pvd_load_to_lds(const char* from, char* lds) {
+    const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(pvd_lptr)lds);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "memory", "m0");
+}
 
 // What follows the product for ROWS x 64 products of one wave in LDS (row r's piece u of four floats at slot u ^ (r & 15)):
 // rows m .., columns n ..; the residuals of several rows are asked for together.
@@ -780,18 +796,63 @@ template <int DT, int TM, int TN, int WM, int WN, int ST> struct PvdNt {
     enum { WAVES = WM * WN, THREADS = 64 * WAVES, BUF = (TM + TN) * 128, LDS = ST * BUF, FM = TM / WM / 16, FN = TN / WN / 16 };
     enum { LOADS = (TM + TN) / (8 * WAVES) };                          // direct loads of a wave per step
     enum { GB = FM * FN <= 16 ? FM : 16 / FN, GROUPS = 2 * FM / GB };  // a step's matrix work: groups of FN x GB fragments
-    enum { FITS = LDS / WAVES / 256, EPR = FITS < TM / WM ? FITS : TM / WM };  // rows of a wave's result that its share of LDS holds
+    enum { FITS = LDS / WAVES / 256, POW = FITS >= 128 ? 128 : FITS >= 64 ? 64 : FITS >= 32 ? 32 : 16 };
+    enum { EPR = POW < TM / WM ? POW : TM / WM };                      // rows of a wave's result that its share of LDS takes at once
     static_assert(TM % (8 * WAVES) == 0 && TN % (8 * WAVES) == 0, "rows are loaded eight per wave");
-    static_assert(FN % 4 == 0 && EPR % 16 == 0 && (TM / WM) % EPR == 0, "a wave's result goes out in pieces 64 columns wide");
+    static_assert(FN % 4 == 0 && FITS >= 16 && (TM / WM) % EPR == 0, "a wave's result goes out in pieces 64 columns wide");
 
-    // rows [row0, row0 + ROWS) of one step into LDS; rows behind the end repeat the last one (their results are dropped)
-    template <int ROWS> static __device__ __forceinline__ void fetch(const char* p, int64_t ld, int rows, int row0, int64_t at, char* lds) {
-        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    enum { SIZE = PvdType<DT>::SIZE, VEC = PvdType<DT>::VEC, KST = 128 / SIZE };  // KST: contraction of a step
+
+    // the exchange of pieces of line k of an operand across, in pieces
+    static __device__ __forceinline__ int across_swap(int k) { return DT == PVD_F32 ? 4 * ((k >> 2) & 3) : 2 * ((k & 3) | ((k >> 3 & 1) << 2)); }
+    // What this lane loads of rows [row0, row0 + ROWS) and step s: a step's rows are ROWS / 8 loads of a wave, load i lies at
+    // i * 1024 in LDS.  Rows behind the end repeat the last ones (their results are dropped).
+    template <int ROWS, bool ACROSS> struct Source {
+        enum { N = ROWS / (8 * WAVES) };
+        const char* at[N];
+        int64_t step;
+        __device__ __forceinline__ Source(const char* p, int64_t ld, int rows, int row0, int s) {
+            const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+            step = ACROSS ? KST * ld : 128;
 #pragma unroll
-        for (int u = 0; u < ROWS / (8 * WAVES); ++u) {
-            const int i = u * WAVES + wave, r = min(row0 + 8 * i + (lane >> 3), rows - 1);
-            const int piece = (lane & 7) ^ (4 * (i & 1) | (lane >> 4));
-            __builtin_amdgcn_global_load_lds((pvd_gptr)(p + r * ld + at + piece * 16), (pvd_lptr)(lds + i * 1024), 16, 0, 0);
+            for (int u = 0; u < N; ++u) {
+                const int i = u * WAVES + wave;
+                if constexpr (ACROSS) {
+                    enum { PIECES = ROWS * SIZE / 16, LINES = 64 / PIECES };  // pieces of a line, lines of a load
+                    const int k = i * LINES + lane / PIECES, piece = (lane % PIECES) ^ across_swap(k);
+                    at[u] = p + k * ld + (int64_t)min(row0 + piece * VEC, rows - VEC) * SIZE;
+                } else {
+                    const int r = min(row0 + 8 * i + (lane >> 3), rows - 1), piece = (lane & 7) ^ (4 * (i & 1) | (lane >> 4));
+                    at[u] = p + r * ld + piece * 16;
+                }
+                at[u] += s * step;
+            }
+        }
+        __device__ __forceinline__ void load(char* lds) {  // and on to the next step
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+                pvd_load_to_lds(at[u], lds + (u * WAVES + (threadIdx.x >> 6)) * 1024);
+                at[u] += step;
+            }
+        }
+    };
+    // the fragment of rows row0 .. row0 + 15 (a multiple of sixteen) and half h of a step
+    template <int ROWS, bool ACROSS> static __device__ __forceinline__ pvd_u32x4 fragment(const char* lds, int row0, int h) {
+        const int lane = threadIdx.x & 63, r16 = lane & 15, q = lane >> 4;
+        if constexpr (!ACROSS) {
+            return piece(lds, row0 + r16, 4 * h + q);
+        } else if constexpr (DT == PVD_F32) {
+            const char* at = lds + (16 * h + 4 * q) * (ROWS * 4) + ((((row0 + r16) >> 2) ^ 4 * q) << 4) + (r16 & 3) * 4;
+            pvd_u32x4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = *reinterpret_cast<const unsigned*>(at + e * (ROWS * 4));
+            return v;
+        } else {
+            const int k = 32 * h + 8 * q + (r16 >> 2);  // this lane's line of the first four; k + 4 has the same exchange
+            const char* at = lds + k * (ROWS * 2) + (((row0 >> 3) ^ across_swap(k)) << 4) + (r16 & 3) * 8;
+            const pvd_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pvd_ltr)at);
+            const pvd_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pvd_ltr)(at + 4 * (ROWS * 2)));
+            return __builtin_bit_cast(pvd_u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         }
     }
     // all but the last `steps` steps that this wave has asked for have arrived, its own reads of LDS too; then every wave's
@@ -811,7 +872,7 @@ template <int DT, int TM, int TN, int WM, int WN, int ST> struct PvdNt {
         return *reinterpret_cast<const pvd_u32x4*>(lds + r * 128 + ((c ^ ((r >> 1) & 7)) << 4));
     }
 
-    static __device__ __forceinline__ void run(const PvdNtJob& J, int block, char* smem) {
+    template <bool XA, bool WA> static __device__ __forceinline__ void run(const PvdNtJob& J, int block, char* smem) {
         const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r16 = lane & 15, q = lane >> 4;
         const int tiles = J.mt * J.nt, total = tiles * J.splits;
         // an XCD's workgroups, block % 8 apart, take consecutive tiles
@@ -828,10 +889,11 @@ template <int DT, int TM, int TN, int WM, int WN, int ST> struct PvdNt {
         for (int i = 0; i < FN; ++i)
 #pragma unroll
             for (int k = 0; k < FM; ++k) acc[i][k] = (pvd_f32x4){0.f, 0.f, 0.f, 0.f};
-        auto get = [&](int s, int slot) {
-            char* lds = smem + slot * BUF;
-            fetch<TM>(J.x, J.ldx, J.x_rows, m0, (int64_t)s * 128, lds);
-            fetch<TN>(J.w, J.ldw, J.w_rows, n0, (int64_t)s * 128, lds + TM * 128);
+        Source<TM, XA> sx(J.x, J.ldx, J.x_rows, m0, s0);
+        Source<TN, WA> sw(J.w, J.ldw, J.w_rows, n0, s0);
+        auto get = [&](int slot) {
+            sx.load(smem + slot * BUF);
+            sw.load(smem + slot * BUF + TM * 128);
         };
         // The fragments of a group are read from LDS while the group before them is multiplied, a quarter into it -- across
         // steps too: behind the first quarter of a step's last group the waves meet, and the next step's first fragments come
@@ -841,9 +903,9 @@ template <int DT, int TM, int TN, int WM, int WN, int ST> struct PvdNt {
             const int h = g / (FM / GB), k0 = g % (FM / GB) * GB;
             if (k0 == 0)
 #pragma unroll
-                for (int i = 0; i < FN; ++i) a[h][i] = piece(lds + TM * 128, wn + 16 * i + r16, 4 * h + q);
+                for (int i = 0; i < FN; ++i) a[h][i] = fragment<TN, WA>(lds + TM * 128, wn + 16 * i, h);
 #pragma unroll
-            for (int k = 0; k < GB; ++k) b[g & 1][k] = piece(lds, wm + 16 * (k0 + k) + r16, 4 * h + q);
+            for (int k = 0; k < GB; ++k) b[g & 1][k] = fragment<TM, XA>(lds, wm + 16 * (k0 + k), h);
         };
         auto multiply = [&](int g, int from, int to) {
             const int h = g / (FM / GB), k0 = g % (FM / GB) * GB;
@@ -857,13 +919,13 @@ template <int DT, int TM, int TN, int WM, int WN, int ST> struct PvdNt {
         enum { EACH = FN * GB, FIRST = EACH / 4 };
 #pragma unroll
         for (int j = 0; j < ST - 1; ++j)
-            if (s0 + j < s1) get(s0 + j, j);
+            if (s0 + j < s1) get(j);
         arrived(min(ST - 2, s1 - 1 - s0));
         read(smem, 0);
         int cur = 0;
         for (int s = s0; s < s1; ++s) {
             const char* lds = smem + cur * BUF;
-            if (s + ST - 1 < s1) get(s + ST - 1, cur == 0 ? ST - 1 : cur - 1);
+            if (s + ST - 1 < s1) get(cur == 0 ? ST - 1 : cur - 1);
 #pragma unroll
             for (int g = 0; g + 1 < GROUPS; ++g) {
                 multiply(g, 0, FIRST);
@@ -916,7 +978,11 @@ __global__ __launch_bounds__(64 * WM * WN) void pvk_dense_nt(const PvdNtJobs P) 
     const int b = blockIdx.x;
     if (b < P.first[2]) {
         const int j = b >= P.first[1];
-        return PvdNt<DT, TM, TN, WM, WN, ST>::run(P.job[j], b - P.first[j], pvd_smem);
+        typedef PvdNt<DT, TM, TN, WM, WN, ST> K;
+        const PvdNtJob& J = P.job[j];
+        if (!J.w_across) return K::template run<false, false>(J, b - P.first[j], pvd_smem);
+        if (!J.x_across) return K::template run<false, true>(J, b - P.first[j], pvd_smem);
+        return K::template run<true, true>(J, b - P.first[j], pvd_smem);
     }
     const int64_t c = (int64_t)(b - P.first[2]) * blockDim.x + threadIdx.x;
     if (c >= P.sum_cols) return;

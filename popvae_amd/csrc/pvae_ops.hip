@@ -195,15 +195,16 @@ int64_t round256(int64_t b) { return ceil_div(b, 256) * 256; }
 // [rows][K] as the product kernel reads it: where it lies, or laid out in the workspace at `at`
 struct NtOperand {
     const void* p;
-    int64_t ld;  // elements
+    int64_t ld;   // elements
     int rows;
+    bool across;  // [K][rows]: contiguous along the rows
 };
 
 struct NtPlan {
     PvdPacks packs{};
     PvdNtJobs jobs{};
     int64_t bytes = 0;     // workspace
-    int tm = 0;            // tile edge
+    int tm = 0, tn = 0;    // tile
     bool deep = false;
 };
 
@@ -228,51 +229,59 @@ struct NtBuilder {
     }
     // a row stride of a laid-out operand: an odd multiple of 128 bytes, so that a tile's rows lie in all of the L2's channels
     int64_t spread(int64_t k) const { return k * size / 128 % 2 ? k : k + 128 / size; }
-    NtOperand same(PvdPack& J) {
+    // the source's rows, as rows of the contraction (across: as its lines, whole steps of them)
+    NtOperand same(PvdPack& J, bool across) {
         J.w_same = pad_k(J.C, size);
+        J.h_same = across ? pad_k(J.R, size) : J.R;
         J.ld_same = spread(J.w_same);
-        J.same = take(J.R * J.ld_same * size);
-        return {J.same, J.ld_same, (int)J.R};
+        J.same = take(J.h_same * J.ld_same * size);
+        return across ? NtOperand{J.same, J.ld_same, (int)J.w_same, true} : NtOperand{J.same, J.ld_same, (int)J.R, false};
     }
     NtOperand transposed(PvdPack& J) {
         J.w_tran = pad_k(J.R, size);
         J.ld_tran = spread(J.w_tran);
         J.tran = take(J.C * J.ld_tran * size);
-        return {J.tran, J.ld_tran, (int)J.C};
+        return {J.tran, J.ld_tran, (int)J.C, false};
     }
-    // an operand given as memory rows (R rows of C contiguous elements): by_rows: its rows are the product's, else its columns
-    NtOperand operand(const void* p, int64_t R, int64_t C, int64_t ld, bool by_rows) {
-        if (by_rows && C * size % 128 == 0 && aligned(p, 16) && (R <= 1 || ld * size % 16 == 0)) return {p, ld, (int)R};
+    // an operand given as memory rows (R rows of C contiguous elements): by_rows: its rows are the product's, else its columns;
+    // may_across: the product takes it as it lies in that case
+    NtOperand operand(const void* p, int64_t R, int64_t C, int64_t ld, bool by_rows, bool may_across) {
+        const bool pieces = aligned(p, 16) && (R <= 1 || ld * size % 16 == 0);
+        if (by_rows && pieces && C * size % 128 == 0) return {p, ld, (int)R, false};
+        if (!by_rows && may_across && pieces && R * size % 128 == 0 && C * size % 16 == 0) return {p, ld, (int)C, true};
         PvdPack& J = source(p, R, C, ld, nullptr, 0, PVD_LINEAR);
-        return by_rows ? same(J) : transposed(J);
+        return by_rows ? same(J, false) : transposed(J);
     }
     void product(const NtOperand& x, const NtOperand& w, int64_t K, const PvdOut& O) {
         PvdNtJob& J = plan.jobs.job[plan.jobs.n++];
         J = PvdNtJob{};
-        J.x = static_cast<const char*>(x.p); J.ldx = x.ld * size; J.x_rows = x.rows;
-        J.w = static_cast<const char*>(w.p); J.ldw = w.ld * size; J.w_rows = w.rows;
+        J.x = static_cast<const char*>(x.p); J.ldx = x.ld * size; J.x_rows = x.rows; J.x_across = x.across;
+        J.w = static_cast<const char*>(w.p); J.ldw = w.ld * size; J.w_rows = w.rows; J.w_across = w.across;
         J.steps = (int)ceil_div(K * size, 128);
         J.O = O;
     }
     // tile edge, pieces, numbering; call when all products are in
     void finish() {
-        auto tile_steps = [&](int tm) {
+        auto tiles = [&](int tm, int tn, bool steps) {
             int64_t n = 0;
             for (int i = 0; i < plan.jobs.n; ++i) {
                 const PvdNtJob& J = plan.jobs.job[i];
-                n += ceil_div(J.O.rows, tm) * ceil_div(J.O.cols, tm) * J.steps;
+                n += ceil_div(J.O.rows, tm) * ceil_div(J.O.cols, tn) * (steps ? J.steps : 1);
             }
             return n;
         };
-        // 128 x 128 with eight waves, two workgroups to a CU.  float32 takes 64 x 64 (five to a CU) where 128 x 128 would give the
-        // CUs less than 40 steps each: matrix work is sixteen times slower there, and an uneven last round counts.
-        plan.tm = size == 4 && tile_steps(128) < 256 * 40 ? 64 : 128;
-        const int64_t per = std::max<int64_t>(8, ceil_div(tile_steps(plan.tm), plan.tm == 64 ? 1024 : 512));
+        // 128 x 256, three steps in LDS, one workgroup to a CU, where that gives every CU a tile (8192 x 8192 x 4096 bf16: 434 us
+        // against 464 with 128 x 128; fewer LDS reads per product); else 128 x 128, two workgroups to a CU.  float32 takes
+        // 64 x 64 (five to a CU) where 128 x 128 would give the CUs less than 40 steps each: matrix work is sixteen times
+        // slower there, and an uneven last round counts.
+        plan.tm = size == 4 && tiles(128, 128, true) < 256 * 40 ? 64 : 128;
+        plan.tn = plan.tm == 64 ? 64 : size == 2 && tiles(128, 256, false) >= 240 ? 256 : 128;
+        const int64_t per = std::max<int64_t>(8, ceil_div(tiles(plan.tm, plan.tn, true), plan.tm == 64 ? 1024 : plan.tn == 256 ? 256 : 512));
         int64_t wgs = 0;
         for (int i = 0; i < plan.jobs.n; ++i) {
             PvdNtJob& J = plan.jobs.job[i];
             J.mt = (int)ceil_div(J.O.rows, plan.tm);
-            J.nt = (int)ceil_div(J.O.cols, plan.tm);
+            J.nt = (int)ceil_div(J.O.cols, plan.tn);
             // a contraction much longer than a CU's fair share is cut into pieces (each costs a write and a read of the result)
             J.per = J.steps > 2 * per ? (int)ceil_div(J.steps, ceil_div(J.steps, per)) : std::max(1, J.steps);
             J.splits = std::max(1, (int)ceil_div(J.steps, J.per));
@@ -281,11 +290,11 @@ struct NtBuilder {
             if (J.splits > 1) J.part = static_cast<float*>(take((int64_t)J.splits * J.O.rows * J.O.cols * 4));
             wgs += (int64_t)J.mt * J.nt * J.splits;
         }
-        plan.deep = plan.tm == 128 && wgs <= 256;  // one workgroup to a CU: four steps in LDS instead of two
+        plan.deep = plan.tn == 128 && wgs <= 256;  // one workgroup to a CU: four steps in LDS instead of two
         int at = 0;
         for (int i = 0; i < plan.packs.n; ++i) {
             PvdPack& J = plan.packs.job[i];
-            J.rt = (int)ceil_div(J.tran ? J.w_tran : J.R, 64);
+            J.rt = (int)ceil_div(J.tran ? J.w_tran : J.h_same, 64);
             J.ct = (int)ceil_div(J.same ? J.w_same : J.C, 64);
             plan.packs.first[i] = at;
             at += J.rt * J.ct;
@@ -294,13 +303,18 @@ struct NtBuilder {
     }
 };
 
-template <int DT, int TM, int WM, int WN, int ST> int launch_nt(const PvdNtJobs& P, int blocks, hipStream_t s) {
-    typedef PvdNt<DT, TM, TM, WM, WN, ST> K;
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(pvk_dense_nt<DT, TM, TM, WM, WN, ST>),
+template <int DT, int TM, int TN, int WM, int WN, int ST> int launch_nt(const PvdNtJobs& P, int blocks, hipStream_t s) {
+    typedef PvdNt<DT, TM, TN, WM, WN, ST> K;
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(pvk_dense_nt<DT, TM, TN, WM, WN, ST>),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, K::LDS);
     if (e != hipSuccess) return refuse(-10, "%d bytes of LDS: %s", (int)K::LDS, hipGetErrorString(e));
-    hipLaunchKernelGGL((pvk_dense_nt<DT, TM, TM, WM, WN, ST>), dim3(blocks), dim3(K::THREADS), K::LDS, s, P);
+    hipLaunchKernelGGL((pvk_dense_nt<DT, TM, TN, WM, WN, ST>), dim3(blocks), dim3(K::THREADS), K::LDS, s, P);
     return launched("dense_nt");
+}
+template <int DT> int launch_nt16(const NtPlan& plan, int blocks, hipStream_t s) {
+    if (plan.tn == 256) return launch_nt<DT, 128, 256, 2, 4, 3>(plan.jobs, blocks, s);
+    if (plan.deep) return launch_nt<DT, 128, 128, 4, 2, 4>(plan.jobs, blocks, s);
+    return launch_nt<DT, 128, 128, 4, 2, 2>(plan.jobs, blocks, s);
 }
 int launch_large(int dt, NtPlan& plan, hipStream_t s) {
     if (plan.packs.n) {
@@ -318,8 +332,14 @@ int launch_large(int dt, NtPlan& plan, hipStream_t s) {
     if (int rc = check_grid(at)) return rc;
     int rc = 0;
     const int blocks = (int)at;
-    if (plan.tm == 64) rc = launch_nt<PVD_F32, 64, 4, 1, 2>(P, blocks, s);
-    else PVD_BY_TYPE(dt, (rc = plan.deep ? launch_nt<D_, 128, 4, 2, 4>(P, blocks, s) : launch_nt<D_, 128, 4, 2, 2>(P, blocks, s)));
+    if (dt == PVAE_F32) {
+        if (plan.tm == 64) rc = launch_nt<PVD_F32, 64, 64, 4, 1, 2>(P, blocks, s);
+        else rc = launch_nt<PVD_F32, 128, 128, 4, 2, 2>(P, blocks, s);
+    } else if (dt == PVAE_BF16) {
+        rc = launch_nt16<PVD_BF16>(plan, blocks, s);
+    } else {
+        rc = launch_nt16<PVD_F16>(plan, blocks, s);
+    }
     if (rc) return rc;
     for (int i = 0; i < P.n; ++i)
         if (P.job[i].splits > 1 && (rc = launch_join(dt, P.job[i].O, P.job[i].part, P.job[i].splits, s))) return rc;
@@ -328,19 +348,17 @@ int launch_large(int dt, NtPlan& plan, hipStream_t s) {
 
 NtPlan large_dense(const pvae_dense_args& a, void* ws) {
     NtBuilder B(a.dtype, ws);
-    const NtOperand x = B.operand(a.x, a.m, a.k, a.ldx, true);
-    const NtOperand w = a.w_sk == 1 ? B.operand(a.w, a.n, a.k, a.w_sn, true) : B.operand(a.w, a.k, a.n, a.w_sk, false);
+    const NtOperand x = B.operand(a.x, a.m, a.k, a.ldx, true, false);
+    const NtOperand w = a.w_sk == 1 ? B.operand(a.w, a.n, a.k, a.w_sn, true, true) : B.operand(a.w, a.k, a.n, a.w_sk, false, true);
     B.product(x, w, a.k, output(a.m, a.n, a.y, a.ldy, a.bias, a.residual, a.ldr, a.pre, a.ldp, a.act));
     B.finish();
     return B.plan;
 }
 NtPlan large_bwd(const pvae_dense_bwd_args& a, void* ws) {
     NtBuilder B(a.dtype, ws);
-    // g: as it lies for dx (contraction over n), transposed for dw (over m), its column sums, and unrounded if asked for
+    // g: rows of the contraction for dx (over n), lines of it for dw (over m); its column sums, and unrounded if asked for
     PvdPack& g = B.source(a.dy, a.m, a.n, a.lddy, a.pre, a.ldp, a.act);
-    NtOperand gx{}, gw{};
-    if (a.dx) gx = B.same(g);
-    if (a.dw) gw = B.transposed(g);
+    const NtOperand gw = B.same(g, true), gx{gw.p, gw.ld, (int)a.m, false};
     g.g32 = a.dpre;
     if (a.dbias) {
         g.sums = static_cast<float*>(B.take(ceil_div(a.m, 64) * a.n * 4));
@@ -350,11 +368,11 @@ NtPlan large_bwd(const pvae_dense_bwd_args& a, void* ws) {
         B.plan.jobs.dbias = a.dbias;
     }
     if (a.dx) {
-        const NtOperand w = a.w_sn == 1 ? B.operand(a.w, a.k, a.n, a.w_sk, true) : B.operand(a.w, a.n, a.k, a.w_sn, false);
+        const NtOperand w = a.w_sn == 1 ? B.operand(a.w, a.k, a.n, a.w_sk, true, true) : B.operand(a.w, a.n, a.k, a.w_sn, false, true);
         B.product(gx, w, a.n, output(a.m, a.k, a.dx, a.lddx, nullptr, a.dx_add, a.ldadd, nullptr, 0, PVD_LINEAR));
     }
     if (a.dw) {
-        const NtOperand x = B.operand(a.x, a.m, a.k, a.ldx, false);
+        const NtOperand x = B.operand(a.x, a.m, a.k, a.ldx, false, true);
         B.product(x, gw, a.m, output(a.k, a.n, a.dw, a.n, nullptr, nullptr, 0, nullptr, 0, PVD_LINEAR));
     }
     B.finish();
