@@ -753,42 +753,53 @@ typedef __attribute__((address_space(3))) pvd_s16x4* pvd_ltr;
 
 // Lane l's sixteen bytes at `from` go to lds + 16 l (lds: the same for the wave).  Written out because the compiler, given its
 // builtin, waits for every such load in flight before each transposing read of LDS (128 x 256 bf16 tiles: 165 us instead of
-// 121 for 4096^3); the loads are waited for in PvdNt::arrived, and write no registers.
+// 121 for 4096^3); the loads are waited for in PvdNt::arrived, and write no registers.  Nothing else in the kernel uses m0.
 __device__ __forceinline__ void pvd_load_to_lds(const char* from, char* lds) {
     const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(pvd_lptr)lds);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "memory");
 }
 
 // What follows the product for ROWS x 64 products of one wave in LDS (row r's piece u of four floats at slot u ^ (r & 15)):
 // rows m .., columns n ..; the residuals of several rows are asked for together.
 template <int DT, int ROWS> __device__ __forceinline__ void pvd_finish_rows(const PvdOut& O, int64_t m, int64_t n, const float* ep) {
-    enum { G = ROWS / 4 < 8 ? ROWS / 4 : 8 };
+    typedef typename PvdType<DT>::T T;
     const int lane = threadIdx.x & 63, er = lane >> 4, eu = lane & 15;  // sixteen lanes, four columns each, on a row
-    const int rows = (int)max((int64_t)0, min((int64_t)ROWS, O.rows - m));
     const int64_t c = n + 4 * eu;
-    if (c >= O.cols) return;
-    const int left = pvd_left(c, O.cols);
-    pvd_f32x4 b4 = {0.f, 0.f, 0.f, 0.f};
-    if (O.bias) b4 = pvd_load_some(O.bias, DT, c, left);
+    if (m + ROWS <= O.rows && n + 64 <= O.cols) {
+        // all of it is there: nothing but the work itself (its addresses and tests took as long as a third of the products at
+        // k = 128 in float32)
+        pvd_f32x4 b4 = {0.f, 0.f, 0.f, 0.f};
+        if (O.bias) b4 = pvm_load4(O.bias, DT, c);
+        const T* rp = static_cast<const T*>(O.res) + (m + er) * O.ldr + c;
+        float* zp = O.pre + (m + er) * O.ldp + c;
+        T* yp = static_cast<T*>(O.y) + (m + er) * O.ldy + c;
+        const int64_t rs = 4 * O.ldr, zs = 4 * O.ldp, ys = 4 * O.ldy;
 #pragma unroll 1
-    for (int r0 = er; r0 < rows; r0 += 4 * G) {
-        pvd_f32x4 r4[G];
-        if (O.res)
+        for (int i0 = 0; i0 < ROWS / 4; i0 += 4) {
+            pvd_f32x4 r4[4];
+            if (O.res)
 #pragma unroll
-            for (int g = 0; g < G; ++g)
-                if (r0 + 4 * g < rows) r4[g] = pvd_load_some(O.res, DT, (m + r0 + 4 * g) * O.ldr + c, left);
+                for (int i = 0; i < 4; ++i, rp += rs) r4[i] = pvm_load4(rp, DT, 0);
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-            const int r = r0 + 4 * g;
-            if (r >= rows) break;
-            pvd_f32x4 z = *reinterpret_cast<const pvd_f32x4*>(ep + r * 64 + ((eu ^ (r & 15)) << 2));
-            z += b4;
-            if (O.pre) pvd_store_some(O.pre, 0, (m + r) * O.ldp + c, z, left);
-            pvd_f32x4 o = pvd_act4(z, O.act);
-            if (O.res) o += r4[g];
-            pvd_store_some(O.y, DT, (m + r) * O.ldy + c, o, left);
+            for (int i = 0; i < 4; ++i) {
+                const int r = 4 * (i0 + i) + er;
+                pvd_f32x4 z = *reinterpret_cast<const pvd_f32x4*>(ep + r * 64 + ((eu ^ (4 * i | er)) << 2));
+                z += b4;
+                if (O.pre) {
+                    pvm_store4(zp, 0, 0, z);
+                    zp += zs;
+                }
+                pvd_f32x4 o = pvd_act4(z, O.act);
+                if (O.res) o += r4[i];
+                pvm_store4(yp, DT, 0, o);
+                yp += ys;
+            }
         }
+        return;
     }
+#pragma unroll 1
+    for (int r = er; r < ROWS; r += 4)
+        pvd_finish4<DT>(O, m + r, c, *reinterpret_cast<const pvd_f32x4*>(ep + r * 64 + ((eu ^ (r & 15)) << 2)));
 }
 
 // TM x TN: tile (x's rows, the weights' columns); WM x WN: waves; ST: steps that LDS holds

@@ -204,7 +204,7 @@ struct NtPlan {
     PvdPacks packs{};
     PvdNtJobs jobs{};
     int64_t bytes = 0;     // workspace
-    int tm = 0, tn = 0;    // tile
+    int tile = 0;          // its edge
     bool deep = false;
 };
 
@@ -262,35 +262,34 @@ struct NtBuilder {
     }
     // tile edge, pieces, numbering; call when all products are in
     void finish() {
-        auto tiles = [&](int tm, int tn, bool steps) {
+        auto tile_steps = [&](int edge) {
             int64_t n = 0;
             for (int i = 0; i < plan.jobs.n; ++i) {
                 const PvdNtJob& J = plan.jobs.job[i];
-                n += ceil_div(J.O.rows, tm) * ceil_div(J.O.cols, tn) * (steps ? J.steps : 1);
+                n += ceil_div(J.O.rows, edge) * ceil_div(J.O.cols, edge) * J.steps;
             }
             return n;
         };
-        // 128 x 256, three steps in LDS, one workgroup to a CU, where that gives every CU a tile (8192 x 8192 x 4096 bf16: 434 us
-        // against 464 with 128 x 128; fewer LDS reads per product); else 128 x 128, two workgroups to a CU.  float32 takes
-        // 64 x 64 (five to a CU) where 128 x 128 would give the CUs less than 40 steps each: matrix work is sixteen times
-        // slower there, and an uneven last round counts.
-        plan.tm = size == 4 && tiles(128, 128, true) < 256 * 40 ? 64 : 128;
-        plan.tn = plan.tm == 64 ? 64 : size == 2 && tiles(128, 256, false) >= 240 ? 256 : 128;
-        const int64_t per = std::max<int64_t>(8, ceil_div(tiles(plan.tm, plan.tn, true), plan.tm == 64 ? 1024 : plan.tn == 256 ? 256 : 512));
-        int64_t wgs = 0;
+        // 128 x 128 with eight waves, two workgroups to a CU (4096^3 bf16 with residual and z: 147 us; 128 x 256, one workgroup to
+        // a CU, whose results nothing hides: 163; the products alone are 124 and 121).  float32 takes 64 x 64 (five to a CU)
+        // where 128 x 128 would give the CUs less than 40 steps each: matrix work is sixteen times slower there, and an
+        // uneven last round counts.
+        plan.tile = size == 4 && tile_steps(128) < 256 * 40 ? 64 : 128;
+        const int64_t per = std::max<int64_t>(8, ceil_div(tile_steps(plan.tile), plan.tile == 64 ? 1024 : 512));
+        int64_t tiles = 0;
         for (int i = 0; i < plan.jobs.n; ++i) {
             PvdNtJob& J = plan.jobs.job[i];
-            J.mt = (int)ceil_div(J.O.rows, plan.tm);
-            J.nt = (int)ceil_div(J.O.cols, plan.tn);
+            J.mt = (int)ceil_div(J.O.rows, plan.tile);
+            J.nt = (int)ceil_div(J.O.cols, plan.tile);
             // a contraction much longer than a CU's fair share is cut into pieces (each costs a write and a read of the result)
             J.per = J.steps > 2 * per ? (int)ceil_div(J.steps, ceil_div(J.steps, per)) : std::max(1, J.steps);
             J.splits = std::max(1, (int)ceil_div(J.steps, J.per));
             // a band's rows of tiles keep their operand in an XCD's L2 while the columns pass by
-            J.band = (int)std::min<int64_t>(J.mt, std::max<int64_t>(4, (1 << 20) / ((int64_t)plan.tm * J.per * 128)));
+            J.band = (int)std::min<int64_t>(J.mt, std::max<int64_t>(4, (1 << 20) / ((int64_t)plan.tile * J.per * 128)));
             if (J.splits > 1) J.part = static_cast<float*>(take((int64_t)J.splits * J.O.rows * J.O.cols * 4));
-            wgs += (int64_t)J.mt * J.nt * J.splits;
+            tiles += (int64_t)J.mt * J.nt * J.splits;
         }
-        plan.deep = plan.tn == 128 && wgs <= 256;  // one workgroup to a CU: four steps in LDS instead of two
+        plan.deep = plan.tile == 128 && tiles <= 256;  // one workgroup to a CU: four steps in LDS instead of two
         int at = 0;
         for (int i = 0; i < plan.packs.n; ++i) {
             PvdPack& J = plan.packs.job[i];
@@ -303,18 +302,13 @@ struct NtBuilder {
     }
 };
 
-template <int DT, int TM, int TN, int WM, int WN, int ST> int launch_nt(const PvdNtJobs& P, int blocks, hipStream_t s) {
-    typedef PvdNt<DT, TM, TN, WM, WN, ST> K;
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(pvk_dense_nt<DT, TM, TN, WM, WN, ST>),
+template <int DT, int TM, int WM, int WN, int ST> int launch_nt(const PvdNtJobs& P, int blocks, hipStream_t s) {
+    typedef PvdNt<DT, TM, TM, WM, WN, ST> K;
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(pvk_dense_nt<DT, TM, TM, WM, WN, ST>),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, K::LDS);
     if (e != hipSuccess) return refuse(-10, "%d bytes of LDS: %s", (int)K::LDS, hipGetErrorString(e));
-    hipLaunchKernelGGL((pvk_dense_nt<DT, TM, TN, WM, WN, ST>), dim3(blocks), dim3(K::THREADS), K::LDS, s, P);
+    hipLaunchKernelGGL((pvk_dense_nt<DT, TM, TM, WM, WN, ST>), dim3(blocks), dim3(K::THREADS), K::LDS, s, P);
     return launched("dense_nt");
-}
-template <int DT> int launch_nt16(const NtPlan& plan, int blocks, hipStream_t s) {
-    if (plan.tn == 256) return launch_nt<DT, 128, 256, 2, 4, 3>(plan.jobs, blocks, s);
-    if (plan.deep) return launch_nt<DT, 128, 128, 4, 2, 4>(plan.jobs, blocks, s);
-    return launch_nt<DT, 128, 128, 4, 2, 2>(plan.jobs, blocks, s);
 }
 int launch_large(int dt, NtPlan& plan, hipStream_t s) {
     if (plan.packs.n) {
@@ -328,18 +322,12 @@ int launch_large(int dt, NtPlan& plan, hipStream_t s) {
         if (i < P.n) at += (int64_t)P.job[i].mt * P.job[i].nt * P.job[i].splits;
     }
     P.first[2] = (int)at;
-    if (P.dbias) at += ceil_div(P.sum_cols, plan.tm == 128 ? 512 : 256);
+    if (P.dbias) at += ceil_div(P.sum_cols, plan.tile == 128 ? 512 : 256);
     if (int rc = check_grid(at)) return rc;
     int rc = 0;
     const int blocks = (int)at;
-    if (dt == PVAE_F32) {
-        if (plan.tm == 64) rc = launch_nt<PVD_F32, 64, 64, 4, 1, 2>(P, blocks, s);
-        else rc = launch_nt<PVD_F32, 128, 128, 4, 2, 2>(P, blocks, s);
-    } else if (dt == PVAE_BF16) {
-        rc = launch_nt16<PVD_BF16>(plan, blocks, s);
-    } else {
-        rc = launch_nt16<PVD_F16>(plan, blocks, s);
-    }
+    if (plan.tile == 64) rc = launch_nt<PVD_F32, 64, 4, 1, 2>(P, blocks, s);
+    else PVD_BY_TYPE(dt, (rc = plan.deep ? launch_nt<D_, 128, 4, 2, 4>(P, blocks, s) : launch_nt<D_, 128, 4, 2, 2>(P, blocks, s)));
     if (rc) return rc;
     for (int i = 0; i < P.n; ++i)
         if (P.job[i].splits > 1 && (rc = launch_join(dt, P.job[i].O, P.job[i].part, P.job[i].splits, s))) return rc;
