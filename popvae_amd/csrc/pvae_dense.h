@@ -136,7 +136,7 @@ struct PvdOperand {  // element (row, k) at p[row * sr + k * sk]; one of the str
 
 enum { PVD_T = 64, PVD_LDB = 144 };  // tile edge; bytes of an LDS row: 128 and 16 that spread the rows over the banks
 
-template <int DT, bool GRAD> struct PvdStage {
+template <int DT> struct PvdStage {
     typedef typename PvdType<DT>::T T;
     enum { VEC = PvdType<DT>::VEC, KS = 128 / PvdType<DT>::SIZE };
     alignas(16) T r[2][VEC];
@@ -144,7 +144,6 @@ template <int DT, bool GRAD> struct PvdStage {
     // one run of VEC elements along the unit stride: first element (row, k), `along_k` which way it runs
     __device__ __forceinline__ void run(const PvdOperand& P, int64_t row, int64_t k, int64_t k1, bool along_k, T* o) {
         const T* p = static_cast<const T*>(P.p) + row * P.sr + k * P.sk;
-        const float* z = GRAD ? P.pre + row * P.pr + k * P.pk : nullptr;
         const int64_t left = along_k ? k1 - k : P.rows - row;
         if (row >= P.rows || k >= k1 || left <= 0) {
 #pragma unroll
@@ -153,24 +152,10 @@ template <int DT, bool GRAD> struct PvdStage {
         }
         if (left >= VEC) {
             *reinterpret_cast<pvd_u32x4*>(o) = *reinterpret_cast<const pvd_u32x4_any*>(p);
-            if (GRAD && P.act != PVD_LINEAR) {
-#pragma unroll
-                for (int e = 0; e < VEC; e += 4) {
-                    const pvd_f32x4 d4 = pvd_act_grad4(pvm_load4(z, 0, e), P.act);
-#pragma unroll
-                    for (int f = 0; f < 4; ++f) o[e + f] = pvd_from_f32<DT>(pvd_to_f32<DT>(o[e + f]) * d4[f]);
-                }
-            }
             return;
         }
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            o[e] = T(0);
-            if (e < left) {
-                o[e] = p[e];
-                if (GRAD && P.act != PVD_LINEAR) o[e] = pvd_from_f32<DT>(pvd_to_f32<DT>(p[e]) * pvd_act_grad(z[e], P.act));
-            }
-        }
+        for (int e = 0; e < VEC; ++e) o[e] = e < left ? p[e] : T(0);
     }
     __device__ __forceinline__ void load(const PvdOperand& P, int64_t row0, int64_t k0, int64_t k1, int tid) {
         if (P.sk == 1) {
@@ -219,15 +204,14 @@ template <int DT> __device__ __forceinline__ pvd_f32x4 pvd_mfma16(pvd_u32x4 a, p
 }
 
 // products of x's rows [m0, m0 + 64) and the weights' columns [n0, n0 + 64) over k0 .. k1, into acc[column group][row group]
-template <int DT, bool GX, bool GW>
+template <int DT>
 __device__ __forceinline__ void pvd_tile(const PvdOperand& X, const PvdOperand& W, int64_t m0, int64_t n0, int64_t k0, int64_t k1,
                                          char* smem, pvd_f32x4 (&acc)[2][2]) {
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 15, q = lane >> 4;
     const int wm = (wave & 1) * 32, wn = (wave >> 1) * 32;
     char *xs = smem, *ws = smem + PVD_T * PVD_LDB;
-    PvdStage<DT, GX> sx;
-    PvdStage<DT, GW> sw;
-    enum { KS = PvdStage<DT, GX>::KS };
+    PvdStage<DT> sx, sw;
+    enum { KS = PvdStage<DT>::KS };
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -269,14 +253,15 @@ struct PvdTileJob {
     float* part;         // splits > 1: [piece][rows][cols] float32
 };
 
-template <int DT, bool GX, bool GW> __device__ __forceinline__ void pvd_tile_job(const PvdTileJob& J, int64_t block, char* smem) {
+template <int DT> __global__ __launch_bounds__(256) void pvk_dense_tile(const PvdTileJob J) {
+    __shared__ __attribute__((aligned(16))) char smem[2 * PVD_T * PVD_LDB];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t tiles = (int64_t)J.mt * J.nt;
-    const int piece = (int)(block / tiles);
-    const int64_t t = block % tiles, m0 = t / J.nt * PVD_T, n0 = t % J.nt * PVD_T;
+    const int piece = (int)(blockIdx.x / tiles);
+    const int64_t t = blockIdx.x % tiles, m0 = t / J.nt * PVD_T, n0 = t % J.nt * PVD_T;
     const int64_t k0 = piece * J.kper, k1 = min(J.K, k0 + J.kper);
     pvd_f32x4 acc[2][2];
-    pvd_tile<DT, GX, GW>(J.X, J.W, m0, n0, k0, k1, smem, acc);
+    pvd_tile<DT>(J.X, J.W, m0, n0, k0, k1, smem, acc);
     const int64_t m = m0 + (wave & 1) * 32 + (lane & 15), n = n0 + (wave >> 1) * 32 + (lane >> 4) * 4;
 #pragma unroll
     for (int j = 0; j < 2; ++j)
@@ -284,13 +269,8 @@ template <int DT, bool GX, bool GW> __device__ __forceinline__ void pvd_tile_job
         for (int i = 0; i < 2; ++i) {
             const int64_t mm = m + 16 * j, nn = n + 16 * i;
             if (J.splits == 1) pvd_finish4<DT>(J.O, mm, nn, acc[i][j]);
-            else if (mm < J.O.rows) pvd_store_some(J.part, 0, (piece * J.O.rows + mm) * J.O.cols + nn, acc[i][j], pvd_left(nn, J.O.cols));
+            else if (mm < J.O.rows && nn < J.O.cols) pvd_store_some(J.part, 0, (piece * J.O.rows + mm) * J.O.cols + nn, acc[i][j], pvd_left(nn, J.O.cols));
         }
-}
-
-template <int DT> __global__ __launch_bounds__(256) void pvk_dense_tile(const PvdTileJob J) {
-    __shared__ __attribute__((aligned(16))) char smem[2 * PVD_T * PVD_LDB];
-    pvd_tile_job<DT, false, false>(J, blockIdx.x, smem);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -372,7 +352,7 @@ template <int DT> __global__ __launch_bounds__(512) void pvk_dense_slim(const Pv
 }
 
 // ---------------------------------------------------------------------------------------------
-// The rows kernel, for up to eight rows (one point asked for an answer): the weights are read once, and that is its time.  A
+// The rows kernel, for up to four rows (one point asked for an answer): the weights are read once, and that is its time.  A
 // lane holds sixteen bytes of a row of w and all rows' sums of those columns in registers; x, as float32, comes from LDS.  The workgroup's eight waves, and pieces of the grid, split the contraction.
 // w^T (contiguous along the contraction): sixteen lanes share a column instead and add up at the end.
 // ---------------------------------------------------------------------------------------------
@@ -562,14 +542,14 @@ struct PvdBwdJob {
 };
 
 // 64 columns of dbias (and of dpre): the workgroup's waves take rows in turn
-template <int DT, int WAVES> __device__ __forceinline__ void pvd_bias_job(const PvdBwdJob& J, int64_t block, float* red) {
+template <int DT> __device__ __forceinline__ void pvd_bias_job(const PvdBwdJob& J, int64_t block, float* red) {
     typedef typename PvdType<DT>::T T;
     const int c = threadIdx.x & 63, g = threadIdx.x >> 6;
     const int64_t n = block * 64 + c;
     float s = 0.f;
     if (n < J.n) {
 #pragma unroll 4
-        for (int64_t m = g; m < J.m; m += WAVES) {
+        for (int64_t m = g; m < J.m; m += PVD_SW) {
             float v = pvd_to_f32<DT>(static_cast<const T*>(J.dy)[m * J.lddy + n]);
             if (J.act != PVD_LINEAR) v *= pvd_act_grad(J.pre[m * J.ldp + n], J.act);
             if (J.dpre) J.dpre[m * J.n + n] = v;
@@ -580,26 +560,18 @@ template <int DT, int WAVES> __device__ __forceinline__ void pvd_bias_job(const 
     __syncthreads();
     if (g == 0 && n < J.n && J.dbias) {
 #pragma unroll
-        for (int w = 1; w < WAVES; ++w) s += red[64 * w + c];
+        for (int w = 1; w < PVD_SW; ++w) s += red[64 * w + c];
         static_cast<T*>(J.dbias)[n] = pvd_from_f32<DT>(s);
     }
 }
 
-template <int DT> __global__ __launch_bounds__(256) void pvk_dense_bwd_tile(const PvdBwdJob J) {
-    __shared__ __attribute__((aligned(16))) char smem[2 * PVD_T * PVD_LDB];
-    int64_t b = blockIdx.x;
-    if (b < J.n_dx) return pvd_tile_job<DT, true, false>(J.dx, b, smem);
-    b -= J.n_dx;
-    if (b < J.n_dw) return pvd_tile_job<DT, false, true>(J.dw, b, smem);
-    pvd_bias_job<DT, 4>(J, b - J.n_dw, reinterpret_cast<float*>(smem));
-}
 template <int DT> __global__ __launch_bounds__(512) void pvk_dense_bwd_slim(const PvdBwdJob J) {
     __shared__ __attribute__((aligned(16))) float red[PVD_SW * PVD_SM * PVD_SN];
     int64_t b = blockIdx.x;
     if (b < J.n_dx) return pvd_slim_job<DT, true, false>(J.dx, b, red);
     b -= J.n_dx;
     if (b < J.n_dw) return pvd_slim_job<DT, false, true>(J.dw, b, red);
-    pvd_bias_job<DT, PVD_SW>(J, b - J.n_dw, red);
+    pvd_bias_job<DT>(J, b - J.n_dw, red);
 }
 
 // ---------------------------------------------------------------------------------------------

@@ -113,9 +113,33 @@ PvdOut output(int64_t rows, int64_t cols, void* y, int64_t ldy, const void* bias
     return {rows, cols, y, ldy, bias, res, ldr, pre, ldp, act};
 }
 
-// A product through the slim kernel (32 x 16 a workgroup) or the tile kernel (64 x 64), and the pieces of its contraction.
-// Slim while its workgroups find room on the chip at once: what counts then is one round trip to memory, not bytes.
-bool is_slim(int64_t rows, int64_t cols) { return ceil_div(rows, PVD_SM) * ceil_div(cols, PVD_SN) <= 1024; }
+// Which kernel makes y (microseconds, float32 / bf16, w as Keras keeps it):
+//                        rows         slim         tile         large
+//      1 x 4096 x 4096   21.1 / 11.0  36.9 / 31.7  37.9 / 19.1  29.3 / 14.2
+//     32 x 1024 x 1024                 9.0 /  7.1  13.3 / 10.9  13.0 / 16.6
+//    256 x  512 x  512                 7.0 /  6.0  13.0 / 11.4  16.4 / 12.8
+//     64 x 4096 x 4096                55.0 / 48.5  41.3 / 24.2  34.3 / 16.7
+//   1000 x   16 x 4000                47.8 / 98.9  13.1 / 10.6  15.5 / 14.3
+//   1000 x  128 x 1000                16.6 / 21.9  11.7 /  8.9   9.5 / 11.1
+enum Kernel { ROWS, SLIM, TILE, LARGE };
+Kernel dense_kernel(int64_t m, int64_t k, int64_t n, int size) {
+    // a few rows: the weights pass once
+    if (m <= 4 && k > 0) return ROWS;
+    // a small result: its workgroups all find room, and what they read over and over (48 rows of contraction each) stays small
+    const int64_t slim = ceil_div(m, PVD_SM) * ceil_div(n, PVD_SN);
+    if (slim <= (size == 4 ? 1024 : 512) && slim * 48 * k <= int64_t(16) << 20) return SLIM;
+    // a short contraction never fills the large kernel's pipeline; 16-bit products are over sooner
+    if (size == 4 ? k >= 64 : k >= 1024 || (double)m * n * k >= 2147483648.0) return LARGE;
+    return TILE;
+}
+// The gradients: slim while what its workgroups read stays small (every value of g is formed anew for each), else large, which
+// forms g once (500 x 29 x 700: slim 16.2 / 21.1 us, large 25.9 / 20.1; 256 x 512 x 512: 23.5 / 35.2 and 20.5 / 15.9;
+// 4000 x 64 x 64, where the slim kernel sums db over long columns: 118 / 157 and 24.4 / 24.7)
+Kernel bwd_kernel(const pvae_dense_bwd_args& a) {
+    const int64_t dx = a.dx ? ceil_div(a.m, PVD_SM) * ceil_div(a.k, PVD_SN) : 0, dw = a.dw ? ceil_div(a.k, PVD_SM) * ceil_div(a.n, PVD_SN) : 0;
+    const int64_t reads = dx * 48 * a.n + dw * 48 * a.m, most = esize(a.dtype) == 4 ? int64_t(7) << 20 : int64_t(3) << 19;
+    return a.m <= 512 && dx + dw <= 1024 && reads <= most ? SLIM : LARGE;
+}
 PvdTileJob tile_job(const PvdOperand& X, const PvdOperand& W, const PvdOut& O, int64_t K, int size, bool slim) {
     PvdTileJob J{X, W, O, K, (int)ceil_div(O.rows, slim ? PVD_SM : PVD_T), (int)ceil_div(O.cols, slim ? PVD_SN : PVD_T), 1, 0, nullptr};
     // pieces: while CUs would be left without work, each with a few steps of the kernel's loop at least
@@ -146,8 +170,7 @@ int launch_join(int dt, const PvdOut& O, const float* part, int pieces, hipStrea
     return launched("dense_join");
 }
 
-// ---- up to eight rows: the weights read once ----
-bool is_rows(const pvae_dense_args& a) { return a.m <= 8 && a.k > 0; }
+// ---- a few rows: the weights read once ----
 bool rows_transposed(const pvae_dense_args& a) { return a.n > 1 ? a.w_sn != 1 : a.w_sk == 1; }  // w's columns are contiguous
 PvdRowsJob rows_job(const pvae_dense_args& a) {
     const int size = esize(a.dtype);
@@ -177,18 +200,13 @@ int run_rows(const pvae_dense_args& a, PvdRowsJob J, void* workspace, hipStream_
     PVD_BY_TYPE(a.dtype, {
         if (a.m == 1) launch_rows<D_, 1>(J, t, s);
         else if (a.m == 2) launch_rows<D_, 2>(J, t, s);
-        else if (a.m <= 4) launch_rows<D_, 4>(J, t, s);
-        else launch_rows<D_, 8>(J, t, s);
+        else launch_rows<D_, 4>(J, t, s);
     });
     if (int rc = launched("dense_rows")) return rc;
     return J.splits > 1 ? launch_join(a.dtype, J.O, J.part, J.splits, s) : 0;
 }
 
 // ---- large products: operands laid out (pvk_dense_pack) where they have to be, then pvk_dense_nt ----
-// A product goes this way when both its sides fill most of a tile, its contraction gives the pipeline some steps, and the
-// whole is large enough to pay for the launches.
-bool is_large(int64_t m, int64_t n, int64_t k) { return m >= 96 && n >= 96 && k >= 64 && (double)m * n * k >= 1 << 25; }
-
 int64_t pad_k(int64_t k, int size) { return ceil_div(k, 128 / size) * (128 / size); }
 int64_t round256(int64_t b) { return ceil_div(b, 256) * 256; }
 
@@ -326,6 +344,7 @@ int launch_large(int dt, NtPlan& plan, hipStream_t s) {
     if (int rc = check_grid(at)) return rc;
     int rc = 0;
     const int blocks = (int)at;
+    if (blocks == 0) return 0;
     if (plan.tile == 64) rc = launch_nt<PVD_F32, 64, 4, 1, 2>(P, blocks, s);
     else PVD_BY_TYPE(dt, (rc = plan.deep ? launch_nt<D_, 128, 4, 2, 4>(P, blocks, s) : launch_nt<D_, 128, 4, 2, 2>(P, blocks, s)));
     if (rc) return rc;
@@ -366,12 +385,10 @@ NtPlan large_bwd(const pvae_dense_bwd_args& a, void* ws) {
     B.finish();
     return B.plan;
 }
-bool bwd_is_large(const pvae_dense_bwd_args& a) { return (a.dx || a.dw) && is_large(a.m, a.n, a.k) && a.k >= 96; }
-
-PvdTileJob dense_job(const pvae_dense_args& a) {
+PvdTileJob dense_job(const pvae_dense_args& a, bool slim) {
     const int size = esize(a.dtype);
     return tile_job(operand(a.x, a.m, a.k, a.ldx, 1), operand(a.w, a.n, a.k, a.w_sn, a.w_sk),
-                    output(a.m, a.n, a.y, a.ldy, a.bias, a.residual, a.ldr, a.pre, a.ldp, a.act), a.k, size, is_slim(a.m, a.n));
+                    output(a.m, a.n, a.y, a.ldy, a.bias, a.residual, a.ldr, a.pre, a.ldp, a.act), a.k, size, slim);
 }
 int check_dense(const pvae_dense_args* a) {
     if (!a) return refuse(-1, "no arguments");
@@ -397,22 +414,20 @@ int check_dense(const pvae_dense_args* a) {
 struct BwdPlan {
     PvdBwdJob J;
     int64_t n_db;
-    bool slim;  // both products through the slim kernel
 };
 BwdPlan bwd_plan(const pvae_dense_bwd_args& a) {
     const int size = esize(a.dtype);
     BwdPlan p{};
-    p.slim = is_slim(a.dx ? a.m : 0, a.k) && is_slim(a.dw ? a.k : 0, a.n);
     PvdOperand gx = operand(a.dy, a.m, a.n, a.lddy, 1), gw = operand(a.dy, a.n, a.m, 1, a.lddy);
     with_grad(gx, a.pre, a.ldp, 1, a.act);
     with_grad(gw, a.pre, 1, a.ldp, a.act);
     // w as an operand of dx: rows are the k of the layer, the contraction its n
     if (a.dx)
         p.J.dx = tile_job(gx, operand(a.w, a.k, a.n, a.w_sk, a.w_sn),
-                          output(a.m, a.k, a.dx, a.lddx, nullptr, a.dx_add, a.ldadd, nullptr, 0, PVD_LINEAR), a.n, size, p.slim);
+                          output(a.m, a.k, a.dx, a.lddx, nullptr, a.dx_add, a.ldadd, nullptr, 0, PVD_LINEAR), a.n, size, true);
     if (a.dw)
         p.J.dw = tile_job(operand(a.x, a.k, a.m, 1, a.ldx), gw,
-                          output(a.k, a.n, a.dw, a.n, nullptr, nullptr, 0, nullptr, 0, PVD_LINEAR), a.m, size, p.slim);
+                          output(a.k, a.n, a.dw, a.n, nullptr, nullptr, 0, nullptr, 0, PVD_LINEAR), a.m, size, true);
     p.J.n_dx = a.dx ? (int64_t)p.J.dx.mt * p.J.dx.nt * p.J.dx.splits : 0;
     p.J.n_dw = a.dw ? (int64_t)p.J.dw.mt * p.J.dw.nt * p.J.dw.splits : 0;
     p.J.dy = a.dy;
@@ -558,49 +573,52 @@ const char* pvae_ops_last_error(void) { return g_err; }
 
 int64_t pvae_dense_workspace(const pvae_dense_args* a) {
     if (check_dense(a) || a->m == 0 || a->n == 0) return 0;
-    if (is_rows(*a)) return rows_bytes(rows_job(*a));
-    if (is_large(a->m, a->n, a->k)) return large_dense(*a, nullptr).bytes;
-    return tile_job_bytes(dense_job(*a));
+    switch (dense_kernel(a->m, a->k, a->n, esize(a->dtype))) {
+        case ROWS: return rows_bytes(rows_job(*a));
+        case SLIM: return tile_job_bytes(dense_job(*a, true));
+        case TILE: return tile_job_bytes(dense_job(*a, false));
+        default: return large_dense(*a, nullptr).bytes;
+    }
 }
 
 int pvae_dense(const pvae_dense_args* a, void* workspace, int64_t workspace_bytes, void* hip_stream) {
     if (int rc = check_dense(a)) return rc;
     if (a->m == 0 || a->n == 0) return 0;
     hipStream_t s = static_cast<hipStream_t>(hip_stream);
-    if (is_rows(*a)) {
+    const Kernel kind = dense_kernel(a->m, a->k, a->n, esize(a->dtype));
+    if (kind == ROWS) {
         const PvdRowsJob J = rows_job(*a);
         if (int rc = check_workspace("pvae_dense", workspace, workspace_bytes, rows_bytes(J))) return rc;
         return run_rows(*a, J, workspace, s);
     }
-    if (is_large(a->m, a->n, a->k)) {
+    if (kind == LARGE) {
         NtPlan plan = large_dense(*a, workspace);
         if (int rc = check_workspace("pvae_dense", workspace, workspace_bytes, plan.bytes)) return rc;
         return launch_large(a->dtype, plan, s);
     }
-    PvdTileJob J = dense_job(*a);
+    PvdTileJob J = dense_job(*a, kind == SLIM);
     if (int rc = check_workspace("pvae_dense", workspace, workspace_bytes, tile_job_bytes(J))) return rc;
     const int64_t blocks = (int64_t)J.mt * J.nt * J.splits;
     if (int rc = check_grid(blocks)) return rc;
     J.part = static_cast<float*>(workspace);
-    if (is_slim(a->m, a->n)) {
+    if (kind == SLIM) {
         PVD_BY_TYPE(a->dtype, hipLaunchKernelGGL(pvk_dense_slim<D_>, dim3((unsigned)blocks), dim3(512), 0, s, J));
     } else {
         PVD_BY_TYPE(a->dtype, hipLaunchKernelGGL(pvk_dense_tile<D_>, dim3((unsigned)blocks), dim3(256), 0, s, J));
     }
-    if (int rc = launched("dense_tile")) return rc;
+    if (int rc = launched("dense")) return rc;
     return J.splits > 1 ? launch_join(a->dtype, J.O, J.part, J.splits, s) : 0;
 }
 
 int64_t pvae_dense_bwd_workspace(const pvae_dense_bwd_args* a) {
     if (check_dense_bwd(a)) return 0;
-    if (bwd_is_large(*a)) return large_bwd(*a, nullptr).bytes;
-    return bwd_bytes(bwd_plan(*a));
+    return bwd_kernel(*a) == SLIM ? bwd_bytes(bwd_plan(*a)) : large_bwd(*a, nullptr).bytes;
 }
 
 int pvae_dense_bwd(const pvae_dense_bwd_args* a, void* workspace, int64_t workspace_bytes, void* hip_stream) {
     if (int rc = check_dense_bwd(a)) return rc;
     hipStream_t s = static_cast<hipStream_t>(hip_stream);
-    if (bwd_is_large(*a)) {
+    if (bwd_kernel(*a) == LARGE) {
         NtPlan plan = large_bwd(*a, workspace);
         if (int rc = check_workspace("pvae_dense_bwd", workspace, workspace_bytes, plan.bytes)) return rc;
         return launch_large(a->dtype, plan, s);
@@ -608,16 +626,11 @@ int pvae_dense_bwd(const pvae_dense_bwd_args* a, void* workspace, int64_t worksp
     BwdPlan p = bwd_plan(*a);
     if (int rc = check_workspace("pvae_dense_bwd", workspace, workspace_bytes, bwd_bytes(p))) return rc;
     const int64_t blocks = p.J.n_dx + p.J.n_dw + p.n_db;
-    if (int rc = check_grid(blocks)) return rc;
     if (blocks == 0) return 0;
     p.J.dx.part = static_cast<float*>(workspace);
     p.J.dw.part = static_cast<float*>(workspace) + (p.J.n_dx ? tile_job_bytes(p.J.dx) / 4 : 0);
-    if (p.slim) {
-        PVD_BY_TYPE(a->dtype, hipLaunchKernelGGL(pvk_dense_bwd_slim<D_>, dim3((unsigned)blocks), dim3(512), 0, s, p.J));
-    } else {
-        PVD_BY_TYPE(a->dtype, hipLaunchKernelGGL(pvk_dense_bwd_tile<D_>, dim3((unsigned)blocks), dim3(256), 0, s, p.J));
-    }
-    if (int rc = launched("dense_bwd_tile")) return rc;
+    PVD_BY_TYPE(a->dtype, hipLaunchKernelGGL(pvk_dense_bwd_slim<D_>, dim3((unsigned)blocks), dim3(512), 0, s, p.J));
+    if (int rc = launched("dense_bwd")) return rc;
     if (p.J.n_dx && p.J.dx.splits > 1)
         if (int rc = launch_join(a->dtype, p.J.dx.O, p.J.dx.part, p.J.dx.splits, s)) return rc;
     if (p.J.n_dw && p.J.dw.splits > 1)

@@ -111,6 +111,25 @@ def test_dense_and_gradients(m, k, n, dtype):
             assert all(torch.equal(p, q) for p, q in zip(got, again))  # no order of sums that changes from run to run
 
 
+# the large product kernel's forms: whole and ragged tiles, few and many of them, contractions in pieces, operands as they lie
+# (aligned) and laid out (not), either orientation
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("m,k,n", [(2048, 1344, 2048), (2100, 1408, 2208), (192, 8192, 256), (640, 1024, 1152), (1543, 1021, 2027),
+                                   (130, 70_001, 129), (5, 2048, 4099), (1024, 64, 3000), (4000, 64, 64), (600, 2500, 17), (4001, 30, 100)])
+def test_large_products(m, k, n, dtype):
+    act = ACTS[(m + n) % 7]
+    for w_t in (False, True):
+        x, r, dy = rnd(m, k, dtype=dtype, seed=1), rnd(m, n, dtype=dtype, seed=2), rnd(m, n, dtype=dtype, seed=3)
+        w = rnd(n, k, dtype=dtype, seed=4, scale=k ** -0.5).t() if w_t else rnd(k, n, dtype=dtype, seed=4, scale=k ** -0.5)
+        b, z = rnd(n, dtype=dtype, seed=5), torch.empty(m, n, device="cuda")
+        check_forward(x, w, b, act, r, ops.dense(x, w, b, act, residual=r, pre=z), z)
+        add = rnd(m, k, dtype=dtype, seed=6)
+        check_backward(dy, x, w, z, act, add, *ops.dense_backward(dy, x, w, z, act, dx_add=add))
+        dx, dw, db = ops.dense_backward(dy, x, w, z, act, need_dx=False, need_dw=False)
+        assert dx is None and dw is None
+        check_backward(dy, x, w, z, act, None, None, None, db)
+
+
 @pytest.mark.parametrize("m,k,n", [(0, 5, 7), (5, 0, 7), (5, 7, 0), (0, 0, 0)])
 def test_empty_sizes(m, k, n):
     x, w, b, r, dy = rnd(m, k), rnd(k, n, seed=1), rnd(n, seed=2), rnd(m, n, seed=3), rnd(m, n, seed=4)
