@@ -616,7 +616,7 @@ template <int DT> __global__ __launch_bounds__(256) void pvk_dense_pack(const Pv
     float sum[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) sum[e] = 0.f;
-#pragma unroll 2
+#pragma unroll
     for (int rr = row; rr < 64; rr += 256 / PER) {
         const int64_t r = r0 + rr, c = c0 + run * VEC;
         alignas(16) T v[VEC];
@@ -892,10 +892,20 @@ template <int DT, int TM, int TN, int WM, int WN, int ST> struct PvdNt {
         };
         auto multiply = [&](int g, int from, int to) {
             const int h = g / (FM / GB), k0 = g % (FM / GB) * GB;
+            if constexpr (DT == PVD_F32) {  // the four products of a fragment apart from each other: each adds to what the last one left
 #pragma unroll
-            for (int u = from; u < to; ++u) {
-                const int k = u / FN, i = u % FN;
-                acc[i][k0 + k] = pvd_mfma16<DT>(a[h][i], b[g & 1][k], acc[i][k0 + k]);
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int u = from; u < to; ++u) {
+                        const int k = u / FN, i = u % FN;
+                        acc[i][k0 + k] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[h][i][e]), __uint_as_float(b[g & 1][k][e]), acc[i][k0 + k], 0, 0, 0);
+                    }
+            } else {
+#pragma unroll
+                for (int u = from; u < to; ++u) {
+                    const int k = u / FN, i = u % FN;
+                    acc[i][k0 + k] = pvd_mfma16<DT>(a[h][i], b[g & 1][k], acc[i][k0 + k]);
+                }
             }
             __builtin_amdgcn_sched_barrier(0);
         };
