@@ -45,14 +45,15 @@ def build_engine(force=False, extra=()):
     srcs += [os.path.join(INC, "pvae.h"), os.path.join(INC, "pvae_ops.h")]
     if force or _newer(out, srcs):
         hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
-        flags = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function", "-Wno-unused-value", *extra]
+        # no packed float32 instructions: some of their forms have given wrong results on this part (the host pass of hipcc does
+        # not know the feature and says so)
+        flags = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function", "-Wno-unused-value",
+                 "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", *extra]
         with tempfile.TemporaryDirectory() as tmp:
             objs, running = [], []
-            # no packed float32 instructions: some of their forms have given wrong results on this part (the host pass of hipcc
-            # does not know the feature and says so)
-            for name, more in (("pvae_engine", []), ("pvae_ops", ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"])):
+            for name in ("pvae_engine", "pvae_ops"):
                 objs.append(os.path.join(tmp, name + ".o"))
-                cmd = [hipcc, *flags, *more, "-c", "-o", objs[-1], os.path.join(CSRC, name + ".hip")]
+                cmd = [hipcc, *flags, "-c", "-o", objs[-1], os.path.join(CSRC, name + ".hip")]
                 print("+", " ".join(cmd), flush=True)
                 running.append((cmd, subprocess.Popen(cmd)))
             for cmd, p in running:
