@@ -2138,7 +2138,7 @@ int pvae_train_epoch(pvae_engine* e, const int32_t* perm, int32_t n_train, const
         HIPCHK(hipMemcpyAsync(e->d_ntotal, &nt, sizeof(int), hipMemcpyHostToDevice, e->stream));
         HIPCHK(hipStreamSynchronize(e->stream));  // nt is a stack variable
         const int base = phase == 0 ? 0 : n_train;
-        SplitScope split(e, phase == 0 && e->split_dec);
+        SplitScope split(e, phase == 0 && e->split_dec && e->fused_narrow);
         GatherScope gscope(e);
         for (int s = 0; s < steps; ++s) {
             if ((rc = join_side(e))) return rc;

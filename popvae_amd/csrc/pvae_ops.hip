@@ -54,7 +54,7 @@ int check_sizes(int32_t dtype, int32_t act, int64_t m, int64_t k, int64_t n) {
 }
 int check_weights(const void* w, int64_t k, int64_t n, int64_t sk, int64_t sn, int size) {
     if (k == 0 || n == 0) return 0;
-    if (sn == 1 || n == 1) return check_matrix("w", w, k, n, std::max(sk, n == 1 ? int64_t(1) : sk), size);
+    if (sn == 1 || n == 1) return check_matrix("w", w, k, n, sk, size);
     if (sk == 1 || k == 1) return check_matrix("w^T", w, n, k, sn, size);
     return refuse(-2, "w: neither rows nor columns are contiguous (strides %lld, %lld)", (long long)sk, (long long)sn);
 }
@@ -329,7 +329,7 @@ template <int DT, int TM, int WM, int WN, int ST> int launch_nt(const PvdNtJobs&
     return launched("dense_nt");
 }
 int launch_large(int dt, NtPlan& plan, hipStream_t s) {
-    if (plan.packs.n) {
+    if (plan.packs.n && plan.packs.first[plan.packs.n]) {
         PVD_BY_TYPE(dt, hipLaunchKernelGGL(pvk_dense_pack<D_>, dim3(plan.packs.first[plan.packs.n]), dim3(256), 0, s, plan.packs));
         if (int rc = launched("dense_pack")) return rc;
     }
@@ -692,8 +692,8 @@ int pvae_adam_step(const pvae_tensor* p, const pvae_tensor* g, const pvae_tensor
         if (int rc = check_tensors("g", g, count, false)) return rc;
         if (int rc = check_tensors("m", m, count, true)) return rc;
         if (int rc = check_tensors("v", v, count, true)) return rc;
-        if (!std::isfinite(lr) || !(beta1 >= 0 && beta1 < 1) || !(beta2 >= 0 && beta2 < 1) || !(eps > 0) || !std::isfinite(eps))
-            return refuse(-2, "lr %g, beta1 %g, beta2 %g, eps %g: finite, 0 <= beta < 1, eps > 0", lr, beta1, beta2, eps);
+        if (!std::isfinite(lr) || !(beta1 >= 0 && beta1 < 1) || !(beta2 >= 0 && beta2 < 1) || !((float)eps > 0) || !std::isfinite((float)eps))
+            return refuse(-2, "lr %g, beta1 %g, beta2 %g, eps %g: finite, 0 <= beta < 1, eps > 0 in float32", lr, beta1, beta2, eps);
         if (!step_dev && step < 1) return refuse(-2, "step %lld: counted from 1", (long long)step);
         if (!(clip_norm >= 0)) return refuse(-2, "clip_norm %g: a positive number, or 0 for none", clip_norm);
         std::vector<Span> spans;

@@ -4,7 +4,8 @@ residual in one pass, its gradients, the global gradient norm, clipping by it, a
 They are what the engine's layers and optimizer do, for tensors that do not live in an ``Engine``: any size, float32, bfloat16
 or float16, other activations.  Everything runs on torch's current stream of the tensors' device, allocates through torch's
 allocator (outputs and scratch memory), never waits for the GPU and may be captured into a graph.  A call that cannot be
-computed raises ValueError before anything is launched.  There is no CPU path.
+computed raises ValueError before anything is launched.  There is no CPU path, and autograd records nothing here:
+gradients are calls of their own.
 
     y = ops.dense(x, w, b, "elu", residual=x, pre=z)               # z: float32, kept for the backward
     dx, dw, db = ops.dense_backward(dy, x, w, z, "elu", dx_add=dy)  # dx_add: the layer's residual was its own input

@@ -174,6 +174,23 @@ def test_a_bound_never_reached_leaves_the_trajectory():
     a.close(), b.close()
 
 
+def test_residual_layers_in_the_staged_step():
+    """The calls that sharding cuts a step into, on one rank: the same gradients as the whole step."""
+    new, dc, w = make(900, 128, 4, 2, 32)
+    e = new()
+    e.set_residual()
+    rows, eps = np.arange(20, dtype=np.int32), np.random.default_rng(2).normal(size=(20, 2)).astype(np.float32)
+    loss = e.grad_step(rows, eps)
+    grads = e.get_grads()
+    e.stage_a(rows, eps, engine.MODE_GRAD)
+    e.stage_b(engine.MODE_GRAD)
+    assert e.stage_c(engine.MODE_GRAD) == loss
+    assert all(np.array_equal(a, b) for a, b in zip(e.get_grads(), grads))
+    e.stage_a(rows, eps, engine.MODE_ENCODE)
+    assert all(np.array_equal(a, b) for a, b in zip(e.stage_encode(20), e.encode(rows, eps)))
+    e.close()
+
+
 def test_refusals():
     new, _, _ = make(300, 32, 2, 2, 32)
     e = new()

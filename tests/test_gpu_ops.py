@@ -130,7 +130,7 @@ def test_large_products(m, k, n, dtype):
         check_backward(dy, x, w, z, act, None, None, None, db)
 
 
-@pytest.mark.parametrize("m,k,n", [(0, 5, 7), (5, 0, 7), (5, 7, 0), (0, 0, 0)])
+@pytest.mark.parametrize("m,k,n", [(0, 5, 7), (5, 0, 7), (5, 7, 0), (0, 0, 0), (3, 0, 9), (600, 5, 0), (600, 0, 5), (0, 300, 400)])
 def test_empty_sizes(m, k, n):
     x, w, b, r, dy = rnd(m, k), rnd(k, n, seed=1), rnd(n, seed=2), rnd(m, n, seed=3), rnd(m, n, seed=4)
     z = torch.full((m, n), 7.0, device="cuda")
@@ -253,7 +253,8 @@ def on_stream(f):
     return r
 
 
-@pytest.mark.parametrize("m,k,n,dtype", [(4, 300, 200, F32), (32, 128, 128, F32), (300, 256, 300, F32), (300, 256, 300, BF16)])
+@pytest.mark.parametrize("m,k,n,dtype", [(4, 300, 200, F32), (32, 128, 128, F32), (300, 256, 300, F32), (300, 256, 300, BF16),
+                                         (700, 520, 900, F32), (700, 512, 901, F16)])
 def test_streams_and_graphs(m, k, n, dtype):
     x, w, b, dy = (rnd(*s, dtype=dtype, seed=i) for i, s in enumerate([(m, k), (k, n), (n,), (m, n)]))
     z, z2 = torch.empty(m, n, device="cuda"), torch.empty(m, n, device="cuda")
@@ -522,3 +523,48 @@ def test_a_training_step_of_residual_layers():
             assert float((b.double() - c).norm()) <= 1e-5 * float(c.norm())
             assert float((a.double() - w).norm()) <= 1e-3 * lr * t * a.numel() ** 0.5 + 1e-6 * float(w.norm())
         ref, rm, rv = [w for w, _, _ in new], [c for _, c, _ in new], [d for _, _, d in new]
+
+
+@pytest.mark.parametrize("m,k,n", [(4, 128, 200), (40, 128, 200), (600, 100, 600), (600, 1024, 1200)])
+def test_subnormal_halves_are_kept(m, k, n):
+    """float16 values below 2^-14 enter the products as they are (rows, slim, tile and large kernels)."""
+    x, w = rnd(m, k, dtype=F16, seed=1, scale=2.0 ** -18), rnd(k, n, dtype=F16, seed=2)
+    check_forward(x, w, None, "linear", None, ops.dense(x, w))
+    dy = rnd(m, n, dtype=F16, seed=3, scale=2.0 ** -18)
+    check_backward(dy, x, w, None, "linear", None, *ops.dense_backward(dy, x, w))
+
+
+def test_products_of_one_hot_rows_are_exact():
+    """A row of zeros and a one picks a row of w, to the bit, whatever the kernel."""
+    for m, k, n, dtype in ((3, 50, 70, F32), (60, 50, 70, F32), (500, 40, 900, F32), (500, 512, 900, F32), (500, 1024, 900, BF16)):
+        w = rnd(k, n, dtype=dtype, seed=1)
+        pick = torch.arange(m, device="cuda") % k
+        x = torch.zeros(m, k, dtype=dtype, device="cuda")
+        x[torch.arange(m, device="cuda"), pick] = 1
+        assert torch.equal(ops.dense(x, w), w[pick])
+        assert torch.equal(ops.dense(x, w.t().contiguous().t()), w[pick])
+
+
+def test_two_streams_at_once():
+    """Calls on two streams that overlap in time share nothing."""
+    m, k, n = 900, 700, 800
+    ins = [[rnd(*s, seed=10 * i + j) for j, s in enumerate([(m, k), (k, n), (n,), (m, n)])] for i in range(2)]
+    z = [torch.empty(m, n, device="cuda") for _ in range(2)]
+
+    def work(i):
+        x, w, b, dy = ins[i]
+        y = ops.dense(x, w, b, "tanh", pre=z[i])
+        out = [torch.empty_like(x), torch.empty_like(w)]
+        norm = ops.clip_by_global_norm([x, w], 1.0 + i, out=out)
+        return [y, *ops.dense_backward(dy, x, w, z[i], "tanh"), norm, *out]
+
+    want = [[t.clone() for t in work(i)] for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [None, None]
+    for _ in range(3):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i] = work(i)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))

@@ -48,7 +48,7 @@ def dense_args(**kw):
 @pytest.mark.parametrize("kw,text", [
     (dict(dtype=3), "type"), (dict(act=7), "activation"), (dict(m=-1), "sizes"), (dict(n=1 << 31), "sizes"), (dict(x=None), "x is NULL"),
     (dict(x=4097), "aligned"), (dict(ldx=3), "x: row stride"), (dict(ldx=1 << 60), "too large"), (dict(w_sk=7), "w: row stride"),
-    (dict(w_sk=16, w_sn=2), "neither"), (dict(w_sk=1, w_sn=3), "w\\^T"), (dict(y=None), "y is NULL"), (dict(ldy=7), "y: row stride"),
+    (dict(w_sk=16, w_sn=2), "neither"), (dict(n=1, ldy=1, w_sk=0), "w: row stride"), (dict(n=1, ldy=1, w_sk=-4), "w: row stride"), (dict(w_sk=1, w_sn=3), "w\\^T"), (dict(y=None), "y is NULL"), (dict(ldy=7), "y: row stride"),
     (dict(residual=4096, ldr=5), "residual"), (dict(pre=4098, ldp=8), "pre is not aligned"), (dict(pre=65536, ldp=4), "pre: row"), (dict(y=4096), "y overlaps x"), (dict(y=8192 + 60), "y overlaps w"),
     (dict(pre=16384 + 32, ldp=8), "y overlaps pre"), (dict(residual=16384 + 4, ldr=8), "y overlaps residual"),
     (dict(residual=16384, ldr=12), "y overlaps residual"), (dict(pre=4096, ldp=8, residual=16384, ldr=8), "pre overlaps x"),
@@ -124,7 +124,7 @@ def test_many_tensor_refusals():
         a = dict(zip(("lr", "b1", "b2", "eps", "step", "step_dev", "clip"), good), **kw)
         return L.pvae_adam_step(p, g, m, v, 1, a["lr"], a["b1"], a["b2"], a["eps"], a["step"], a["step_dev"], a["clip"], None, None, 0, None)
 
-    for kw in (dict(lr=float("inf")), dict(b1=1.0), dict(b2=-0.1), dict(eps=0.0), dict(step=0), dict(clip=-1.0), dict(clip=1.0),
+    for kw in (dict(lr=float("inf")), dict(b1=1.0), dict(b2=-0.1), dict(eps=0.0), dict(eps=1e-60), dict(eps=1e60), dict(step=0), dict(clip=-1.0), dict(clip=1.0),
                dict(p=g), dict(m=v), dict(p=table((4096, 8, 1, 0))), dict(g=table((8192, 9, 0, 0))), dict(p=table((4096, 8, 0, 4))),
                dict(p=table((4096, 8, 0, 4)), m=table((4096 + 16, 8, 0, 4)), v=table((4096 + 16, 8, 0, 4)))):
         assert adam(**kw) < 0, kw
