@@ -56,7 +56,7 @@ int pvae_dense(const pvae_dense_args* a, void* workspace, int64_t workspace_byte
  * dy [m][n]; pre [m][n] float32 (NULL with PVAE_LINEAR); dx [m][k], dw [k][n] contiguous, dbias [n]: each may be NULL.
  * dx_add [m][k] with row stride ldadd, or NULL: added to dx before its one rounding (a layer whose residual is its own
  * input passes dy; dx may be dx_add itself).  dpre [m][n] float32 contiguous, or NULL: receives g.
- * g enters the products in the tensors' type (16-bit types: one rounding of g); dbias sums the unrounded g. */
+ * g enters the products in the tensors' type (16-bit types: rounded once at most); dbias sums the unrounded g. */
 typedef struct pvae_dense_bwd_args {
     int32_t dtype, act;
     int64_t m, k, n;

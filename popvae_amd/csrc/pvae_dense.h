@@ -281,11 +281,13 @@ template <int DT> __global__ __launch_bounds__(256) void pvk_dense_tile(const Pv
 // ---------------------------------------------------------------------------------------------
 enum { PVD_SM = 32, PVD_SN = 16, PVD_SW = 8 };
 
-// VEC elements of row `row` from k on, as a lane of the matrix instruction holds them; zeros outside
-template <int DT, bool GRAD> __device__ __forceinline__ pvd_u32x4 pvd_slim_load(const PvdOperand& P, int64_t row, int64_t k, int64_t k1) {
+// VEC elements of row `row` from k on, as a lane of the matrix instruction holds them; zeros outside.  g of a 16-bit type comes in
+// two terms, the second into `lo`: here, where few values of g may make a whole gradient, one rounding of each would show,
+// and a second matrix instruction costs nothing.
+template <int DT, bool GRAD> __device__ __forceinline__ pvd_u32x4 pvd_slim_load(const PvdOperand& P, int64_t row, int64_t k, int64_t k1, pvd_u32x4& lo) {
     typedef typename PvdType<DT>::T T;
     enum { VEC = PvdType<DT>::VEC };
-    alignas(16) T v[VEC];
+    alignas(16) T v[VEC], l[VEC] = {};
     const T* p = static_cast<const T*>(P.p) + row * P.sr + k * P.sk;
     const bool grad = GRAD && P.act != PVD_LINEAR;
     const float* z = grad ? P.pre + row * P.pr + k * P.pk : nullptr;
@@ -304,9 +306,17 @@ template <int DT, bool GRAD> __device__ __forceinline__ pvd_u32x4 pvd_slim_load(
         for (int e = 0; e < VEC; e += 4) {
             const pvd_f32x4 d = pvd_act_grad4(*reinterpret_cast<const pvd_f32x4*>(zz + e), P.act);
 #pragma unroll
-            for (int f = 0; f < 4; ++f) v[e + f] = pvd_from_f32<DT>(pvd_to_f32<DT>(v[e + f]) * d[f]);
+            for (int f = 0; f < 4; ++f) {
+                const float g = pvd_to_f32<DT>(v[e + f]) * d[f];
+                v[e + f] = pvd_from_f32<DT>(g);
+                if constexpr (DT != PVD_F32) {
+                    const float rest = g - pvd_to_f32<DT>(v[e + f]);  // not finite where g is not, or rounds to infinity
+                    l[e + f] = pvd_from_f32<DT>(fabsf(rest) < __builtin_inff() ? rest : 0.f);
+                }
+            }
         }
     }
+    lo = *reinterpret_cast<const pvd_u32x4*>(l);
     return *reinterpret_cast<const pvd_u32x4*>(v);
 }
 
@@ -319,18 +329,22 @@ template <int DT, bool GX, bool GW> __device__ __forceinline__ void pvd_slim_job
     const int64_t k0 = piece * J.kper, k1 = min(J.K, k0 + J.kper);
     pvd_f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
     for (int64_t k = k0 + wave * (RUN * KS); k < k1; k += PVD_SW * RUN * KS) {
-        pvd_u32x4 a[RUN], b[RUN][2];
+        pvd_u32x4 a[RUN], b[RUN][2], al[RUN], bl[RUN][2];
 #pragma unroll
         for (int u = 0; u < RUN; ++u) {
             const int64_t kk = k + u * KS + q * PvdType<DT>::VEC;
-            a[u] = pvd_slim_load<DT, GW>(J.W, n0 + r, kk, k1);
-            b[u][0] = pvd_slim_load<DT, GX>(J.X, m0 + r, kk, k1);
-            b[u][1] = pvd_slim_load<DT, GX>(J.X, m0 + 16 + r, kk, k1);
+            a[u] = pvd_slim_load<DT, GW>(J.W, n0 + r, kk, k1, al[u]);
+            b[u][0] = pvd_slim_load<DT, GX>(J.X, m0 + r, kk, k1, bl[u][0]);
+            b[u][1] = pvd_slim_load<DT, GX>(J.X, m0 + 16 + r, kk, k1, bl[u][1]);
         }
 #pragma unroll
         for (int u = 0; u < RUN; ++u)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) acc[j] = pvd_mfma16<DT>(a[u], b[u][j], acc[j]);
+            for (int j = 0; j < 2; ++j) {
+                acc[j] = pvd_mfma16<DT>(a[u], b[u][j], acc[j]);
+                if constexpr (DT != PVD_F32 && GW) acc[j] = pvd_mfma16<DT>(al[u], b[u][j], acc[j]);
+                if constexpr (DT != PVD_F32 && GX) acc[j] = pvd_mfma16<DT>(a[u], bl[u][j], acc[j]);
+            }
     }
     // red[wave][row][16 columns]
 #pragma unroll
