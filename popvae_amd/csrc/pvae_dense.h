@@ -155,7 +155,9 @@ template <int DT> struct PvdStage {
             return;
         }
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) o[e] = e < left ? p[e] : T(0);
+        for (int e = 0; e < VEC; ++e) o[e] = p[min((int64_t)e, left - 1)];  // the last element again: no load waits for a branch
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) o[e] = e < left ? o[e] : T(0);
     }
     __device__ __forceinline__ void load(const PvdOperand& P, int64_t row0, int64_t k0, int64_t k1, int tid) {
         if (P.sk == 1) {
@@ -281,30 +283,53 @@ template <int DT> __global__ __launch_bounds__(256) void pvk_dense_tile(const Pv
 // ---------------------------------------------------------------------------------------------
 enum { PVD_SM = 32, PVD_SN = 16, PVD_SW = 8 };
 
-// VEC elements of row `row` from k on, as a lane of the matrix instruction holds them; zeros outside.  g of a 16-bit type comes in
-// two terms, the second into `lo`: here, where few values of g may make a whole gradient, one rounding of each would show,
-// and a second matrix instruction costs nothing.
-template <int DT, bool GRAD> __device__ __forceinline__ pvd_u32x4 pvd_slim_load(const PvdOperand& P, int64_t row, int64_t k, int64_t k1, pvd_u32x4& lo) {
+// VEC elements of row `row` from k on, as a lane of the matrix instruction holds them, zeros outside; and z there, if g is asked for
+template <int DT, bool GRAD> struct PvdSlim {
     typedef typename PvdType<DT>::T T;
     enum { VEC = PvdType<DT>::VEC };
-    alignas(16) T v[VEC], l[VEC] = {};
-    const T* p = static_cast<const T*>(P.p) + row * P.sr + k * P.sk;
-    const bool grad = GRAD && P.act != PVD_LINEAR;
-    const float* z = grad ? P.pre + row * P.pr + k * P.pk : nullptr;
-    const bool in = row < P.rows;
-    if (P.sk == 1 && in && k + VEC <= k1) {
-        *reinterpret_cast<pvd_u32x4*>(v) = *reinterpret_cast<const pvd_u32x4_any*>(p);
-    } else {
+    alignas(16) T v[VEC];
+    alignas(16) float z[VEC];
+
+    __device__ __forceinline__ void load(const PvdOperand& P, int64_t row, int64_t k, int64_t k1) {
+        const bool grad = GRAD && P.act != PVD_LINEAR, in = row < P.rows, whole = P.sk == 1 && k + VEC <= k1;
+        const int64_t rr = min(row, P.rows - 1);
+        const T* p = static_cast<const T*>(P.p) + rr * P.sr;
+        const float* pz = grad ? P.pre + rr * P.pr : nullptr;
+        T t[VEC];
+        float f[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) v[e] = in && k + e < k1 ? p[e * P.sk] : T(0);
+        for (int e = 0; e < VEC; ++e) f[e] = 0.f;
+        if (whole) {
+            const pvd_u32x4 d = *reinterpret_cast<const pvd_u32x4_any*>(p + k);
+            __builtin_memcpy(t, &d, 16);
+            if (grad)
+#pragma unroll
+                for (int e = 0; e < VEC; e += 4) {
+                    const pvd_f32x4 d4 = pvm_load4(pz, 0, k + e);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) f[e + i] = d4[i];
+                }
+        } else {  // what lies outside reads the last element inside instead: no load waits for a branch
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) t[e] = p[min(k + e, k1 - 1) * P.sk];
+            if (grad)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) f[e] = pz[min(k + e, k1 - 1) * P.pk];
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const bool there = in && (whole || k + e < k1);
+            v[e] = there ? t[e] : T(0);
+            z[e] = there ? f[e] : 0.f;
+        }
     }
-    if (grad) {
-        alignas(16) float zz[VEC];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) zz[e] = in && k + e < k1 ? z[e * P.pk] : 0.f;
+    // v becomes g; g of a 16-bit type has two terms, the second goes into `lo`: here, where few values of g may make a whole
+    // gradient, one rounding of each would show, and a second matrix instruction costs nothing
+    __device__ __forceinline__ void grad(int act, pvd_u32x4& lo) {
+        alignas(16) T l[VEC];
 #pragma unroll
         for (int e = 0; e < VEC; e += 4) {
-            const pvd_f32x4 d = pvd_act_grad4(*reinterpret_cast<const pvd_f32x4*>(zz + e), P.act);
+            const pvd_f32x4 d = pvd_act_grad4(*reinterpret_cast<const pvd_f32x4*>(z + e), act);
 #pragma unroll
             for (int f = 0; f < 4; ++f) {
                 const float g = pvd_to_f32<DT>(v[e + f]) * d[f];
@@ -315,10 +340,10 @@ template <int DT, bool GRAD> __device__ __forceinline__ pvd_u32x4 pvd_slim_load(
                 }
             }
         }
+        if constexpr (DT != PVD_F32) lo = *reinterpret_cast<const pvd_u32x4*>(l);
     }
-    lo = *reinterpret_cast<const pvd_u32x4*>(l);
-    return *reinterpret_cast<const pvd_u32x4*>(v);
-}
+    __device__ __forceinline__ pvd_u32x4 bits() const { return *reinterpret_cast<const pvd_u32x4*>(v); }
+};
 
 template <int DT, bool GX, bool GW> __device__ __forceinline__ void pvd_slim_job(const PvdTileJob& J, int64_t block, float* red) {
     enum { KS = 4 * PvdType<DT>::VEC, RUN = 2 };  // contraction of one matrix instruction group; groups under way per wave
@@ -327,24 +352,34 @@ template <int DT, bool GX, bool GW> __device__ __forceinline__ void pvd_slim_job
     const int piece = (int)(block / tiles);
     const int64_t t = block % tiles, m0 = t / J.nt * PVD_SM, n0 = t % J.nt * PVD_SN;
     const int64_t k0 = piece * J.kper, k1 = min(J.K, k0 + J.kper);
+    const bool gx = GX && J.X.act != PVD_LINEAR, gw = GW && J.W.act != PVD_LINEAR;
+    const int halves = m0 + 16 < J.X.rows ? 2 : 1;
     pvd_f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
     for (int64_t k = k0 + wave * (RUN * KS); k < k1; k += PVD_SW * RUN * KS) {
-        pvd_u32x4 a[RUN], b[RUN][2], al[RUN], bl[RUN][2];
+        PvdSlim<DT, GW> a[RUN];
+        PvdSlim<DT, GX> b[RUN][2];
 #pragma unroll
         for (int u = 0; u < RUN; ++u) {
             const int64_t kk = k + u * KS + q * PvdType<DT>::VEC;
-            a[u] = pvd_slim_load<DT, GW>(J.W, n0 + r, kk, k1, al[u]);
-            b[u][0] = pvd_slim_load<DT, GX>(J.X, m0 + r, kk, k1, bl[u][0]);
-            b[u][1] = pvd_slim_load<DT, GX>(J.X, m0 + 16 + r, kk, k1, bl[u][1]);
+            a[u].load(J.W, n0 + r, kk, k1);
+            b[u][0].load(J.X, m0 + r, kk, k1);
+            b[u][1].load(J.X, m0 + 16 + r, kk, k1);
         }
 #pragma unroll
-        for (int u = 0; u < RUN; ++u)
+        for (int u = 0; u < RUN; ++u) {
+            if (k + u * KS < k1) {  // the same for the whole wave, as is the number of halves
+                pvd_u32x4 al, bl;
+                if (gw) a[u].grad(J.W.act, al);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                acc[j] = pvd_mfma16<DT>(a[u], b[u][j], acc[j]);
-                if constexpr (DT != PVD_F32 && GW) acc[j] = pvd_mfma16<DT>(al[u], b[u][j], acc[j]);
-                if constexpr (DT != PVD_F32 && GX) acc[j] = pvd_mfma16<DT>(a[u], bl[u][j], acc[j]);
+                for (int j = 0; j < 2; ++j)
+                    if (j < halves) {
+                        if (gx) b[u][j].grad(J.X.act, bl);
+                        acc[j] = pvd_mfma16<DT>(a[u].bits(), b[u][j].bits(), acc[j]);
+                        if (DT != PVD_F32 && gw) acc[j] = pvd_mfma16<DT>(al, b[u][j].bits(), acc[j]);
+                        if (DT != PVD_F32 && gx) acc[j] = pvd_mfma16<DT>(a[u].bits(), bl, acc[j]);
+                    }
             }
+        }
     }
     // red[wave][row][16 columns]
 #pragma unroll
@@ -360,7 +395,7 @@ template <int DT, bool GX, bool GW> __device__ __forceinline__ void pvd_slim_job
     else if (m < J.O.rows) pvd_store_some(J.part, 0, (piece * J.O.rows + m) * J.O.cols + n, z, pvd_left(n, J.O.cols));
 }
 
-template <int DT> __global__ __launch_bounds__(512) void pvk_dense_slim(const PvdTileJob J) {
+template <int DT> __global__ __launch_bounds__(512, 4) void pvk_dense_slim(const PvdTileJob J) {
     __shared__ __attribute__((aligned(16))) float red[PVD_SW * PVD_SM * PVD_SN];
     pvd_slim_job<DT, false, false>(J, blockIdx.x, red);
 }
@@ -434,13 +469,17 @@ template <int DT, int R> __global__ __launch_bounds__(512) void pvk_dense_rows(c
             }
             add(v, k);
         }
-    } else if (left > 0) {  // the lane with the last columns
+    } else if (left > 0) {  // the lane with the last columns; behind them the last one again, which is not stored
         for (int k = 4 * wave; k < K; k += 4 * PVD_RW) {
             T v[4][VEC];
 #pragma unroll
             for (int j = 0; j < 4; ++j)
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) v[j][e] = k + j < K && e < left ? w[(int64_t)(k + j) * J.ldw + lane * VEC + e] : T(0);
+                for (int e = 0; e < VEC; ++e) v[j][e] = w[(int64_t)min(k + j, K - 1) * J.ldw + lane * VEC + min(e, left - 1)];
+#pragma unroll
+            for (int j = 1; j < 4; ++j)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) v[j][e] = k + j < K ? v[j][e] : T(0);
             add(v, k);
         }
     }
@@ -485,12 +524,16 @@ template <int DT, int R> __global__ __launch_bounds__(512) void pvk_dense_rows_t
         alignas(16) T v[4][VEC];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            const int64_t n = n0 + group + 32 * c;
-            const T* p = static_cast<const T*>(J.w) + n * J.ldw + k0 + k;
-            if (n < J.O.cols && k + VEC <= K) *reinterpret_cast<pvd_u32x4*>(v[c]) = *reinterpret_cast<const pvd_u32x4_any*>(p);
-            else
+            // a column behind the last is the last again, and is not stored
+            const T* p = static_cast<const T*>(J.w) + min(n0 + group + 32 * c, J.O.cols - 1) * J.ldw + k0;
+            if (k + VEC <= K) {
+                *reinterpret_cast<pvd_u32x4*>(v[c]) = *reinterpret_cast<const pvd_u32x4_any*>(p + k);
+            } else {
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) v[c][e] = n < J.O.cols && k + e < K ? p[e] : T(0);
+                for (int e = 0; e < VEC; ++e) v[c][e] = p[min(k + e, K - 1)];
+#pragma unroll
+                for (int e = 1; e < VEC; ++e) v[c][e] = k + e < K ? v[c][e] : T(0);
+            }
         }
 #pragma unroll
         for (int r = 0; r < R; ++r)
