@@ -115,30 +115,43 @@ PvdOut output(int64_t rows, int64_t cols, void* y, int64_t ldy, const void* bias
 
 // Which kernel makes y (microseconds, float32 / bf16, w as Keras keeps it):
 //                        rows         slim         tile         large
-//      1 x 4096 x 4096   21.1 / 11.0  36.9 / 31.7  37.9 / 19.1  29.3 / 14.2
-//     32 x 1024 x 1024                 9.0 /  7.1  13.3 / 10.9  13.0 / 16.6
-//    256 x  512 x  512                 7.0 /  6.0  13.0 / 11.4  16.4 / 12.8
-//     64 x 4096 x 4096                55.0 / 48.5  41.3 / 24.2  34.3 / 16.7
-//   1000 x   16 x 4000                47.8 / 98.9  13.1 / 10.6  15.5 / 14.3
-//   1000 x  128 x 1000                16.6 / 21.9  11.7 /  8.9   9.5 / 11.1
+//      1 x  512 x  512    7.7 /  8.1   5.9 /  5.5  11.1 /  9.4  15.0 /  9.0
+//      1 x   16 x 20000   4.1 /  4.3   6.5 / 11.7   6.8 /  6.4   9.9 /  9.8
+//      1 x 2000 x  128    7.5 /  8.3   9.1 / 10.8  13.9 / 11.2  15.6 / 13.8
+//      1 x 4096 x 4096   21.2 / 10.9  27.8 / 27.1  37.4 / 18.0  29.4 / 14.4
+//      2 x 100000 x 3    17.0 / 23.8  11.2 / 12.2  25.0 / 17.1  26.2 / 20.1
+//      4 x 8192 x 4096   32.8 / 22.1  49.9 / 48.2  64.7 / 26.6  48.8 / 18.9
+//     32 x 1024 x 1024                 9.4 /  8.1  13.4 / 10.9  12.8 / 16.5
+//    256 x  512 x  512                 7.4 /  6.4  13.0 / 10.6  16.4 / 12.7
+//     64 x 4096 x 4096                55.7 / 45.2  39.9 / 19.6  34.6 / 17.0
+//   1000 x   16 x 4000                34.1 / 75.2  13.2 / 14.5  15.1 / 14.2
+//   1000 x  128 x 1000                14.9 / 18.1  11.8 /  9.0   9.5 / 11.1
 enum Kernel { ROWS, SLIM, TILE, LARGE };
 Kernel dense_kernel(int64_t m, int64_t k, int64_t n, int size) {
-    // a few rows: the weights pass once
-    if (m <= 4 && k > 0) return ROWS;
-    // a small result: its workgroups all find room, and what they read over and over (48 rows of contraction each) stays small
-    const int64_t slim = ceil_div(m, PVD_SM) * ceil_div(n, PVD_SN);
-    if (slim <= (size == 4 ? 1024 : 512) && slim * 48 * k <= int64_t(16) << 20) return SLIM;
+    // small results: the slim kernel's workgroups all find room, and what they read over and over (48 rows of contraction each)
+    // stays small
+    const int64_t slim = ceil_div(m, PVD_SM) * ceil_div(n, PVD_SN), reads = slim <= (size == 4 ? 1024 : 512) ? slim * 48 * k : INT64_MAX;
+    // a few rows: the weights pass once, and the contraction is split over the chip and joined in a second launch.  The slim
+    // kernel makes a small result in one (less than 4096 bytes of contraction), and needs far fewer pieces of a very long
+    // contraction; below 128 the rows kernel does not split either.  16-bit products of more than two rows over long
+    // contractions cost the rows kernel more arithmetic than reading.
+    if (m <= 4 && k > 0) {
+        if ((k * size < 4096 || k >= 16384) && (m > 2 || k >= 128) && reads <= int64_t(8) << 20) return SLIM;
+        if (size == 4 || m <= 2 || k < 4096) return ROWS;
+    }
+    if (reads <= int64_t(16) << 20) return SLIM;
     // a short contraction never fills the large kernel's pipeline; 16-bit products are over sooner
     if (size == 4 ? k >= 64 : k >= 1024 || (double)m * n * k >= 2147483648.0) return LARGE;
     return TILE;
 }
 // The gradients: slim while what its workgroups read stays small (every value of g is formed anew for each), else large, which
-// forms g once (500 x 29 x 700: slim 16.2 / 21.1 us, large 25.9 / 20.1; 256 x 512 x 512: 23.5 / 35.2 and 20.5 / 15.9;
-// 4000 x 64 x 64, where the slim kernel sums db over long columns: 118 / 157 and 24.4 / 24.7)
+// forms g once (float32 / bf16: 100 x 600 x 600 slim 13.2 / 25.7 us, large 18.4 / 18.6; 256 x 512 x 512: 20.8 / 31.9 and
+// 20.4 / 15.8; 500 x 16 x 500: 16.5 / 21.2 and 22.0 / 18.1; 4000 x 64 x 64, where the slim kernel sums db over long columns:
+// 117 / 157 and 24.4 / 24.4)
 Kernel bwd_kernel(const pvae_dense_bwd_args& a) {
     const int64_t dx = a.dx ? ceil_div(a.m, PVD_SM) * ceil_div(a.k, PVD_SN) : 0, dw = a.dw ? ceil_div(a.k, PVD_SM) * ceil_div(a.n, PVD_SN) : 0;
-    const int64_t reads = dx * 48 * a.n + dw * 48 * a.m, most = esize(a.dtype) == 4 ? int64_t(7) << 20 : int64_t(3) << 19;
-    return a.m <= 512 && dx + dw <= 1024 && reads <= most ? SLIM : LARGE;
+    const int64_t reads = dx * 48 * a.n + dw * 48 * a.m, most = esize(a.dtype) == 4 ? int64_t(10) << 20 : int64_t(3) << 19;
+    return a.m <= (esize(a.dtype) == 4 ? 512 : 256) && dx + dw <= 1024 && reads <= most ? SLIM : LARGE;
 }
 PvdTileJob tile_job(const PvdOperand& X, const PvdOperand& W, const PvdOut& O, int64_t K, int size, bool slim) {
     PvdTileJob J{X, W, O, K, (int)ceil_div(O.rows, slim ? PVD_SM : PVD_T), (int)ceil_div(O.cols, slim ? PVD_SN : PVD_T), 1, 0, nullptr};
