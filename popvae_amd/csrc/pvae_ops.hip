@@ -113,6 +113,10 @@ PvdOut output(int64_t rows, int64_t cols, void* y, int64_t ldy, const void* bias
     return {rows, cols, y, ldy, bias, res, ldr, pre, ldp, act};
 }
 
+// R rows of C contiguous elements as an operand that the large kernel reads as it lies: along the contraction, or across it
+bool lies_well(const void* p, int64_t R, int64_t C, int64_t ld, int size, bool along) {
+    return aligned(p, 16) && (R <= 1 || ld * size % 16 == 0) && (along ? C * size % 128 == 0 : R * size % 128 == 0 && C * size % 16 == 0);
+}
 // Which kernel makes y (microseconds, float32 / bf16, w as Keras keeps it):
 //                        rows         slim         tile         large
 //      1 x  512 x  512    7.7 /  8.1   5.9 /  5.5  11.1 /  9.4  15.0 /  9.0
@@ -126,22 +130,37 @@ PvdOut output(int64_t rows, int64_t cols, void* y, int64_t ldy, const void* bias
 //     64 x 4096 x 4096                55.7 / 45.2  39.9 / 19.6  34.6 / 17.0
 //   1000 x   16 x 4000                34.1 / 75.2  13.2 / 14.5  15.1 / 14.2
 //   1000 x  128 x 1000                14.9 / 18.1  11.8 /  9.0   9.5 / 11.1
+//                   ... k or n odd: w is laid out anew first
+//     16 x 3216 x 2854                23.0 / 21.0  33.8 / 20.3  42.4 / 26.1
+//     32 x  100 x 20000                9.4 / 13.0  13.5 /  9.1  18.3 / 15.1
+//     64 x 4001 x 4001                             50.1 / 28.5  62.8 / 36.0
+//    256 x 2401 x 1000                             28.5 / 18.1  33.1 / 21.1
+//    512 x 4001 x 4001                            289.3 / 124.8 181.3 / 51.7
 enum Kernel { ROWS, SLIM, TILE, LARGE };
-Kernel dense_kernel(int64_t m, int64_t k, int64_t n, int size) {
+Kernel dense_kernel(const pvae_dense_args& a) {
+    const int64_t m = a.m, k = a.k, n = a.n;
+    const int size = esize(a.dtype);
     // small results: the slim kernel's workgroups all find room, and what they read over and over (48 rows of contraction each)
     // stays small
     const int64_t slim = ceil_div(m, PVD_SM) * ceil_div(n, PVD_SN), reads = slim <= (size == 4 ? 1024 : 512) ? slim * 48 * k : INT64_MAX;
     // a few rows: the weights pass once, and the contraction is split over the chip and joined in a second launch.  The slim
     // kernel makes a small result in one (less than 4096 bytes of contraction), and needs far fewer pieces of a very long
-    // contraction; below 128 the rows kernel does not split either.  16-bit products of more than two rows over long
-    // contractions cost the rows kernel more arithmetic than reading.
+    // contraction (w^T, whose columns it reads sixteen bytes at a time, sooner: 1 x 700 x 8000 9.0 us, rows 10.6); below 128 the
+    // rows kernel does not split either.  16-bit products of more than two rows over long contractions cost the rows kernel
+    // more arithmetic than reading.
     if (m <= 4 && k > 0) {
-        if ((k * size < 4096 || k >= 16384) && (m > 2 || k >= 128) && reads <= int64_t(8) << 20) return SLIM;
+        if ((k * size < 4096 || k >= 16384) && (m > 2 || k >= 128) && reads <= int64_t(a.w_sk == 1 ? 20 : 8) << 20) return SLIM;
         if (size == 4 || m <= 2 || k < 4096) return ROWS;
     }
-    if (reads <= int64_t(16) << 20) return SLIM;
+    if (reads <= int64_t(size == 4 ? 16 : 12) << 20) return SLIM;
+    // where the large kernel would lay w out first, a few rows do not repay it: up to 32 the slim kernel reads w once as well,
+    // up to 64 the tile kernel
+    const bool lies = a.w_sk == 1 ? lies_well(a.w, n, k, a.w_sn, size, true) : lies_well(a.w, k, n, a.w_sk, size, false);
+    if (size == 4 && m <= (lies ? 16 : 32) && (k >= 256 || (!lies && k >= 64 && slim <= 2048))) return SLIM;
+    if (!lies && m <= 64) return TILE;
     // a short contraction never fills the large kernel's pipeline; 16-bit products are over sooner
-    if (size == 4 ? k >= 64 : k >= 1024 || (double)m * n * k >= 2147483648.0) return LARGE;
+    const double work = (double)m * n * k;
+    if (size == 4 ? k >= 64 && (lies || work >= 536870912.0) : lies ? k >= 1024 || work >= 536870912.0 : work >= 1073741824.0) return LARGE;
     return TILE;
 }
 // The gradients: slim while what its workgroups read stays small (every value of g is formed anew for each), else large, which
@@ -277,9 +296,8 @@ struct NtBuilder {
     // an operand given as memory rows (R rows of C contiguous elements): by_rows: its rows are the product's, else its columns;
     // may_across: the product takes it as it lies in that case
     NtOperand operand(const void* p, int64_t R, int64_t C, int64_t ld, bool by_rows, bool may_across) {
-        const bool pieces = aligned(p, 16) && (R <= 1 || ld * size % 16 == 0);
-        if (by_rows && pieces && C * size % 128 == 0) return {p, ld, (int)R, false};
-        if (!by_rows && may_across && pieces && R * size % 128 == 0 && C * size % 16 == 0) return {p, ld, (int)C, true};
+        if (by_rows && lies_well(p, R, C, ld, size, true)) return {p, ld, (int)R, false};
+        if (!by_rows && may_across && lies_well(p, R, C, ld, size, false)) return {p, ld, (int)C, true};
         PvdPack& J = source(p, R, C, ld, nullptr, 0, PVD_LINEAR);
         return by_rows ? same(J, false) : transposed(J);
     }
@@ -303,9 +321,10 @@ struct NtBuilder {
         };
         // 128 x 128 with eight waves, two workgroups to a CU (4096^3 bf16 with residual and z: 147 us; 128 x 256, one workgroup to
         // a CU, whose results nothing hides: 163; the products alone are 124 and 121).  float32 takes 64 x 64 (five to a CU)
-        // where 128 x 128 would give the CUs less than 40 steps each: matrix work is sixteen times slower there, and an
-        // uneven last round counts.
-        plan.tile = size == 4 && tile_steps(128) < 256 * 40 ? 64 : 128;
+        // where 128 x 128 would give the CUs less than 40 steps each -- matrix work is sixteen times slower there, and an
+        // uneven last round counts -- or would spend a fifth of its work on rows and columns that are not there
+        // (64 x 512 x 100000: 148 us, with 64 x 64 tiles 74).
+        plan.tile = size == 4 && (tile_steps(128) < 256 * 40 || tile_steps(64) * 5 < tile_steps(128) * 16) ? 64 : 128;
         const int64_t per = std::max<int64_t>(8, ceil_div(tile_steps(plan.tile), plan.tile == 64 ? 1024 : 512));
         int64_t tiles = 0;
         for (int i = 0; i < plan.jobs.n; ++i) {
@@ -586,7 +605,7 @@ const char* pvae_ops_last_error(void) { return g_err; }
 
 int64_t pvae_dense_workspace(const pvae_dense_args* a) {
     if (check_dense(a) || a->m == 0 || a->n == 0) return 0;
-    switch (dense_kernel(a->m, a->k, a->n, esize(a->dtype))) {
+    switch (dense_kernel(*a)) {
         case ROWS: return rows_bytes(rows_job(*a));
         case SLIM: return tile_job_bytes(dense_job(*a, true));
         case TILE: return tile_job_bytes(dense_job(*a, false));
@@ -598,7 +617,7 @@ int pvae_dense(const pvae_dense_args* a, void* workspace, int64_t workspace_byte
     if (int rc = check_dense(a)) return rc;
     if (a->m == 0 || a->n == 0) return 0;
     hipStream_t s = static_cast<hipStream_t>(hip_stream);
-    const Kernel kind = dense_kernel(a->m, a->k, a->n, esize(a->dtype));
+    const Kernel kind = dense_kernel(*a);
     if (kind == ROWS) {
         const PvdRowsJob J = rows_job(*a);
         if (int rc = check_workspace("pvae_dense", workspace, workspace_bytes, rows_bytes(J))) return rc;
