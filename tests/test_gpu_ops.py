@@ -568,3 +568,25 @@ def test_two_streams_at_once():
                 got[i] = work(i)
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
+
+
+# sizes at which the choice of kernel changes: few rows of odd weights, long and short contractions
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("m,k,n", [(1, 700, 8000), (2, 120, 1559), (3, 20_000, 5), (4, 5000, 70), (2, 3, 20_000), (9, 1216, 1301), (31, 300, 5003),
+                                   (48, 2401, 500), (130, 130, 515), (600, 130, 2500)])
+def test_what_lies_beside_an_operand_never_enters(m, k, n, dtype):
+    """Every operand is cut out of a buffer of NaN."""
+    def inside(t):
+        buf = torch.full((t.shape[0] + 2, t.shape[1] + 17), float("nan"), dtype=t.dtype, device="cuda")
+        view = buf[1:-1, 9:9 + t.shape[1]]
+        view.copy_(t)
+        return view
+
+    act = ACTS[(m + k + n) % 7]
+    for w_t in (False, True):
+        x, r, dy = (inside(rnd(m, j, dtype=dtype, seed=q)) for q, j in ((1, k), (2, n), (3, n)))
+        w = rnd(k, n, dtype=dtype, seed=4, scale=k ** -0.5)
+        w = inside(w.t()).t() if w_t else inside(w)
+        b, z = inside(rnd(1, n, dtype=dtype, seed=5))[0], inside(torch.zeros(m, n, device="cuda"))
+        check_forward(x, w, b, act, r, ops.dense(x, w, b, act, residual=r, pre=z), z)
+        check_backward(dy, x, w, z, act, None, *ops.dense_backward(dy, x, w, z, act))
