@@ -572,6 +572,7 @@ template <int DT, int R> __global__ __launch_bounds__(512) void pvk_dense_rows_t
 
 // The pieces of a split contraction, added in a fixed order, and what follows the product.  G lanes share four columns when
 // there are many pieces of a small result: lane g adds pieces g, g + G, ..., the G sums are added in turn.
+// Bound by its launch and the pieces' way from the L2: 4 to 5 us (eight pieces of 512 x 512 in float32 4.6).
 template <int DT, int G> __global__ __launch_bounds__(256) void pvk_dense_join(const PvdOut O, const float* __restrict__ part, int pieces) {
     const int64_t quads = (O.cols + 3) / 4, i = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
     const bool in = i < O.rows * quads;
@@ -763,11 +764,12 @@ template <int DT> __global__ __launch_bounds__(256) void pvk_dense_pack(const Pv
 // Pairs of pieces (float32: runs of four) of a line are exchanged by the line's number so that the lines which are read
 // together lie in different banks.
 // The direct loads write lane after lane, so the lanes choose their source accordingly.
-//   Measured: 4096 x 4096 x 4096 bf16 with bias, GELU, residual and z 142 us = 970 TFLOP/s (the products alone 122 us = 1.13
-// PFLOP/s, a library product 105 to 111), its two gradient products 145 us each way = 940; 2504 x 128 x 100000 float32 with
-// sigmoid 666 us = 96 TFLOP/s, 1.6 TB/s (150 TFLOP/s is what a library product reaches; a tile has four steps only, and 1 GB
-// of results with a sigmoid each).  What bounds it: the path from memory to LDS takes 64 bytes a clock per CU, which 128 x 128
-// tiles of 16-bit types use to three quarters, and the epilogue, which the other workgroup of the CU hides only partly.
+//   Measured: 4096 x 4096 x 4096 bf16 with bias, SiLU, residual and z 142 us = 970 TFLOP/s (the products alone 122 us = 1.13
+// PFLOP/s; a library product reaches 1.24 to 1.31); both gradient products of 4096 x 2048 x 4096 in one launch 145 us = 950;
+// 2504 x 128 x 100000 float32 with sigmoid 666 us = 96 TFLOP/s, 1.6 TB/s (a library product: 150 TFLOP/s; here a tile has four
+// steps only, and 1 GB of results takes a sigmoid each).  What bounds it: the path from memory to LDS moves 64 bytes a clock
+// per CU, which 128 x 128 tiles of 16-bit types use to three quarters, and the results' way out, which the CU's other
+// workgroup hides only partly.
 //   Tiles are numbered so that the workgroups of one XCD (blockIdx % 8) work on neighbouring tiles and find each other's
 // operands in their L2.
 // ---------------------------------------------------------------------------------------------
