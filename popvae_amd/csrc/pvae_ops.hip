@@ -194,7 +194,7 @@ int64_t tile_job_bytes(const PvdTileJob& J) { return J.splits > 1 ? (int64_t)J.s
 int launch_join(int dt, const PvdOut& O, const float* part, int pieces, hipStream_t s) {
     const int64_t quads = O.rows * ceil_div(O.cols, 4);
     // sixteen lanes to four columns where a lane of its own would leave the chip empty and walk a long way
-    if (pieces >= 16 && quads < 64 * 1024) {
+    if (pieces >= 16 ? quads < 64 * 1024 : pieces >= 4 && quads < 16 * 1024) {
         PVD_BY_TYPE(dt, hipLaunchKernelGGL((pvk_dense_join<D_, 16>), dim3((unsigned)ceil_div(quads, 16)), dim3(256), 0, s, O, part, pieces));
     } else {
         PVD_BY_TYPE(dt, hipLaunchKernelGGL((pvk_dense_join<D_, 1>), dim3((unsigned)ceil_div(quads, 256)), dim3(256), 0, s, O, part, pieces));
