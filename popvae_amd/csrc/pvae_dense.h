@@ -404,7 +404,7 @@ template <int DT> __global__ __launch_bounds__(512, 4) void pvk_dense_slim(const
 }
 
 // ---------------------------------------------------------------------------------------------
-// The rows kernel, for up to four rows (one point asked for an answer): the weights are read once, and that is its time.  A
+// The rows kernel, for up to four rows, float32 up to eight (one point asked for an answer): the weights are read once, and that is its time.  A
 // lane holds sixteen bytes of a row of w and all rows' sums of those columns in registers; x, as float32, comes from LDS.  The
 // workgroup's eight waves, and pieces of the grid, split the contraction.  Matrix instructions would compute sixteen rows for
 // one and need w transposed on the way; plain ones keep up with memory as long as rows are few.  1 x 128 x 100000 in

@@ -125,6 +125,8 @@ bool lies_well(const void* p, int64_t R, int64_t C, int64_t ld, int size, bool a
 //      1 x 4096 x 4096   21.2 / 10.9  27.8 / 27.1  37.4 / 18.0  29.4 / 14.4
 //      2 x 100000 x 3    17.0 / 23.8  11.2 / 12.2  25.0 / 17.1  26.2 / 20.1
 //      4 x 8192 x 4096   32.8 / 22.1  49.9 / 48.2  64.7 / 26.6  48.8 / 18.9
+//      8 x 3159 x 6998   29.1 / 37.8  40.1 / 36.3  64.7 / 31.4  71.1 / 38.5
+//      8 x  512 x 100000 41.9 / 40.6  64.3 / 72.4  84.5 / 35.7  72.7 / 27.1
 //     32 x 1024 x 1024                 9.4 /  8.1  13.4 / 10.9  12.8 / 16.5
 //    256 x  512 x  512                 7.4 /  6.4  13.0 / 10.6  16.4 / 12.7
 //     64 x 4096 x 4096                55.7 / 45.2  39.9 / 19.6  34.6 / 17.0
@@ -153,14 +155,17 @@ Kernel dense_kernel(const pvae_dense_args& a) {
         if (size == 4 || m <= 2 || k < 4096) return ROWS;
     }
     if (reads <= int64_t(size == 4 ? 16 : 12) << 20) return SLIM;
+    // up to eight float32 rows over large weights (16-bit ones: the large kernel is as good)
+    if (size == 4 && m <= 8 && (double)k * n >= (a.w_sk == 1 ? 48 : 16) * 1048576.0) return ROWS;
     // where the large kernel would lay w out first, a few rows do not repay it: up to 32 the slim kernel reads w once as well,
     // up to 64 the tile kernel
     const bool lies = a.w_sk == 1 ? lies_well(a.w, n, k, a.w_sn, size, true) : lies_well(a.w, k, n, a.w_sk, size, false);
     if (size == 4 && m <= (lies ? 16 : 32) && (k >= 256 || (!lies && k >= 64 && slim <= 2048))) return SLIM;
     if (!lies && m <= 64) return TILE;
-    // a short contraction never fills the large kernel's pipeline; 16-bit products are over sooner
+    // a short contraction never fills the large kernel's pipeline; 16-bit products are over sooner, but it reads large weights
+    // faster than the tile kernel (5 x 512 x 100000 bf16: 27 and 36 us)
     const double work = (double)m * n * k;
-    if (size == 4 ? k >= 64 && (lies || work >= 536870912.0) : lies ? k >= 1024 || work >= 536870912.0 : work >= 1073741824.0) return LARGE;
+    if (size == 4 ? k >= 64 && (lies || work >= 536870912.0) : lies ? k >= 1024 || work >= 536870912.0 || (double)k * n >= 8388608.0 : work >= 1073741824.0) return LARGE;
     return TILE;
 }
 // The gradients: slim while what its workgroups read stays small (every value of g is formed anew for each), else large, which
@@ -232,7 +237,8 @@ int run_rows(const pvae_dense_args& a, PvdRowsJob J, void* workspace, hipStream_
     PVD_BY_TYPE(a.dtype, {
         if (a.m == 1) launch_rows<D_, 1>(J, t, s);
         else if (a.m == 2) launch_rows<D_, 2>(J, t, s);
-        else launch_rows<D_, 4>(J, t, s);
+        else if (D_ != PVD_F32 || a.m <= 4) launch_rows<D_, 4>(J, t, s);
+        else launch_rows<PVD_F32, 8>(J, t, s);
     });
     if (int rc = launched("dense_rows")) return rc;
     return J.splits > 1 ? launch_join(a.dtype, J.O, J.part, J.splits, s) : 0;

@@ -573,7 +573,7 @@ def test_two_streams_at_once():
 # sizes at which the choice of kernel changes: few rows of odd weights, long and short contractions
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("m,k,n", [(1, 700, 8000), (2, 120, 1559), (3, 20_000, 5), (4, 5000, 70), (2, 3, 20_000), (9, 1216, 1301), (31, 300, 5003),
-                                   (48, 2401, 500), (130, 130, 515), (600, 130, 2500)])
+                                   (48, 2401, 500), (130, 130, 515), (600, 130, 2500), (7, 2401, 7003), (5, 520, 100_003)])
 def test_what_lies_beside_an_operand_never_enters(m, k, n, dtype):
     """Every operand is cut out of a buffer of NaN."""
     def inside(t):
