@@ -3,9 +3,9 @@
  *
  * They take device pointers of the caller's own tensors (the engine of pvae.h keeps its own) and run on the stream that is
  * passed, on the current device; nothing is allocated, nothing waits for the GPU, and every launch may be captured into a
- * graph.  Where a call needs scratch memory the caller passes it: pvae_*_workspace says how many bytes, the memory belongs
- * to the call until its work on the stream is done, and no call finds in it what another one left.  Two calls that may run
- * at the same time need a workspace each.
+ * graph.  Where a call needs scratch memory the caller passes it: pvae_*_workspace says how many bytes for those very
+ * arguments, addresses and strides included; the memory belongs to the call until its work on the stream is done, and no call
+ * finds in it what another one left.  Two calls that may run at the same time need a workspace each.
  *
  * Every function returns 0 or a negative code; pvae_ops_last_error() gives the calling thread's text.  A refused call has
  * launched nothing.
