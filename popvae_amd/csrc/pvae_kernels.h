@@ -2790,9 +2790,16 @@ __device__ __forceinline__ void pv_enc_bwd_train(const float* __restrict__ W1, c
         request(bk[0], blk);
         words(blk, xw, xn);
     }
-    for (int i = tid; i < 32 * T * ldp; i += 256) {
-        const int b = i / ldp, u = i % ldp;
-        smem[((u / WG_UNITS) * (32 * T) + b) * WG_UNITS + (u % WG_UNITS)] = dpre[i];
+    // eight requests under way at a time: one after another they cost a round trip each (2 us a step at 100 000 SNPs)
+    for (int i0 = tid; i0 < 32 * T * ldp; i0 += 8 * 256) {
+        float d[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) d[j] = dpre[min(i0 + 256 * j, 32 * T * ldp - 1)];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int i = i0 + 256 * j, b = i / ldp, u = i % ldp;
+            if (i < 32 * T * ldp) smem[((u / WG_UNITS) * (32 * T) + b) * WG_UNITS + (u % WG_UNITS)] = d[j];
+        }
     }
     __syncthreads();
     PV_WT(1, 1);
@@ -2901,9 +2908,15 @@ __global__ __launch_bounds__(256, 2) void pvk_enc_bwd(const float* __restrict__ 
     const int slot = __builtin_amdgcn_readfirstlane((int)(blockIdx.x / ngrp) * 4 + wave), nslots = (gridDim.x / ngrp) * 4;
     const float alpha = st->alpha;
     const bool acc_grads = MODE == PV_MODE_GRAD && st->acc != 0;
-    for (int i = tid; i < 32 * T * ldp; i += 256) {
-        const int b = i / ldp, u = i % ldp;
-        smem[((u / WG_UNITS) * (32 * T) + b) * WG_UNITS + (u % WG_UNITS)] = dpre[i];
+    for (int i0 = tid; i0 < 32 * T * ldp; i0 += 8 * 256) {
+        float d[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) d[j] = dpre[min(i0 + 256 * j, 32 * T * ldp - 1)];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int i = i0 + 256 * j, b = i / ldp, u = i % ldp;
+            if (i < 32 * T * ldp) smem[((u / WG_UNITS) * (32 * T) + b) * WG_UNITS + (u % WG_UNITS)] = d[j];
+        }
     }
     __syncthreads();
     for (int blk = slot; blk < nblk; blk += nslots) {
