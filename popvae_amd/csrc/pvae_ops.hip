@@ -92,12 +92,18 @@ Extent weights_extent(const void* w, int64_t k, int64_t n, int64_t sk, int64_t s
     return {"w", lo, lo + (uintptr_t)(((k - 1) * sk + (n - 1) * sn + 1) * size)};
 }
 
-// an operand of the tile and slim kernels: rows x K
-PvdOperand operand(const void* p, int64_t rows, int64_t cols_k, int64_t sr, int64_t sk) {
+// Arguments that passed their checks, as the choice of kernel and all plans take them: w with a single row or column may come
+// with any strides, and the one that is never used becomes 1, so that one of the two always is.
+template <typename Args> Args plain(const Args& a) {
+    Args b = a;
+    if (b.w_sk != 1 && b.w_sn != 1) (b.n == 1 ? b.w_sn : b.w_sk) = 1;
+    return b;
+}
+// an operand of the tile and slim kernels: rows x K, one of the strides 1
+PvdOperand operand(const void* p, int64_t rows, int64_t sr, int64_t sk) {
     PvdOperand o{};
     o.p = p;
     o.rows = rows;
-    if (sk != 1 && sr != 1) (cols_k == 1 ? sk : sr) = 1;  // a single row or column: its stride is never used
     o.sr = sr;
     o.sk = sk;
     return o;
@@ -425,7 +431,7 @@ NtPlan large_bwd(const pvae_dense_bwd_args& a, void* ws) {
 }
 PvdTileJob dense_job(const pvae_dense_args& a, bool slim) {
     const int size = esize(a.dtype);
-    return tile_job(operand(a.x, a.m, a.k, a.ldx, 1), operand(a.w, a.n, a.k, a.w_sn, a.w_sk),
+    return tile_job(operand(a.x, a.m, a.ldx, 1), operand(a.w, a.n, a.w_sn, a.w_sk),
                     output(a.m, a.n, a.y, a.ldy, a.bias, a.residual, a.ldr, a.pre, a.ldp, a.act), a.k, size, slim);
 }
 int check_dense(const pvae_dense_args* a) {
@@ -456,15 +462,15 @@ struct BwdPlan {
 BwdPlan bwd_plan(const pvae_dense_bwd_args& a) {
     const int size = esize(a.dtype);
     BwdPlan p{};
-    PvdOperand gx = operand(a.dy, a.m, a.n, a.lddy, 1), gw = operand(a.dy, a.n, a.m, 1, a.lddy);
+    PvdOperand gx = operand(a.dy, a.m, a.lddy, 1), gw = operand(a.dy, a.n, 1, a.lddy);
     with_grad(gx, a.pre, a.ldp, 1, a.act);
     with_grad(gw, a.pre, 1, a.ldp, a.act);
     // w as an operand of dx: rows are the k of the layer, the contraction its n
     if (a.dx)
-        p.J.dx = tile_job(gx, operand(a.w, a.k, a.n, a.w_sk, a.w_sn),
+        p.J.dx = tile_job(gx, operand(a.w, a.k, a.w_sk, a.w_sn),
                           output(a.m, a.k, a.dx, a.lddx, nullptr, a.dx_add, a.ldadd, nullptr, 0, PVD_LINEAR), a.n, size, true);
     if (a.dw)
-        p.J.dw = tile_job(operand(a.x, a.k, a.m, 1, a.ldx), gw,
+        p.J.dw = tile_job(operand(a.x, a.k, 1, a.ldx), gw,
                           output(a.k, a.n, a.dw, a.n, nullptr, nullptr, 0, nullptr, 0, PVD_LINEAR), a.m, size, true);
     p.J.n_dx = a.dx ? (int64_t)p.J.dx.mt * p.J.dx.nt * p.J.dx.splits : 0;
     p.J.n_dw = a.dw ? (int64_t)p.J.dw.mt * p.J.dw.nt * p.J.dw.splits : 0;
@@ -609,70 +615,74 @@ extern "C" {
 
 const char* pvae_ops_last_error(void) { return g_err; }
 
-int64_t pvae_dense_workspace(const pvae_dense_args* a) {
-    if (check_dense(a) || a->m == 0 || a->n == 0) return 0;
-    switch (dense_kernel(*a)) {
-        case ROWS: return rows_bytes(rows_job(*a));
-        case SLIM: return tile_job_bytes(dense_job(*a, true));
-        case TILE: return tile_job_bytes(dense_job(*a, false));
-        default: return large_dense(*a, nullptr).bytes;
+int64_t pvae_dense_workspace(const pvae_dense_args* args) {
+    if (check_dense(args) || args->m == 0 || args->n == 0) return 0;
+    const pvae_dense_args a = plain(*args);
+    switch (dense_kernel(a)) {
+        case ROWS: return rows_bytes(rows_job(a));
+        case SLIM: return tile_job_bytes(dense_job(a, true));
+        case TILE: return tile_job_bytes(dense_job(a, false));
+        default: return large_dense(a, nullptr).bytes;
     }
 }
 
-int pvae_dense(const pvae_dense_args* a, void* workspace, int64_t workspace_bytes, void* hip_stream) {
-    if (int rc = check_dense(a)) return rc;
-    if (a->m == 0 || a->n == 0) return 0;
+int pvae_dense(const pvae_dense_args* args, void* workspace, int64_t workspace_bytes, void* hip_stream) {
+    if (int rc = check_dense(args)) return rc;
+    if (args->m == 0 || args->n == 0) return 0;
+    const pvae_dense_args a = plain(*args);
     hipStream_t s = static_cast<hipStream_t>(hip_stream);
-    const Kernel kind = dense_kernel(*a);
+    const Kernel kind = dense_kernel(a);
     if (kind == ROWS) {
-        const PvdRowsJob J = rows_job(*a);
+        const PvdRowsJob J = rows_job(a);
         if (int rc = check_workspace("pvae_dense", workspace, workspace_bytes, rows_bytes(J))) return rc;
-        return run_rows(*a, J, workspace, s);
+        return run_rows(a, J, workspace, s);
     }
     if (kind == LARGE) {
-        NtPlan plan = large_dense(*a, workspace);
+        NtPlan plan = large_dense(a, workspace);
         if (int rc = check_workspace("pvae_dense", workspace, workspace_bytes, plan.bytes)) return rc;
-        return launch_large(a->dtype, plan, s);
+        return launch_large(a.dtype, plan, s);
     }
-    PvdTileJob J = dense_job(*a, kind == SLIM);
+    PvdTileJob J = dense_job(a, kind == SLIM);
     if (int rc = check_workspace("pvae_dense", workspace, workspace_bytes, tile_job_bytes(J))) return rc;
     const int64_t blocks = (int64_t)J.mt * J.nt * J.splits;
     if (int rc = check_grid(blocks)) return rc;
     J.part = static_cast<float*>(workspace);
     if (kind == SLIM) {
-        PVD_BY_TYPE(a->dtype, hipLaunchKernelGGL(pvk_dense_slim<D_>, dim3((unsigned)blocks), dim3(512), 0, s, J));
+        PVD_BY_TYPE(a.dtype, hipLaunchKernelGGL(pvk_dense_slim<D_>, dim3((unsigned)blocks), dim3(512), 0, s, J));
     } else {
-        PVD_BY_TYPE(a->dtype, hipLaunchKernelGGL(pvk_dense_tile<D_>, dim3((unsigned)blocks), dim3(256), 0, s, J));
+        PVD_BY_TYPE(a.dtype, hipLaunchKernelGGL(pvk_dense_tile<D_>, dim3((unsigned)blocks), dim3(256), 0, s, J));
     }
     if (int rc = launched("dense")) return rc;
-    return J.splits > 1 ? launch_join(a->dtype, J.O, J.part, J.splits, s) : 0;
+    return J.splits > 1 ? launch_join(a.dtype, J.O, J.part, J.splits, s) : 0;
 }
 
-int64_t pvae_dense_bwd_workspace(const pvae_dense_bwd_args* a) {
-    if (check_dense_bwd(a)) return 0;
-    return bwd_kernel(*a) == SLIM ? bwd_bytes(bwd_plan(*a)) : large_bwd(*a, nullptr).bytes;
+int64_t pvae_dense_bwd_workspace(const pvae_dense_bwd_args* args) {
+    if (check_dense_bwd(args)) return 0;
+    const pvae_dense_bwd_args a = plain(*args);
+    return bwd_kernel(a) == SLIM ? bwd_bytes(bwd_plan(a)) : large_bwd(a, nullptr).bytes;
 }
 
-int pvae_dense_bwd(const pvae_dense_bwd_args* a, void* workspace, int64_t workspace_bytes, void* hip_stream) {
-    if (int rc = check_dense_bwd(a)) return rc;
+int pvae_dense_bwd(const pvae_dense_bwd_args* args, void* workspace, int64_t workspace_bytes, void* hip_stream) {
+    if (int rc = check_dense_bwd(args)) return rc;
+    const pvae_dense_bwd_args a = plain(*args);
     hipStream_t s = static_cast<hipStream_t>(hip_stream);
-    if (bwd_kernel(*a) == LARGE) {
-        NtPlan plan = large_bwd(*a, workspace);
+    if (bwd_kernel(a) == LARGE) {
+        NtPlan plan = large_bwd(a, workspace);
         if (int rc = check_workspace("pvae_dense_bwd", workspace, workspace_bytes, plan.bytes)) return rc;
-        return launch_large(a->dtype, plan, s);
+        return launch_large(a.dtype, plan, s);
     }
-    BwdPlan p = bwd_plan(*a);
+    BwdPlan p = bwd_plan(a);
     if (int rc = check_workspace("pvae_dense_bwd", workspace, workspace_bytes, bwd_bytes(p))) return rc;
     const int64_t blocks = p.J.n_dx + p.J.n_dw + p.n_db;
     if (blocks == 0) return 0;
     p.J.dx.part = static_cast<float*>(workspace);
     p.J.dw.part = static_cast<float*>(workspace) + (p.J.n_dx ? tile_job_bytes(p.J.dx) / 4 : 0);
-    PVD_BY_TYPE(a->dtype, hipLaunchKernelGGL(pvk_dense_bwd_slim<D_>, dim3((unsigned)blocks), dim3(512), 0, s, p.J));
+    PVD_BY_TYPE(a.dtype, hipLaunchKernelGGL(pvk_dense_bwd_slim<D_>, dim3((unsigned)blocks), dim3(512), 0, s, p.J));
     if (int rc = launched("dense_bwd")) return rc;
     if (p.J.n_dx && p.J.dx.splits > 1)
-        if (int rc = launch_join(a->dtype, p.J.dx.O, p.J.dx.part, p.J.dx.splits, s)) return rc;
+        if (int rc = launch_join(a.dtype, p.J.dx.O, p.J.dx.part, p.J.dx.splits, s)) return rc;
     if (p.J.n_dw && p.J.dw.splits > 1)
-        if (int rc = launch_join(a->dtype, p.J.dw.O, p.J.dw.part, p.J.dw.splits, s)) return rc;
+        if (int rc = launch_join(a.dtype, p.J.dw.O, p.J.dw.part, p.J.dw.splits, s)) return rc;
     return 0;
 }
 

@@ -1,0 +1,96 @@
+"""The operators on device tensors (popvae_amd.ops) at the edges of what they take, against 64-bit formulas.
+
+Where the inputs are small whole numbers and f' is 0 or 1 (linear, relu), every product and every sum is exact in float32
+(below 2^24), so a result is the exact one rounded once to its type: such tests compare bit for bit, and one product lost,
+added or taken from a neighbour shows.  Elsewhere the tolerances count roundings: u = 2^-24, h = finfo.eps / 2 of the type,
+tiny = half its smallest subnormal."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+from popvae_amd import ops
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+TYPES = [F32, BF16, F16]
+
+
+def whole(*shape, dtype=F32, seed=0, top=2):
+    """Whole numbers -top .. top."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randint(-top, top + 1, shape, generator=g, device="cuda").to(dtype)
+
+
+def rnd(*shape, dtype=F32, seed=0, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(shape, generator=g, device="cuda") * scale).to(dtype)
+
+
+def f64(t):
+    return t.double().contiguous()
+
+
+def half(t):
+    return torch.finfo(t).eps / 2, torch.finfo(t).smallest_normal * torch.finfo(t).eps / 2
+
+
+def act64(z, name):
+    return {"linear": lambda: z, "relu": lambda: z.clamp(min=0), "elu": lambda: torch.where(z > 0, z, torch.expm1(z)),
+            "sigmoid": lambda: torch.sigmoid(z), "tanh": lambda: torch.tanh(z), "silu": lambda: z * torch.sigmoid(z),
+            "gelu": lambda: z * torch.erfc(-z / math.sqrt(2)) / 2}[name]()
+
+
+def dact64(z, name):
+    z = z.clone().requires_grad_(True)
+    act64(z, name).sum().backward()
+    return z.grad
+
+
+def grads64(dy, x, w, z, act):
+    """dx, dw and db in 64 bits."""
+    g = f64(dy) if act == "linear" else f64(dy) * dact64(f64(z), act)
+    return g @ f64(w).t().contiguous(), f64(x).t().contiguous() @ g, g.sum(0)
+
+
+def check(got, want, bound, what):
+    got = got.double()
+    bad = ~((got - want).abs() <= bound)
+    assert not bad.any(), (what, int(bad.sum()), float((got - want).abs().max()), float(bound.max()))
+
+
+def check_exact(x, w, dy, z, dtype):
+    """Forward and gradients of whole numbers, bit for bit."""
+    pre = torch.empty(x.shape[0], w.shape[1], device="cuda")
+    y = ops.dense(x, w, activation="relu", pre=pre)
+    want = f64(x) @ f64(w)
+    assert torch.equal(pre.double(), want) and torch.equal(y, want.clamp(min=0).to(dtype))
+    for act in ("relu", "linear"):
+        got = ops.dense_backward(dy, x, w, z, act)
+        for name, a, b in zip(("dx", "dw", "db"), got, grads64(dy, x, w, z, act)):
+            assert torch.equal(a, b.to(dtype)), (act, name, int((a.double() != b).sum()))
+
+
+# one column, or one row, of weights cut out of a wider tensor: neither stride is 1
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m", [3, 40, 600, 2000])
+def test_a_single_column_or_row_of_weights_with_any_strides(m, dtype):
+    k, n = 70, 70
+    x, dy, z = whole(m, k, dtype=dtype, seed=1), whole(m, 1, dtype=dtype, seed=2), rnd(m, 1, seed=3)
+    w = whole(k, 10, dtype=dtype, seed=4)[:, ::5][:, :1]
+    assert w.stride() == (10, 5)
+    check_exact(x, w, dy, z, dtype)
+    x, dy, z = whole(m, 1, dtype=dtype, seed=5), whole(m, n, dtype=dtype, seed=6), rnd(m, n, seed=7)
+    w = whole(9, 3 * n, dtype=dtype, seed=8)[::7, ::3][:1]
+    assert w.stride() == (21 * n, 3)
+    check_exact(x, w, dy, z, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_a_single_row_of_weights_in_the_large_kernel(dtype):
+    """k = 1 and a result of 2^30 elements, w's only row with neither stride 1: every product is exact."""
+    m = n = 1 << 15
+    x, w = whole(m, 1, dtype=dtype, seed=1), whole(9, 3 * n, dtype=dtype, seed=2)[::7, ::3][:1]
+    assert torch.equal(ops.dense(x, w), x * w)
