@@ -294,7 +294,8 @@ template <int DT, bool GRAD> struct PvdSlim {
     alignas(16) float z[VEC];
 
     __device__ __forceinline__ void load(const PvdOperand& P, int64_t row, int64_t k, int64_t k1) {
-        const bool grad = GRAD && P.act != PVD_LINEAR, in = row < P.rows, whole = P.sk == 1 && k + VEC <= k1;
+        const bool grad = GRAD && P.act != PVD_LINEAR, in = row < P.rows;
+        const bool whole = P.sk == 1 && (!grad || P.pk == 1) && k + VEC <= k1;  // z's stride is its own (dy of one column, z of more)
         const int64_t rr = min(row, P.rows - 1);
         const T* p = static_cast<const T*>(P.p) + rr * P.sr;
         const float* pz = grad ? P.pre + rr * P.pr : nullptr;

@@ -94,3 +94,15 @@ def test_a_single_row_of_weights_in_the_large_kernel(dtype):
     m = n = 1 << 15
     x, w = whole(m, 1, dtype=dtype, seed=1), whole(9, 3 * n, dtype=dtype, seed=2)[::7, ::3][:1]
     assert torch.equal(ops.dense(x, w), x * w)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m", [2, 9, 40, 300, 700])
+@pytest.mark.parametrize("dy_ld,pre_ld", [(1, 4), (1, 7), (5, 1), (3, 2)])
+def test_a_single_output_with_strided_pre_or_dy(m, dy_ld, pre_ld, dtype):
+    """n = 1: dy's rows lie next to each other and pre's do not, or the other way round."""
+    k = 33
+    x, w = whole(m, k, dtype=dtype, seed=1), whole(k, 1, dtype=dtype, seed=2)
+    dy = whole(m, dy_ld, dtype=dtype, seed=3)[:, dy_ld // 2:][:, :1]
+    z = rnd(m, pre_ld, seed=4)[:, pre_ld // 2:][:, :1]
+    check_exact(x, w, dy, z, dtype)
