@@ -359,6 +359,7 @@ template <int DT, bool GX, bool GW> __device__ __forceinline__ void pvd_slim_job
     const bool gx = GX && J.X.act != PVD_LINEAR, gw = GW && J.W.act != PVD_LINEAR;
     const int halves = m0 + 16 < J.X.rows ? 2 : 1;
     pvd_f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    pvd_f32x4 low[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};  // the second terms' products
     for (int64_t k = k0 + wave * (RUN * KS); k < k1; k += PVD_SW * RUN * KS) {
         PvdSlim<DT, GW> a[RUN];
         PvdSlim<DT, GX> b[RUN][2];
@@ -379,11 +380,19 @@ template <int DT, bool GX, bool GW> __device__ __forceinline__ void pvd_slim_job
                     if (j < halves) {
                         if (gx) b[u][j].grad(J.X.act, bl);
                         acc[j] = pvd_mfma16<DT>(a[u].bits(), b[u][j].bits(), acc[j]);
-                        if (DT != PVD_F32 && gw) acc[j] = pvd_mfma16<DT>(al, b[u][j].bits(), acc[j]);
-                        if (DT != PVD_F32 && gx) acc[j] = pvd_mfma16<DT>(a[u].bits(), bl, acc[j]);
+                        if (DT != PVD_F32 && gw) low[j] = pvd_mfma16<DT>(al, b[u][j].bits(), low[j]);
+                        if (DT != PVD_F32 && gx) low[j] = pvd_mfma16<DT>(a[u].bits(), bl, low[j]);
                     }
             }
         }
+    }
+    // a second term meets the same infinities of the other operand as the first and would turn them into NaN (0 inf, inf - inf)
+    if constexpr (DT != PVD_F32 && (GX || GW)) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (fabsf(acc[j][e]) < __builtin_inff()) acc[j][e] += low[j][e];
     }
     // red[wave][row][16 columns]
 #pragma unroll

@@ -106,3 +106,17 @@ def test_a_single_output_with_strided_pre_or_dy(m, dy_ld, pre_ld, dtype):
     dy = whole(m, dy_ld, dtype=dtype, seed=3)[:, dy_ld // 2:][:, :1]
     z = rnd(m, pre_ld, seed=4)[:, pre_ld // 2:][:, :1]
     check_exact(x, w, dy, z, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,k,n", [(5, 9, 4), (40, 70, 50), (260, 24, 20), (700, 256, 300)])
+@pytest.mark.parametrize("act", ["silu", "relu", "elu"])
+def test_infinities_in_the_gradients_operands(m, k, n, act, dtype):
+    """An infinite x or w makes the gradients that it enters infinite, with the formula's sign, whatever kernel runs; NaN
+    only where the formula has it (0 times infinity, infinities of both signs)."""
+    x, w, dy, z = rnd(m, k, dtype=dtype, seed=1), rnd(k, n, dtype=dtype, seed=2), rnd(m, n, dtype=dtype, seed=3), rnd(m, n, seed=4)
+    x[1, 3], x[m - 1, 0], w[2, 1], w[k - 1, n - 1] = float("inf"), float("-inf"), float("-inf"), float("inf")
+    dy[0] = 1.0  # exact in every type
+    for name, a, b in zip(("dx", "dw", "db"), ops.dense_backward(dy, x, w, z, act), grads64(dy, x, w, z, act)):
+        assert torch.equal(a.isnan(), b.isnan()), (name, int(a.isnan().sum()), int(b.isnan().sum()))
+        assert torch.equal(a.isinf(), b.isinf()) and torch.equal(a[a.isinf()].double(), b[b.isinf()]), name
