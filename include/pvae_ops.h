@@ -56,7 +56,8 @@ int pvae_dense(const pvae_dense_args* a, void* workspace, int64_t workspace_byte
  * dy [m][n]; pre [m][n] float32 (NULL with PVAE_LINEAR); dx [m][k], dw [k][n] contiguous, dbias [n]: each may be NULL.
  * dx_add [m][k] with row stride ldadd, or NULL: added to dx before its one rounding (a layer whose residual is its own
  * input passes dy; dx may be dx_add itself).  dpre [m][n] float32 contiguous, or NULL: receives g.
- * g enters the products in the tensors' type (16-bit types: rounded once at most); dbias sums the unrounded g. */
+ * g of a 16-bit type enters the products in two terms of the type (bf16: 16 bits of g; float16: 22 bits, to 2^-35 at worst, and
+ * above the type's largest value), so dx and dw are rounded once, at their end; dbias sums the unrounded g. */
 typedef struct pvae_dense_bwd_args {
     int32_t dtype, act;
     int64_t m, k, n;

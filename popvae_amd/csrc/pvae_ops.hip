@@ -259,7 +259,8 @@ struct NtOperand {
     const void* p;
     int64_t ld;   // elements
     int rows;
-    bool across;  // [K][rows]: contiguous along the rows
+    bool across;      // [K][rows]: contiguous along the rows
+    int64_t low = 0;  // g's second terms: bytes from the first
 };
 
 struct NtPlan {
@@ -268,6 +269,7 @@ struct NtPlan {
     int64_t bytes = 0;     // workspace
     int tile = 0;          // its edge
     bool deep = false;
+    bool two = false;      // g in two terms: every product goes through its contraction twice
 };
 
 struct NtBuilder {
@@ -316,8 +318,8 @@ struct NtBuilder {
     void product(const NtOperand& x, const NtOperand& w, int64_t K, const PvdOut& O) {
         PvdNtJob& J = plan.jobs.job[plan.jobs.n++];
         J = PvdNtJob{};
-        J.x = static_cast<const char*>(x.p); J.ldx = x.ld * size; J.x_rows = x.rows; J.x_across = x.across;
-        J.w = static_cast<const char*>(w.p); J.ldw = w.ld * size; J.w_rows = w.rows; J.w_across = w.across;
+        J.x = static_cast<const char*>(x.p); J.ldx = x.ld * size; J.x_rows = x.rows; J.x_across = x.across; J.x_low = x.low;
+        J.w = static_cast<const char*>(w.p); J.ldw = w.ld * size; J.w_rows = w.rows; J.w_across = w.across; J.w_low = w.low;
         J.steps = (int)ceil_div(K * size, 128);
         J.O = O;
     }
@@ -329,7 +331,7 @@ struct NtBuilder {
                 const PvdNtJob& J = plan.jobs.job[i];
                 n += ceil_div(J.O.rows, edge) * ceil_div(J.O.cols, edge) * J.steps;
             }
-            return n;
+            return plan.two ? 2 * n : n;
         };
         // 128 x 128 with eight waves, two workgroups to a CU (4096^3 bf16 with residual and z: 147 us; 128 x 256, one workgroup to
         // a CU, whose results nothing hides: 163; the products alone are 124 and 121).  float32 takes 64 x 64 (five to a CU)
@@ -337,7 +339,8 @@ struct NtBuilder {
         // uneven last round counts -- or would spend a fifth of its work on rows and columns that are not there
         // (64 x 512 x 100000: 148 us, with 64 x 64 tiles 74).
         plan.tile = size == 4 && (tile_steps(128) < 256 * 40 || tile_steps(64) * 5 < tile_steps(128) * 16) ? 64 : 128;
-        const int64_t per = std::max<int64_t>(8, ceil_div(tile_steps(plan.tile), plan.tile == 64 ? 1024 : 512));
+        int64_t per = std::max<int64_t>(8, ceil_div(tile_steps(plan.tile), plan.tile == 64 ? 1024 : 512));
+        if (plan.two) per = ceil_div(per, 2);  // steps of the contraction, each gone through twice
         int64_t tiles = 0;
         for (int i = 0; i < plan.jobs.n; ++i) {
             PvdNtJob& J = plan.jobs.job[i];
@@ -364,12 +367,12 @@ struct NtBuilder {
     }
 };
 
-template <int DT, int TM, int WM, int WN, int ST> int launch_nt(const PvdNtJobs& P, int blocks, hipStream_t s) {
-    typedef PvdNt<DT, TM, TM, WM, WN, ST> K;
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(pvk_dense_nt<DT, TM, TM, WM, WN, ST>),
+template <int DT, int TM, int WM, int WN, int ST, bool TWO = false> int launch_nt(const PvdNtJobs& P, int blocks, hipStream_t s) {
+    typedef PvdNt<DT, TM, TM, WM, WN, ST, TWO> K;
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(pvk_dense_nt<DT, TM, TM, WM, WN, ST, TWO>),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, K::LDS);
     if (e != hipSuccess) return refuse(-10, "%d bytes of LDS: %s", (int)K::LDS, hipGetErrorString(e));
-    hipLaunchKernelGGL((pvk_dense_nt<DT, TM, TM, WM, WN, ST>), dim3(blocks), dim3(K::THREADS), K::LDS, s, P);
+    hipLaunchKernelGGL((pvk_dense_nt<DT, TM, TM, WM, WN, ST, TWO>), dim3(blocks), dim3(K::THREADS), K::LDS, s, P);
     return launched("dense_nt");
 }
 int launch_large(int dt, NtPlan& plan, hipStream_t s) {
@@ -390,6 +393,8 @@ int launch_large(int dt, NtPlan& plan, hipStream_t s) {
     const int blocks = (int)at;
     if (blocks == 0) return 0;
     if (plan.tile == 64) rc = launch_nt<PVD_F32, 64, 4, 1, 2>(P, blocks, s);
+    else if (plan.two && dt == PVD_BF16) rc = plan.deep ? launch_nt<PVD_BF16, 128, 4, 2, 4, true>(P, blocks, s) : launch_nt<PVD_BF16, 128, 4, 2, 2, true>(P, blocks, s);
+    else if (plan.two) rc = plan.deep ? launch_nt<PVD_F16, 128, 4, 2, 4, true>(P, blocks, s) : launch_nt<PVD_F16, 128, 4, 2, 2, true>(P, blocks, s);
     else PVD_BY_TYPE(dt, (rc = plan.deep ? launch_nt<D_, 128, 4, 2, 4>(P, blocks, s) : launch_nt<D_, 128, 4, 2, 2>(P, blocks, s)));
     if (rc) return rc;
     for (int i = 0; i < P.n; ++i)
@@ -409,7 +414,13 @@ NtPlan large_bwd(const pvae_dense_bwd_args& a, void* ws) {
     NtBuilder B(a.dtype, ws);
     // g: rows of the contraction for dx (over n), lines of it for dw (over m); its column sums, and unrounded if asked for
     PvdPack& g = B.source(a.dy, a.m, a.n, a.lddy, a.pre, a.ldp, a.act);
-    const NtOperand gw = B.same(g, true), gx{gw.p, gw.ld, (int)a.m, false};
+    NtOperand gw = B.same(g, true);
+    if (B.size == 2 && g.pre) {
+        g.low = B.take(g.h_same * g.ld_same * B.size);
+        gw.low = static_cast<char*>(g.low) - static_cast<char*>(g.same);
+        B.plan.two = true;
+    }
+    const NtOperand gx{gw.p, gw.ld, (int)a.m, false, gw.low};
     g.g32 = a.dpre;
     if (a.dbias) {
         g.sums = static_cast<float*>(B.take(ceil_div(a.m, 64) * a.n * 4));

@@ -181,7 +181,7 @@ def dense_backward(dy, x, w, pre=None, activation="linear", dx_add=None, need_dx
 
     dy [m, n]; x, w and activation as in the forward, pre what it left (not needed for "linear").  dx_add [m, k] is added to
     dx before its rounding: a layer whose residual is its own input passes dy.  (The gradient of the residual is dy itself;
-    summed over the rows for an expanded one.)  With a 16-bit type, dy * f'(pre) is rounded to it at most once before the two products."""
+    summed over the rows for an expanded one.)  dx, dw and db are rounded to their type once, at their end."""
     dtype, device, m, k, n, ldx = _layer(x, w)
     if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):

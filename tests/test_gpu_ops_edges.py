@@ -120,3 +120,45 @@ def test_infinities_in_the_gradients_operands(m, k, n, act, dtype):
     for name, a, b in zip(("dx", "dw", "db"), ops.dense_backward(dy, x, w, z, act), grads64(dy, x, w, z, act)):
         assert torch.equal(a.isnan(), b.isnan()), (name, int(a.isnan().sum()), int(b.isnan().sum()))
         assert torch.equal(a.isinf(), b.isinf()) and torch.equal(a[a.isinf()].double(), b[b.isinf()]), name
+
+
+def check_gradients_rounded_once(dy, x, w, z, act, dtype):
+    """dx and dw are off by what f' (16 u (1 + |z|)), g's two terms (bf16: 2^-17 of g; f16: 2^-21 and 2^-35; float32: u) and
+    float32 sums (u a term) are off by, and one rounding of the result: a rounding of g to a 16-bit type is not in it."""
+    dx, dw, _ = ops.dense_backward(dy, x, w, z, act)
+    X, W, DY, Z = f64(x), f64(w), f64(dy), f64(z)
+    G = DY * dact64(Z, act)
+    rel, least = {F32: (2 * U, 0.0), BF16: (2.0 ** -17, 0.0), F16: (2.0 ** -21, 2.0 ** -35)}[dtype]
+    eg = 16 * U * (1 + Z.abs()) * DY.abs() + rel * G.abs() + least
+    h, tiny = half(dtype)
+    for what, got, want, e, terms, size in (
+            ("dx", dx, G @ W.t().contiguous(), eg @ W.t().abs().contiguous(), W.shape[1], (G.abs() + eg) @ W.t().abs().contiguous()),
+            ("dw", dw, X.t().contiguous() @ G, X.t().abs().contiguous() @ eg, X.shape[0], X.t().abs().contiguous() @ (G.abs() + eg))):
+        # a sum of `terms` values (twice as many with two terms of g) is off by u a term of the values' sizes
+        e = e + (2 * terms + 8) * U * size
+        check(got, want, e + h * (want.abs() + e) + tiny, (what, act))
+
+
+# few terms to a sum, so that a second rounding could not hide among others; both kernels of the gradients
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,k,n", [(1, 5, 3), (2, 300, 2), (3, 40, 1), (40, 30, 3), (200, 17, 40), (300, 260, 2), (700, 300, 3),
+                                   (700, 512, 16), (260, 2000, 1), (2048, 24, 8), (513, 130, 70), (1024, 256, 512)])
+def test_gradients_are_rounded_once(m, k, n, dtype):
+    for act in ("gelu", "tanh"):
+        x, w, dy, z = rnd(m, k, dtype=dtype, seed=1), rnd(k, n, dtype=dtype, seed=2), rnd(m, n, dtype=dtype, seed=3), rnd(m, n, seed=4)
+        check_gradients_rounded_once(dy, x, w, z, act, dtype)
+        check_gradients_rounded_once(dy, x, rnd(n, k, dtype=dtype, seed=5).t(), z, act, dtype)
+
+
+@pytest.mark.parametrize("m,k,n", [(3, 20, 4), (40, 30, 50), (300, 30, 50), (700, 256, 300)])
+def test_half_precision_gradients_beyond_the_types_range(m, k, n):
+    """float16: dy f'(pre) below the least subnormal or above the largest value, while the gradients themselves fit."""
+    z = rnd(m, n, seed=4)
+    small = rnd(m, n, dtype=F16, seed=3, scale=2.0 ** -22)
+    x, w = rnd(m, k, dtype=F16, seed=1, scale=2.0 ** 10), rnd(k, n, dtype=F16, seed=2, scale=2.0 ** 10)
+    for act in ("silu", "sigmoid"):
+        check_gradients_rounded_once(small, x, w, z, act, F16)
+    large = torch.where(rnd(m, n, seed=5) > 0, 60000.0, -61000.0).to(F16)  # times gelu'(sqrt 2) = 1.128: above 65504
+    z = torch.full((m, n), math.sqrt(2.0), device="cuda")
+    x, w = rnd(m, k, dtype=F16, seed=1, scale=2.0 ** -9), rnd(k, n, dtype=F16, seed=2, scale=2.0 ** -9)
+    check_gradients_rounded_once(large, x, w, z, "gelu", F16)
