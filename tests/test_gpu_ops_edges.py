@@ -162,3 +162,35 @@ def test_half_precision_gradients_beyond_the_types_range(m, k, n):
     z = torch.full((m, n), math.sqrt(2.0), device="cuda")
     x, w = rnd(m, k, dtype=F16, seed=1, scale=2.0 ** -9), rnd(k, n, dtype=F16, seed=2, scale=2.0 ** -9)
     check_gradients_rounded_once(large, x, w, z, "gelu", F16)
+
+
+def test_activations_far_from_zero():
+    """The tails of the activations and their derivatives in float32, relative to their own size: exp, the sum and the
+    reciprocal are off by 5 u together, every product by u more."""
+    z = torch.cat([torch.linspace(-80, 80, 40_001, device="cuda"), -torch.logspace(-6, 1.9, 999, device="cuda")])[:, None].contiguous()
+    one = torch.ones(1, 1, device="cuda")
+    Z = z.double()
+    s, q = torch.sigmoid(Z), torch.sigmoid(-Z)
+    check(ops.dense(z, one, activation="sigmoid"), s, 8 * U * s, "sigmoid")
+    check(ops.dense(z, one, activation="silu"), Z * s, 10 * U * (Z * s).abs(), "silu")
+
+    def slope(act):
+        return ops.dense_backward(torch.ones_like(z), z, one, z, act, need_dw=False, need_bias=False)[0]
+
+    check(slope("sigmoid"), s * q, 18 * U * s * q, "sigmoid'")
+    check(slope("elu"), torch.exp(Z.clamp(max=0)), 4 * U * torch.exp(Z.clamp(max=0)), "elu'")
+    check(slope("silu"), s * (1 + Z * q), 18 * U * s * (1 + Z.abs() * q), "silu'")
+    phi = torch.exp(-Z * Z / 2) / math.sqrt(2 * math.pi)
+    # z^2 / 2 is rounded before exp sees it (u z^2 / 2, relative); Phi comes from 1 + erf: 4 u absolute
+    check(slope("gelu"), torch.special.ndtr(Z) + Z * phi, 4 * U + (10 + Z * Z) * U * (Z * phi).abs(), "gelu'")
+
+
+def test_activations_of_infinities_and_nan():
+    z = torch.tensor([[float("inf")], [float("-inf")], [float("nan")], [3e38], [-3e38]], device="cuda")
+    one = torch.ones(1, 1, device="cuda")
+    for act in ("sigmoid", "tanh", "relu", "elu"):
+        y = ops.dense(z, one, activation=act)
+        assert torch.equal(torch.nan_to_num(y.double(), 7.0, 8.0, 9.0), torch.nan_to_num(act64(z.double(), act), 7.0, 8.0, 9.0)), act
+        g = ops.dense_backward(torch.ones_like(z), z, one, z, act, need_dw=False, need_bias=False)[0]
+        want = {"sigmoid": [0.0, 0.0, 0.0, 0.0], "tanh": [0.0, 0.0, 0.0, 0.0], "relu": [1.0, 0.0, 1.0, 0.0], "elu": [1.0, 0.0, 1.0, 0.0]}[act]
+        assert g[[0, 1, 3, 4], 0].tolist() == want, act
