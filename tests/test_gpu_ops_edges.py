@@ -194,3 +194,41 @@ def test_activations_of_infinities_and_nan():
         g = ops.dense_backward(torch.ones_like(z), z, one, z, act, need_dw=False, need_bias=False)[0]
         want = {"sigmoid": [0.0, 0.0, 0.0, 0.0], "tanh": [0.0, 0.0, 0.0, 0.0], "relu": [1.0, 0.0, 1.0, 0.0], "elu": [1.0, 0.0, 1.0, 0.0]}[act]
         assert g[[0, 1, 3, 4], 0].tolist() == want, act
+
+
+# contractions in pieces and their remainders, ragged ends, unaligned rows, long sums over rows: nothing may be lost, added
+# or taken twice
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,k,n", [(1, 8192, 96), (2, 70_001, 33), (4, 1000, 4099), (8, 3159, 2001), (16, 8192, 130), (33, 5000, 65),
+                                   (64, 4001, 403), (130, 70_001, 129), (192, 8192, 256), (5, 2048, 4099), (5, 520, 100_003),
+                                   (600, 2500, 17), (20_011, 24, 40), (4000, 64, 64), (1543, 1021, 515), (70_001, 130, 3)])
+def test_whole_numbers_are_exact(m, k, n, dtype):
+    x, dy, z = whole(m, k, dtype=dtype, seed=1), whole(m, n, dtype=dtype, seed=2), rnd(m, n, seed=3)
+    check_exact(x, whole(k, n, dtype=dtype, seed=4), dy, z, dtype)
+    check_exact(x, whole(n, k, dtype=dtype, seed=5).t(), dy, z, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,k,n", [(1, 4, 1), (32, 128, 128), (33, 65, 129), (700, 40, 70), (600, 256, 513)])
+def test_g_itself(m, k, n, dtype):
+    """pvae_dense_bwd's dpre, unrounded, from both kernels, alone and beside the gradients."""
+    x, w, dy, z = rnd(m, k, dtype=dtype, seed=1), rnd(k, n, dtype=dtype, seed=2), rnd(m, n, dtype=dtype, seed=3), rnd(m, n, seed=4)
+    L = ops.lib()
+    for act in ("linear", "relu", "gelu"):
+        G = f64(dy) if act == "linear" else f64(dy) * dact64(f64(z), act)
+        bound = 0 * G if act != "gelu" else 16 * U * (1 + f64(z).abs()) * f64(dy).abs() + U * G.abs()
+        for alone in (False, True):
+            g = torch.full((m + 1, n), float("nan"), device="cuda")
+            dx, dw, db = torch.empty_like(x), torch.empty(k, n, dtype=dtype, device="cuda"), torch.empty(n, dtype=dtype, device="cuda")
+            a = ops._DenseBwd(dtype=ops.DTYPES[dtype], act=ops.ACTIVATIONS[act], m=m, k=k, n=n, dy=dy.data_ptr(), lddy=n, x=x.data_ptr(),
+                              ldx=k, w=w.data_ptr(), w_sk=n, w_sn=1, pre=z.data_ptr(), ldp=n, dpre=g.data_ptr())
+            if not alone:
+                a.dx, a.lddx, a.dw, a.dbias = dx.data_ptr(), k, dw.data_ptr(), db.data_ptr()
+            need = L.pvae_dense_bwd_workspace(C.byref(a))
+            work = torch.empty(max(1, need), dtype=torch.uint8, device="cuda")
+            assert L.pvae_dense_bwd(C.byref(a), work.data_ptr(), need, torch.cuda.current_stream().cuda_stream) == 0
+            check(g[:m], G, bound, act)
+            assert bool(g[m].isnan().all())
+            if not alone:
+                want = ops.dense_backward(dy, x, w, z, act)
+                assert all(torch.equal(p, q) for p, q in zip((dx, dw, db), want))
