@@ -845,10 +845,13 @@ typedef __attribute__((address_space(3))) pvd_s16x4* pvd_ltr;
 
 // Lane l's sixteen bytes at `from` go to lds + 16 l (lds: the same for the wave).  Written out because the compiler, given its
 // builtin, waits for every such load in flight before each transposing read of LDS (128 x 256 bf16 tiles: 165 us instead of
-// 121 for 4096^3); the loads are waited for in PvdNt::arrived, and write no registers.  Nothing else in the kernel uses m0.
+// 121 for 4096^3); the loads are waited for in PvdNt::arrived, and write no registers.
 __device__ __forceinline__ void pvd_load_to_lds(const char* from, char* lds) {
     const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(pvd_lptr)lds);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "memory");
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // m0 is the compiler's own and not kept across this: so it is meant
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "memory", "m0");
+#pragma clang diagnostic pop
 }
 
 // What follows the product for ROWS x 64 products of one wave in LDS (row r's piece u of four floats at slot u ^ (r & 15)):
