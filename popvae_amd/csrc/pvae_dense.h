@@ -897,25 +897,24 @@ template <int DT, int ROWS> __device__ __forceinline__ void pvd_finish_rows(cons
         pvd_finish4<DT>(O, m + r, c, *reinterpret_cast<const pvd_f32x4*>(ep + r * 64 + ((eu ^ (r & 15)) << 2)));
 }
 
-// TM x TN: tile (x's rows, the weights' columns); WM x WN: waves; ST: steps that LDS holds; TWO: one side is g in two terms, and
-// a piece's steps are gone through once with each
-template <int DT, int TM, int TN, int WM, int WN, int ST, bool TWO> struct PvdNt {
-    enum { WAVES = WM * WN, THREADS = 64 * WAVES, BUF = (TM + TN) * 128, LDS = ST * BUF, FM = TM / WM / 16, FN = TN / WN / 16 };
-    enum { LOADS = (TM + TN) / (8 * WAVES) };                          // direct loads of a wave per step
-    enum { GB = FM * FN <= 16 ? FM : 16 / FN, GROUPS = 2 * FM / GB };  // a step's matrix work: groups of FN x GB fragments
-    enum { FITS = LDS / WAVES / 256, POW = FITS >= 128 ? 128 : FITS >= 64 ? 64 : FITS >= 32 ? 32 : 16 };
-    enum { EPR = POW < TM / WM ? POW : TM / WM };                      // rows of a wave's result that its share of LDS takes at once
-    static_assert(TM % (8 * WAVES) == 0 && TN % (8 * WAVES) == 0, "rows are loaded eight per wave");
-    static_assert(FN % 4 == 0 && FITS >= 16 && (TM / WM) % EPR == 0, "a wave's result goes out in pieces 64 columns wide");
+// EDGE: of the tile (x's rows, the weights' columns); WM x WN: waves; ST: steps that LDS holds, two or
+// four; TWO: one side is g in two terms, and a piece's steps are gone through once with each
+template <int DT, int EDGE, int WM, int WN, int ST, bool TWO> struct PvdNt {
+    enum { WAVES = WM * WN, THREADS = 64 * WAVES, SIDE = EDGE * 128, BUF = 2 * SIDE, LDS = ST * BUF };
+    enum { ROWS = EDGE / WM, FM = ROWS / 16, FN = EDGE / WN / 16 };  // a wave's rows, its fragments of either side
+    enum { LOADS = 2 * EDGE / (8 * WAVES) };                         // direct loads of a wave per step
+    static_assert(EDGE % (8 * WAVES) == 0, "rows are loaded eight per wave");
+    static_assert(FN % 4 == 0 && LDS >= WAVES * ROWS * 256, "a wave's result goes out through its share of LDS");
+    static_assert(ST == 2 || ST == 4, "what `arrived` waits for");
 
     enum { SIZE = PvdType<DT>::SIZE, VEC = PvdType<DT>::VEC, KST = 128 / SIZE };  // KST: contraction of a step
 
     // the exchange of pieces of line k of an operand across, in pieces
     static __device__ __forceinline__ int across_swap(int k) { return DT == PVD_F32 ? 4 * ((k >> 2) & 3) : 2 * ((k & 3) | ((k >> 3 & 1) << 2)); }
-    // What this lane loads of rows [row0, row0 + ROWS) and step s: a step's rows are ROWS / 8 loads of a wave, load i lies at
+    // What this lane loads of rows [row0, row0 + EDGE) and step s: a step's rows are EDGE / 8 loads of a wave, load i lies at
     // i * 1024 in LDS.  Rows behind the end repeat the last ones (their results are dropped).
-    template <int ROWS, bool ACROSS> struct Source {
-        enum { N = ROWS / (8 * WAVES) };
+    template <bool ACROSS> struct Source {
+        enum { N = EDGE / (8 * WAVES) };
         const char* at[N];
         int64_t step;
         __device__ __forceinline__ Source(const char* p, int64_t ld, int rows, int row0, int s) {
@@ -925,7 +924,7 @@ template <int DT, int TM, int TN, int WM, int WN, int ST, bool TWO> struct PvdNt
             for (int u = 0; u < N; ++u) {
                 const int i = u * WAVES + wave;
                 if constexpr (ACROSS) {
-                    enum { PIECES = ROWS * SIZE / 16, LINES = 64 / PIECES };  // pieces of a line, lines of a load
+                    enum { PIECES = EDGE * SIZE / 16, LINES = 64 / PIECES };  // pieces of a line, lines of a load
                     const int k = i * LINES + lane / PIECES, piece = (lane % PIECES) ^ across_swap(k);
                     at[u] = p + k * ld + (int64_t)min(row0 + piece * VEC, rows - VEC) * SIZE;
                 } else {
@@ -948,28 +947,28 @@ template <int DT, int TM, int TN, int WM, int WN, int ST, bool TWO> struct PvdNt
         }
     };
     // the fragment of rows row0 .. row0 + 15 (a multiple of sixteen) and half h of a step
-    template <int ROWS, bool ACROSS> static __device__ __forceinline__ pvd_u32x4 fragment(const char* lds, int row0, int h) {
+    template <bool ACROSS> static __device__ __forceinline__ pvd_u32x4 fragment(const char* lds, int row0, int h) {
         const int lane = threadIdx.x & 63, r16 = lane & 15, q = lane >> 4;
         if constexpr (!ACROSS) {
             return piece(lds, row0 + r16, 4 * h + q);
         } else if constexpr (DT == PVD_F32) {
-            const char* at = lds + (16 * h + 4 * q) * (ROWS * 4) + ((((row0 + r16) >> 2) ^ 4 * q) << 4) + (r16 & 3) * 4;
+            const char* at = lds + (16 * h + 4 * q) * (EDGE * 4) + ((((row0 + r16) >> 2) ^ 4 * q) << 4) + (r16 & 3) * 4;
             pvd_u32x4 v;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = *reinterpret_cast<const unsigned*>(at + e * (ROWS * 4));
+            for (int e = 0; e < 4; ++e) v[e] = *reinterpret_cast<const unsigned*>(at + e * (EDGE * 4));
             return v;
         } else {
             const int k = 32 * h + 8 * q + (r16 >> 2);  // this lane's line of the first four; k + 4 has the same exchange
-            const char* at = lds + k * (ROWS * 2) + (((row0 >> 3) ^ across_swap(k)) << 4) + (r16 & 3) * 8;
+            const char* at = lds + k * (EDGE * 2) + (((row0 >> 3) ^ across_swap(k)) << 4) + (r16 & 3) * 8;
             const pvd_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pvd_ltr)at);
-            const pvd_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pvd_ltr)(at + 4 * (ROWS * 2)));
+            const pvd_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pvd_ltr)(at + 4 * (EDGE * 2)));
             return __builtin_bit_cast(pvd_u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         }
     }
     // all but the last `steps` steps that this wave has asked for have arrived, its own reads of LDS too; then every wave's
     static __device__ __forceinline__ void arrived(int steps) {
-        if (ST > 3 && steps >= 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * LOADS) : "memory");
-        else if (ST > 2 && steps >= 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS) : "memory");
+        if (ST == 4 && steps >= 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * LOADS) : "memory");
+        else if (ST == 4 && steps == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS) : "memory");
         else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
@@ -992,22 +991,22 @@ template <int DT, int TM, int TN, int WM, int WN, int ST, bool TWO> struct PvdNt
         const int pc = t / tiles;
         t -= pc * tiles;
         const int per_band = J.band * J.nt, bi = t / per_band, in = t - bi * per_band, bh = min(J.band, J.mt - bi * J.band);
-        const int m0 = (bi * J.band + in % bh) * TM, n0 = in / bh * TN;
+        const int m0 = (bi * J.band + in % bh) * EDGE, n0 = in / bh * EDGE;
         const int s0 = pc * J.per, len = min(J.steps, s0 + J.per) - s0, steps = TWO ? 2 * len : len;
-        const int wm = (wave % WM) * (TM / WM), wn = (wave / WM) * (TN / WN);
+        const int wm = (wave % WM) * ROWS, wn = (wave / WM) * (EDGE / WN);
         pvd_f32x4 acc[FN][FM];
 #pragma unroll
         for (int i = 0; i < FN; ++i)
 #pragma unroll
             for (int k = 0; k < FM; ++k) acc[i][k] = (pvd_f32x4){0.f, 0.f, 0.f, 0.f};
-        Source<TM, XA> sx(J.x, J.ldx, J.x_rows, m0, s0);
-        Source<TN, WA> sw(J.w, J.ldw, J.w_rows, n0, s0);
+        Source<XA> sx(J.x, J.ldx, J.x_rows, m0, s0);
+        Source<WA> sw(J.w, J.ldw, J.w_rows, n0, s0);
         // TWO: the second terms first, so that what infinities of the other side make of them can be dropped
         if (TWO) sx.move(J.x_low), sw.move(J.w_low);
         int asked = 0;
         auto get = [&](int slot) {
             sx.load(smem + slot * BUF);
-            sw.load(smem + slot * BUF + TM * 128);
+            sw.load(smem + slot * BUF + SIDE);
             if (TWO && ++asked == len) {  // the piece once more, with the first terms
                 sx.move(-J.x_low - len * sx.step);
                 sw.move(-J.w_low - len * sw.step);
@@ -1021,38 +1020,35 @@ template <int DT, int TM, int TN, int WM, int WN, int ST, bool TWO> struct PvdNt
 #pragma unroll
                     for (int e = 0; e < 4; ++e) acc[i][k][e] = f(acc[i][k][e]);
         };
-        // The fragments of a group are read from LDS while the group before them is multiplied, a quarter into it -- across
-        // steps too: behind the first quarter of a step's last group the waves meet, and the next step's first fragments come
-        // in under the rest.
-        pvd_u32x4 a[2][FN], b[2][GB];
-        auto read = [&](const char* lds, int g) {
-            const int h = g / (FM / GB), k0 = g % (FM / GB) * GB;
-            if (k0 == 0)
+        // A step is two halves.  The fragments of one are read from LDS while the other is multiplied, a quarter into it --
+        // across steps too: behind the first quarter of a step's second half the waves meet, and the next step's first fragments
+        // come in under the rest.
+        pvd_u32x4 a[2][FN], b[2][FM];
+        auto read = [&](const char* lds, int h) {
 #pragma unroll
-                for (int i = 0; i < FN; ++i) a[h][i] = fragment<TN, WA>(lds + TM * 128, wn + 16 * i, h);
+            for (int i = 0; i < FN; ++i) a[h][i] = fragment<WA>(lds + SIDE, wn + 16 * i, h);
 #pragma unroll
-            for (int k = 0; k < GB; ++k) b[g & 1][k] = fragment<TM, XA>(lds, wm + 16 * (k0 + k), h);
+            for (int k = 0; k < FM; ++k) b[h][k] = fragment<XA>(lds, wm + 16 * k, h);
         };
-        auto multiply = [&](int g, int from, int to) {
-            const int h = g / (FM / GB), k0 = g % (FM / GB) * GB;
+        auto multiply = [&](int h, int from, int to) {
             if constexpr (DT == PVD_F32) {  // the four products of a fragment apart from each other: each adds to what the last one left
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
 #pragma unroll
                     for (int u = from; u < to; ++u) {
                         const int k = u / FN, i = u % FN;
-                        acc[i][k0 + k] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[h][i][e]), __uint_as_float(b[g & 1][k][e]), acc[i][k0 + k], 0, 0, 0);
+                        acc[i][k] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[h][i][e]), __uint_as_float(b[h][k][e]), acc[i][k], 0, 0, 0);
                     }
             } else {
 #pragma unroll
                 for (int u = from; u < to; ++u) {
                     const int k = u / FN, i = u % FN;
-                    acc[i][k0 + k] = pvd_mfma16<DT>(a[h][i], b[g & 1][k], acc[i][k0 + k]);
+                    acc[i][k] = pvd_mfma16<DT>(a[h][i], b[h][k], acc[i][k]);
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
         };
-        enum { EACH = FN * GB, FIRST = EACH / 4 };
+        enum { HALVES = 2, EACH = FN * FM, FIRST = EACH / 4 };
 #pragma unroll
         for (int j = 0; j < ST - 1; ++j)
             if (j < steps) get(j);
@@ -1063,42 +1059,41 @@ template <int DT, int TM, int TN, int WM, int WN, int ST, bool TWO> struct PvdNt
             const char* lds = smem + cur * BUF;
             if (s + ST - 1 < steps) get(cur == 0 ? ST - 1 : cur - 1);
 #pragma unroll
-            for (int g = 0; g + 1 < GROUPS; ++g) {
-                multiply(g, 0, FIRST);
-                read(lds, g + 1);
+            for (int h = 0; h < HALVES - 1; ++h) {
+                multiply(h, 0, FIRST);
+                read(lds, h + 1);
                 __builtin_amdgcn_sched_barrier(0);
-                multiply(g, FIRST, EACH);
+                multiply(h, FIRST, EACH);
             }
-            multiply(GROUPS - 1, 0, FIRST);
+            multiply(HALVES - 1, 0, FIRST);
             cur = cur + 1 == ST ? 0 : cur + 1;
             if (s + 1 < steps) {
                 arrived(min(ST - 2, steps - 2 - s));
                 read(smem + cur * BUF, 0);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            multiply(GROUPS - 1, FIRST, EACH);
+            multiply(HALVES - 1, FIRST, EACH);
             if (TWO && s + 1 == len)  // behind the second terms
                 each_sum([](float a) { return fabsf(a) < __builtin_inff() ? a * PvdTerms<DT>::LOW : 0.f; });
         }
         if (TWO && PvdTerms<DT>::UNIT != 1.f) each_sum([](float a) { return a * PvdTerms<DT>::UNIT; });
         arrived(0);
-        // through LDS, as many rows at a time as fit, so that sixteen lanes read and write 64 consecutive columns of a row; the
-        // sixteen pieces of a row of 64 floats are spread by the row's number
-        float* ep = reinterpret_cast<float*>(smem) + wave * EPR * 64;
+        // through LDS, 64 columns at a time, so that sixteen lanes read and write consecutive columns of a row; the sixteen pieces of
+        // a row of 64 floats are spread by the row's number
+        float* ep = reinterpret_cast<float*>(smem) + wave * ROWS * 64;
 #pragma unroll
-        for (int kc = 0; kc < FM * 16 / EPR * (FN / 4); ++kc) {
-            const int k0 = kc / (FN / 4) * (EPR / 16), i0 = kc % (FN / 4) * 4;
+        for (int i0 = 0; i0 < FN; i0 += 4) {
 #pragma unroll
-            for (int k = 0; k < EPR / 16; ++k)
+            for (int k = 0; k < FM; ++k)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    *reinterpret_cast<pvd_f32x4*>(ep + (16 * k + r16) * 64 + (((4 * i + q) ^ r16) << 2)) = acc[i0 + i][k0 + k];
+                    *reinterpret_cast<pvd_f32x4*>(ep + (16 * k + r16) * 64 + (((4 * i + q) ^ r16) << 2)) = acc[i0 + i][k];
             same_wave();
-            const int64_t m = m0 + wm + 16 * k0, n = n0 + wn + 16 * i0;
+            const int64_t m = m0 + wm, n = n0 + wn + 16 * i0;
             if (J.splits == 1) {
-                pvd_finish_rows<DT, EPR>(J.O, m, n, ep);
+                pvd_finish_rows<DT, ROWS>(J.O, m, n, ep);
             } else {
-                for (int row = lane >> 4; row < EPR && m + row < J.O.rows; row += 4) {
+                for (int row = lane >> 4; row < ROWS && m + row < J.O.rows; row += 4) {
                     const int u = lane & 15;
                     const pvd_f32x4 z = *reinterpret_cast<const pvd_f32x4*>(ep + row * 64 + ((u ^ (row & 15)) << 2));
                     if (n + 4 * u < J.O.cols)
@@ -1110,14 +1105,14 @@ template <int DT, int TM, int TN, int WM, int WN, int ST, bool TWO> struct PvdNt
     }
 };
 
-template <int DT, int TM, int TN, int WM, int WN, int ST, bool TWO>
+template <int DT, int EDGE, int WM, int WN, int ST, bool TWO>
 __global__ __launch_bounds__(64 * WM * WN) void pvk_dense_nt(const PvdNtJobs P) {
     extern __shared__ __attribute__((aligned(1024))) char pvd_smem[];
     typedef typename PvdType<DT>::T T;
     const int b = blockIdx.x;
     if (b < P.first[2]) {
         const int j = b >= P.first[1];
-        typedef PvdNt<DT, TM, TN, WM, WN, ST, TWO> K;
+        typedef PvdNt<DT, EDGE, WM, WN, ST, TWO> K;
         const PvdNtJob& J = P.job[j];
         if (!J.w_across) return K::template run<false, false>(J, b - P.first[j], pvd_smem);
         if (!J.x_across) return K::template run<false, true>(J, b - P.first[j], pvd_smem);

@@ -367,12 +367,12 @@ struct NtBuilder {
     }
 };
 
-template <int DT, int TM, int WM, int WN, int ST, bool TWO = false> int launch_nt(const PvdNtJobs& P, int blocks, hipStream_t s) {
-    typedef PvdNt<DT, TM, TM, WM, WN, ST, TWO> K;
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(pvk_dense_nt<DT, TM, TM, WM, WN, ST, TWO>),
+template <int DT, int EDGE, int WM, int WN, int ST, bool TWO = false> int launch_nt(const PvdNtJobs& P, int blocks, hipStream_t s) {
+    typedef PvdNt<DT, EDGE, WM, WN, ST, TWO> K;
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(pvk_dense_nt<DT, EDGE, WM, WN, ST, TWO>),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, K::LDS);
     if (e != hipSuccess) return refuse(-10, "%d bytes of LDS: %s", (int)K::LDS, hipGetErrorString(e));
-    hipLaunchKernelGGL((pvk_dense_nt<DT, TM, TM, WM, WN, ST, TWO>), dim3(blocks), dim3(K::THREADS), K::LDS, s, P);
+    hipLaunchKernelGGL((pvk_dense_nt<DT, EDGE, WM, WN, ST, TWO>), dim3(blocks), dim3(K::THREADS), K::LDS, s, P);
     return launched("dense_nt");
 }
 int launch_large(int dt, NtPlan& plan, hipStream_t s) {
