@@ -31,7 +31,8 @@ const char* pvae_ops_last_error(void);
  * w [k][n]: element (i, j) at i * w_sk + j * w_sn, one of the two strides 1 (Keras kernels: w_sn == 1).
  * bias [n] or NULL.  residual [m][n] with row stride ldr (0: one row added to every row) or NULL.
  * pre [m][n] float32, row stride ldp, or NULL: receives z = x w + bias, which pvae_dense_bwd reads.
- * y may be the residual itself; otherwise outputs overlap neither each other nor an input.
+ * y may be the residual itself; otherwise outputs share no byte with each other or an input (they may be other columns of one
+ * buffer; with row strides of different lengths their ranges have to be apart).
  * m, k, n >= 0; with k == 0 z is the bias. */
 typedef struct pvae_dense_args {
     int32_t dtype, act;

@@ -70,26 +70,36 @@ int check_grid(int64_t blocks) {
     return 0;
 }
 
-// the bytes that a matrix of `rows` rows of `cols` elements reaches; an output may not meet another output or an input
+// The bytes of a matrix: `rows` runs of `width`, `pitch` apart (pitch 0: one row for all).  An output may not meet another
+// output or an input, but may lie between the rows of one: column ranges of one buffer are apart.
 struct Extent {
     const char* name;
     uintptr_t lo, hi;
+    int64_t rows;
+    uintptr_t pitch, width;
 };
 Extent extent(const char* name, const void* p, int64_t rows, int64_t cols, int64_t ld, int size) {
-    if (!p || rows == 0 || cols == 0) return {name, 0, 0};
-    const uintptr_t lo = reinterpret_cast<uintptr_t>(p);
-    return {name, lo, lo + (uintptr_t)(((rows - 1) * ld + cols) * size)};
+    if (!p || rows == 0 || cols == 0) return {name, 0, 0, 0, 0, 0};
+    if (ld == 0) rows = 1;
+    const uintptr_t lo = reinterpret_cast<uintptr_t>(p), pitch = (uintptr_t)(ld * size), width = (uintptr_t)(cols * size);
+    return {name, lo, lo + (uintptr_t)(rows - 1) * pitch + width, rows, pitch, width};
+}
+bool meet(const Extent& a, const Extent& b) {
+    if (a.lo >= b.hi || b.lo >= a.hi) return false;
+    if (a.lo > b.lo) return meet(b, a);
+    if ((a.rows == 1 && b.rows == 1) || (a.rows > 1 && b.rows > 1 && a.pitch != b.pitch)) return true;
+    // b's runs begin `d` behind those of a (a single row's, too), all `pitch` apart
+    const uintptr_t pitch = a.rows > 1 ? a.pitch : b.pitch, d = (b.lo - a.lo) % pitch;
+    return d < a.width || d + b.width > pitch;
 }
 int check_apart(const Extent* e, int n_out, int n) {  // e[0 .. n_out) are outputs
     for (int i = 0; i < n_out; ++i)
         for (int j = i + 1; j < n; ++j)
-            if (e[i].lo < e[j].hi && e[j].lo < e[i].hi) return refuse(-2, "%s overlaps %s", e[i].name, e[j].name);
+            if (meet(e[i], e[j])) return refuse(-2, "%s overlaps %s", e[i].name, e[j].name);
     return 0;
 }
 Extent weights_extent(const void* w, int64_t k, int64_t n, int64_t sk, int64_t sn, int size) {
-    if (!w || k == 0 || n == 0) return {"w", 0, 0};
-    const uintptr_t lo = reinterpret_cast<uintptr_t>(w);
-    return {"w", lo, lo + (uintptr_t)(((k - 1) * sk + (n - 1) * sn + 1) * size)};
+    return sn == 1 || n == 1 ? extent("w", w, k, n, sk, size) : extent("w", w, n, k, sn, size);
 }
 
 // Arguments that passed their checks, as the choice of kernel and all plans take them: w with a single row or column may come
@@ -521,7 +531,7 @@ int check_dense_bwd(const pvae_dense_bwd_args* a) {
                         extent("dbias", a->dbias, 1, a->n, a->n, size), extent("dpre", a->dpre, a->m, a->n, a->n, 4),
                         extent("dy", a->dy, a->m, a->n, a->lddy, size), extent("pre", a->act == PVAE_LINEAR ? nullptr : a->pre, a->m, a->n, a->ldp, 4),
                         extent("x", a->dw ? a->x : nullptr, a->m, a->k, a->ldx, size),
-                        a->dx ? weights_extent(a->w, a->k, a->n, a->w_sk, a->w_sn, size) : Extent{"w", 0, 0},
+                        a->dx ? weights_extent(a->w, a->k, a->n, a->w_sk, a->w_sn, size) : Extent{"w", 0, 0, 0, 0, 0},
                         extent("dx_add", in_place || !a->dx ? nullptr : a->dx_add, a->m, a->k, a->ldadd, size)};
     return check_apart(e, 4, 9);
 }

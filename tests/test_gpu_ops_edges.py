@@ -38,7 +38,7 @@ def half(t):
 
 
 def act64(z, name):
-    return {"linear": lambda: z, "relu": lambda: z.clamp(min=0), "elu": lambda: torch.where(z > 0, z, torch.expm1(z)),
+    return {"linear": lambda: z, "relu": lambda: torch.relu(z), "elu": lambda: torch.where(z > 0, z, torch.expm1(z)),
             "sigmoid": lambda: torch.sigmoid(z), "tanh": lambda: torch.tanh(z), "silu": lambda: z * torch.sigmoid(z),
             "gelu": lambda: z * torch.erfc(-z / math.sqrt(2)) / 2}[name]()
 
@@ -232,3 +232,25 @@ def test_g_itself(m, k, n, dtype):
             if not alone:
                 want = ops.dense_backward(dy, x, w, z, act)
                 assert all(torch.equal(p, q) for p, q in zip((dx, dw, db), want))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,k,n", [(1, 30, 20), (4, 70, 33), (40, 128, 64), (300, 130, 200), (700, 256, 512)])
+def test_operands_that_are_columns_of_one_buffer(m, k, n, dtype):
+    """x, the residual, y and dy side by side in one buffer; w and dw's source likewise: nothing beside an output is written."""
+    buf = whole(m, k + 3 * n + 5, dtype=dtype, seed=1)
+    x, r, y, dy = buf[:, 1:1 + k], buf[:, 1 + k:1 + k + n], buf[:, 1 + k + n:1 + k + 2 * n], buf[:, 3 + k + 2 * n:3 + k + 3 * n]
+    both = whole(k, 2 * n, dtype=dtype, seed=2)
+    w, z = both[:, :n], torch.empty(m, 2 * n, device="cuda")
+    before, want = buf.clone(), (f64(x) @ f64(w)).clamp(min=0) + f64(r)
+    assert ops.dense(x, w, activation="relu", residual=r, pre=z[:, n:], out=y).data_ptr() == y.data_ptr()
+    assert torch.equal(y, want.to(dtype)) and torch.equal(z[:, n:].double(), f64(x) @ f64(w))
+    before[:, 1 + k + n:1 + k + 2 * n] = y
+    assert torch.equal(buf, before)
+    for name, a, b in zip(("dx", "dw", "db"), ops.dense_backward(dy, x, w, z[:, n:], "relu"), grads64(dy, x, w, z[:, n:], "relu")):
+        assert torch.equal(a, b.to(dtype)), name
+    if m > 1:
+        with pytest.raises(ValueError, match="overlaps"):
+            ops.dense(x, w, out=buf[:, k:k + n])  # x's last column
+        with pytest.raises(ValueError, match="overlaps"):
+            ops.dense(x, w, out=buf.view(-1)[k + 1:k + 1 + m * n].view(m, n))  # rows of another length

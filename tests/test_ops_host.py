@@ -129,3 +129,25 @@ def test_many_tensor_refusals():
                dict(p=table((4096, 8, 0, 4)), m=table((4096 + 16, 8, 0, 4)), v=table((4096 + 16, 8, 0, 4)))):
         assert adam(**kw) < 0, kw
     assert L.pvae_adam_step(p, g, m, v, 0, *good, None, None, 0, None) == 0  # no tensors: nothing to do
+
+
+K = 100_000  # a contraction that is split: an accepted call asks for a workspace, a refused one for none
+X, W, Y = 1 << 30, 1 << 31, 1 << 32
+
+
+@pytest.mark.parametrize("kw,ok", [
+    (dict(), True), (dict(y=X + 4 * K, ldy=K + 8), True), (dict(y=X + 4 * K - 4, ldy=K + 8), False), (dict(y=X + 4 * K + 4, ldy=K + 8), False),
+    (dict(y=X - 32, ldy=K + 8), True), (dict(y=X - 28, ldy=K + 8), False), (dict(y=X + 4 * K, ldy=K + 9), False),
+    (dict(y=X + 4 * (2 * K + 8), ldy=K + 8), True), (dict(m=1, y=X + 4 * K, ldy=8), True), (dict(m=1, y=X + 4 * K - 4, ldy=8), False),
+    (dict(w_sk=20, y=W + 32, ldy=20), True), (dict(w_sk=20, y=W + 28, ldy=20), False), (dict(w_sk=20, y=W + 52, ldy=20), False),
+    (dict(w_sk=1, w_sn=K + 8, y=W + 4 * K, ldy=K + 8), True), (dict(w_sk=1, w_sn=K + 8, y=W + 4 * K - 4, ldy=K + 8), False),
+    (dict(ldy=16, pre=Y + 32, ldp=16), True), (dict(ldy=16, pre=Y + 28, ldp=16), False), (dict(ldy=16, pre=Y + 32, ldp=15), False),
+    (dict(ldy=16, bias=Y + 32), True), (dict(ldy=16, bias=Y + 28), False), (dict(ldy=16, bias=Y + 36), False),
+    (dict(ldy=16, residual=Y + 32, ldr=0), True), (dict(ldy=16, residual=Y + 28, ldr=0), False), (dict(ldy=16, residual=Y, ldr=16), True),
+    (dict(ldy=16, residual=Y, ldr=0), False)])
+def test_columns_of_one_buffer_are_apart(kw, ok):
+    """An output may lie between the rows of an operand, at the byte."""
+    a = dense_args(**dict(dict(m=2, k=K, n=8, x=X, ldx=K + 8, w=W, w_sk=8, y=Y, ldy=8), **kw))
+    assert (ops.lib().pvae_dense_workspace(C.byref(a)) > 0) == ok
+    if not ok:
+        assert "overlaps" in ops.lib().pvae_ops_last_error().decode()
