@@ -54,7 +54,7 @@ int pvae_dense(const pvae_dense_args* a, void* workspace, int64_t workspace_byte
 
 /* The gradients of pvae_dense: g = dy * f'(pre); dx = g w^T (+ dx_add); dw = x^T g; dbias = column sums of g.  The
  * residual's gradient is dy itself.
- * dy [m][n]; pre [m][n] float32 (NULL with PVAE_LINEAR); dx [m][k], dw [k][n] contiguous, dbias [n]: each may be NULL.
+ * dy [m][n] (lddy 0: one row for all); pre [m][n] float32 (NULL with PVAE_LINEAR); dx [m][k], dw [k][n] contiguous, dbias [n]: each may be NULL.
  * dx_add [m][k] with row stride ldadd, or NULL: added to dx before its one rounding (a layer whose residual is its own
  * input passes dy; dx may be dx_add itself).  dpre [m][n] float32 contiguous, or NULL: receives g.
  * g of a 16-bit type enters the products in two terms of the type (bf16: 16 bits of g; float16: 22 bits, to 2^-35 at worst, and

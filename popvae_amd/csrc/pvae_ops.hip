@@ -512,7 +512,7 @@ int check_dense_bwd(const pvae_dense_bwd_args* a) {
     if (!a) return refuse(-1, "no arguments");
     if (int rc = check_sizes(a->dtype, a->act, a->m, a->k, a->n)) return rc;
     const int size = esize(a->dtype);
-    if (int rc = check_matrix("dy", a->dy, a->m, a->n, a->lddy, size)) return rc;
+    if (int rc = check_matrix("dy", a->dy, a->lddy == 0 ? 1 : a->m, a->n, a->lddy, size)) return rc;
     if (a->act != PVAE_LINEAR)
         if (int rc = check_matrix("pre", a->pre, a->m, a->n, a->ldp, 4)) return rc;
     if (a->dw)

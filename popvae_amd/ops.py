@@ -179,7 +179,7 @@ def dense(x, w, bias=None, activation="linear", residual=None, pre=None, out=Non
 def dense_backward(dy, x, w, pre=None, activation="linear", dx_add=None, need_dx=True, need_dw=True, need_bias=True):
     """Gradients of ``dense``: ``(dx, dw, db)``, with None for what is not needed.
 
-    dy [m, n]; x, w and activation as in the forward, pre what it left (not needed for "linear").  dx_add [m, k] is added to
+    dy [m, n] (an expanded row is fine); x, w and activation as in the forward, pre what it left (not needed for "linear").  dx_add [m, k] is added to
     dx before its rounding: a layer whose residual is its own input passes dy.  (The gradient of the residual is dy itself;
     summed over the rows for an expanded one.)  dx, dw and db are rounded to their type once, at their end."""
     dtype, device, m, k, n, ldx = _layer(x, w)
@@ -187,7 +187,7 @@ def dense_backward(dy, x, w, pre=None, activation="linear", dx_add=None, need_dx
         with torch.cuda.device(device):
             return dense_backward(dy, x, w, pre, activation, dx_add, need_dx, need_dw, need_bias)
     act = _act(activation)
-    lddy = _matrix("dy", dy, m, n, dtype, device)
+    lddy = _matrix("dy", dy, m, n, dtype, device, expand=True)
     zp = ldp = ap = ldadd = 0
     if pre is not None:
         ldp, zp = _matrix("pre", pre, m, n, torch.float32, device), pre.data_ptr()

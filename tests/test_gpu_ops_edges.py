@@ -254,3 +254,13 @@ def test_operands_that_are_columns_of_one_buffer(m, k, n, dtype):
             ops.dense(x, w, out=buf[:, k:k + n])  # x's last column
         with pytest.raises(ValueError, match="overlaps"):
             ops.dense(x, w, out=buf.view(-1)[k + 1:k + 1 + m * n].view(m, n))  # rows of another length
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,k,n", [(2, 5, 1), (40, 30, 50), (300, 70, 1), (700, 256, 300)])
+def test_an_expanded_row_as_dy(m, k, n, dtype):
+    x, w, z = whole(m, k, dtype=dtype, seed=1), whole(k, n, dtype=dtype, seed=2), rnd(m, n, seed=3)
+    dy = whole(1, n, dtype=dtype, seed=4).expand(m, n)
+    check_exact(x, w, dy, z, dtype)
+    for a, b in zip(ops.dense_backward(dy, x, w, z, "gelu"), ops.dense_backward(dy.contiguous(), x, w, z, "gelu")):
+        assert torch.equal(a, b)
