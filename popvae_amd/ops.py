@@ -4,8 +4,9 @@ residual in one pass, its gradients, the global gradient norm, clipping by it, a
 They are what the engine's layers and optimizer do, for tensors that do not live in an ``Engine``: any size, float32, bfloat16
 or float16, other activations.  Everything runs on torch's current stream of the tensors' device, allocates through torch's
 allocator (outputs and scratch memory), never waits for the GPU and may be captured into a graph.  A call that cannot be
-computed raises ValueError before anything is launched.  There is no CPU path, and autograd records nothing here:
-gradients are calls of their own.
+computed raises ValueError before anything is launched.  There is no CPU path.  Autograd records nothing here, gradients are
+calls of their own: where grad mode is on, ``dense`` and ``dense_backward`` refuse tensors that require a gradient (call them
+under ``torch.no_grad()``).
 
     y = ops.dense(x, w, b, "elu", residual=x, pre=z)               # z: float32, kept for the backward
     dx, dw, db = ops.dense_backward(dy, x, w, z, "elu", dx_add=dy)  # dx_add: the layer's residual was its own input
@@ -125,6 +126,17 @@ def _layer(x, w):
     return dtype, device, m, k, w.shape[1], _matrix("x", x, m, k, dtype, device)
 
 
+_recording = torch.is_grad_enabled
+
+
+def _no_history(*tensors):
+    """Where autograd would record, a result without history would pass for one that depends on nothing."""
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            raise ValueError("a tensor requires a gradient, and autograd records nothing here: call under torch.no_grad() and "
+                             "take the gradients from dense_backward")
+
+
 def _stream(device):
     """torch's current stream of a device as a hipStream_t."""
     return torch.cuda.current_stream(device).cuda_stream
@@ -157,6 +169,8 @@ def dense(x, w, bias=None, activation="linear", residual=None, pre=None, out=Non
     if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):
             return dense(x, w, bias, activation, residual, pre, out)
+    if _recording():
+        _no_history(x, w, bias, residual, pre, out)
     bp = rp = zp = ldr = ldp = 0
     if bias is not None:
         _vector("bias", bias, n, dtype, device)
@@ -186,6 +200,8 @@ def dense_backward(dy, x, w, pre=None, activation="linear", dx_add=None, need_dx
     if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):
             return dense_backward(dy, x, w, pre, activation, dx_add, need_dx, need_dw, need_bias)
+    if _recording():
+        _no_history(dy, x, w, pre, dx_add)
     act = _act(activation)
     lddy = _matrix("dy", dy, m, n, dtype, device, expand=True)
     zp = ldp = ap = ldadd = 0

@@ -264,3 +264,27 @@ def test_an_expanded_row_as_dy(m, k, n, dtype):
     check_exact(x, w, dy, z, dtype)
     for a, b in zip(ops.dense_backward(dy, x, w, z, "gelu"), ops.dense_backward(dy.contiguous(), x, w, z, "gelu")):
         assert torch.equal(a, b)
+
+
+def test_autograd_is_not_left_in_the_dark():
+    """A tensor that requires a gradient is refused where autograd would record; without recording the same call runs."""
+    x, w, b, r, z, dy = rnd(5, 6, seed=1), rnd(6, 4, seed=2), rnd(4, seed=3), rnd(5, 4, seed=4), rnd(5, 4, seed=5), rnd(5, 4, seed=6)
+    y = ops.dense(x, w, b, "elu", residual=r)
+    for t in (x, w, b, r):
+        t.requires_grad_(True)
+        with pytest.raises(ValueError, match="no_grad"):
+            ops.dense(x, w, b, "elu", residual=r)
+        with torch.no_grad():
+            assert torch.equal(ops.dense(x, w, b, "elu", residual=r), y)
+        t.requires_grad_(False)
+    for t in (x, w, dy, z):
+        t.requires_grad_(True)
+        with pytest.raises(ValueError, match="no_grad"):
+            ops.dense_backward(dy, x, w, z, "elu")
+        with torch.inference_mode():
+            ops.dense_backward(dy, x, w, z, "elu")
+        t.requires_grad_(False)
+    # parameters that require a gradient are what an optimizer updates
+    p = [w.clone().requires_grad_(True)]
+    ops.adam_step(p, [rnd(6, 4, seed=7)], [torch.zeros_like(w)], [torch.zeros_like(w)], 1)
+    assert p[0].requires_grad and not torch.equal(p[0].detach(), w)
