@@ -6,7 +6,7 @@ or float16, other activations.  Everything runs on torch's current stream of the
 allocator (outputs and scratch memory), never waits for the GPU and may be captured into a graph.  A call that cannot be
 computed raises ValueError before anything is launched.  There is no CPU path.  Autograd records nothing here, gradients are
 calls of their own: where grad mode is on, ``dense`` and ``dense_backward`` refuse tensors that require a gradient (call them
-under ``torch.no_grad()``).
+under ``torch.no_grad()``).  What is written in place counts as changed for what autograd has saved.
 
     y = ops.dense(x, w, b, "elu", residual=x, pre=z)               # z: float32, kept for the backward
     dx, dw, db = ops.dense_backward(dy, x, w, z, "elu", dx_add=dy)  # dx_add: the layer's residual was its own input
@@ -137,6 +137,9 @@ def _no_history(*tensors):
                              "take the gradients from dense_backward")
 
 
+_changed = torch.autograd.graph.increment_version  # of some tensors: a later backward refuses those that it has saved
+
+
 def _stream(device):
     """torch's current stream of a device as a hipStream_t."""
     return torch.cuda.current_stream(device).cuda_stream
@@ -175,18 +178,23 @@ def dense(x, w, bias=None, activation="linear", residual=None, pre=None, out=Non
     if bias is not None:
         _vector("bias", bias, n, dtype, device)
         bp = bias.data_ptr()
+    changed = []
     if residual is not None:
         ldr, rp = _matrix("residual", residual, m, n, dtype, device, expand=True), residual.data_ptr()
     if pre is not None:
         ldp, zp = _matrix("pre", pre, m, n, torch.float32, device), pre.data_ptr()
+        changed.append(pre)
     if out is None:
         out, ldy = torch.empty((m, n), dtype=dtype, device=device), n
     else:
         ldy = _matrix("out", out, m, n, dtype, device)
+        changed.append(out)
     sk, sn = w.stride()
     L = _lib or lib()
     _call(L.pvae_dense, _pack_dense(DTYPES[dtype], _act(activation), m, k, n, x.data_ptr(), ldx, w.data_ptr(), sk, sn, bp, rp, ldr,
                                     out.data_ptr(), ldy, zp, ldp), L.pvae_dense_workspace, device)
+    if changed:
+        _changed(changed)
     return out
 
 
@@ -302,6 +310,7 @@ def clip_by_global_norm(tensors, max_norm, out=None):
     into = table if o is s else o._same()
     norm, work, need = _scratch(device)
     _check(_lib.pvae_clip_by_global_norm(table, into, len(s), float(max_norm), norm.data_ptr(), work.data_ptr(), need, _stream(device)))
+    _changed(o.tensors)
     return norm
 
 
@@ -331,4 +340,6 @@ def adam_step(params, grads, m, v, step, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e
         norm, work, need = _scratch(device)
     _check(L.pvae_adam_step(p._same(), g._same(), m._same(), v._same(), len(p), lr, beta1, beta2, eps, int(step), at,
                             float(clip_norm or 0.0), _ptr(norm), _ptr(work), need, _stream(device)))
+    for written in (p, m, v):
+        _changed(written.tensors)
     return norm

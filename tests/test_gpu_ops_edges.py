@@ -288,3 +288,29 @@ def test_autograd_is_not_left_in_the_dark():
     p = [w.clone().requires_grad_(True)]
     ops.adam_step(p, [rnd(6, 4, seed=7)], [torch.zeros_like(w)], [torch.zeros_like(w)], 1)
     assert p[0].requires_grad and not torch.equal(p[0].detach(), w)
+
+
+def test_what_is_written_in_place_counts_as_changed():
+    """A tensor that autograd has saved and an operator overwrites makes the backward fail, as torch's own in-place operations do."""
+    x, w, g = rnd(5, 6, seed=1), rnd(6, 6, seed=2), rnd(5, 6, seed=3)
+    m, v = torch.zeros_like(g), torch.zeros_like(g)
+
+    def writes():
+        yield "out", lambda t: ops.dense(x, w, out=t)
+        yield "pre", lambda t: ops.dense(x, w, pre=t)
+        yield "clip in place", lambda t: ops.clip_by_global_norm([t], 0.1)
+        yield "clip into", lambda t: ops.clip_by_global_norm([g], 0.1, out=[t])
+        yield "parameters", lambda t: ops.adam_step([t], [g], [m], [v], 1)
+        yield "first moment", lambda t: ops.adam_step([m], [g], [t], [v], 1)
+        yield "second moment", lambda t: ops.adam_step([m], [g], [v], [t], 1)
+
+    for name, write in writes():
+        a, saved = rnd(5, 6, seed=4).requires_grad_(True), rnd(5, 6, seed=5).abs()
+        loss = (a * saved).sum()  # saves `saved`
+        write(saved)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+            raise AssertionError(name)
+        loss = (a * saved).sum()
+        loss.backward()
+        assert torch.equal(a.grad, saved), name
