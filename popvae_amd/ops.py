@@ -238,11 +238,15 @@ def _ptr(t):
 
 class TensorSet:
     """A list of contiguous tensors on one GPU, checked and described once: what the operators over all tensors of a model take
-    (a plain list works too, and is described anew by every call).  The tensors must keep their storage: a set one of
-    whose tensors has moved is refused."""
+    (a plain list works too, and is described anew by every call).  The tensors must keep their storage, which the set holds on
+    to: a set one of whose tensors has moved is refused."""
 
     def __init__(self, tensors):
-        ts = list(tensors)
+        self._describe(list(tensors))
+        # while the set lives nothing else is allocated where its tensors are, whatever becomes of them
+        self._storages = [t.detach() for t in self.tensors]
+
+    def _describe(self, ts):
         self.device = ts[0].device if ts else None
         for i, t in enumerate(ts):
             if t.dtype not in DTYPES:
@@ -267,7 +271,11 @@ class TensorSet:
 
 
 def _set(t):
-    return t if isinstance(t, TensorSet) else TensorSet(t)
+    if isinstance(t, TensorSet):
+        return t
+    s = TensorSet.__new__(TensorSet)  # for one call
+    s._describe(list(t))
+    return s
 
 
 def _device_of(s):

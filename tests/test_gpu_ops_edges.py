@@ -314,3 +314,17 @@ def test_what_is_written_in_place_counts_as_changed():
         loss = (a * saved).sum()
         loss.backward()
         assert torch.equal(a.grad, saved), name
+
+
+def test_a_set_keeps_the_storage_that_it_describes():
+    """A tensor of the set that lets go of its storage and later gets another of fewer elements: the allocator may hand out the
+    same address again, so the set holds on to the storage and refuses the tensor."""
+    t = rnd(1000, seed=1)
+    s, at = ops.TensorSet([t]), t.data_ptr()
+    t.data = torch.empty(0, device="cuda")
+    others = [torch.zeros(990, device="cuda") for _ in range(64)]
+    assert at not in [o.data_ptr() for o in others]
+    for o in others:
+        t.data = o
+        with pytest.raises(ValueError, match="storage"):
+            ops.global_norm(s)
