@@ -86,8 +86,8 @@ int pvae_set_bce_mode(pvae_engine* e, int mode);
 int pvae_set_clip_norm(pvae_engine* e, float clip_norm);
 int pvae_get_grad_norm(pvae_engine* e, float* norm);
 /* No counterpart in the reference: hidden layers of equal width as residual layers, h = elu(h W + b) + h (encoder layers
- * 2 .. depth, decoder layers 2 .. depth; the first layer of each side and the heads stay as they are).  Same tensors, same
- * weight files; runs layer by layer (pvae_dense, pvae_dense_bwd), 32 rows per device pass.  0 returns to plain layers. */
+ * 2 .. depth, decoder layers 2 .. depth; the first layer of each side and the heads stay as they are).  Same tensors
+ * (which kind of model they belong to is for their file to say); runs layer by layer (pvae_dense, pvae_dense_bwd), 32 rows per device pass.  0 returns to plain layers. */
 int pvae_set_residual(pvae_engine* e, int on);
 
 /* one train_step of vae.fit (popvae.py:490): rows = sample indices into the resident matrix (n <= batch_size),

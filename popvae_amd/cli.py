@@ -246,7 +246,11 @@ def main(argv=None):
     if args.init_weights:  # vae.load_weights before fit (per-step parity from a Keras export)
         from .weights_io import load_weights_file
         log("initialising from " + args.init_weights)
-        eng.set_weights(load_weights_file(args.init_weights))
+        try:
+            init = load_weights_file(args.init_weights, residual=args.residual)
+        except ValueError as ex:
+            raise SystemExit(f"--init_weights: {ex}") from ex
+        eng.set_weights(init)
 
     t1 = time.time()
     history, cbs = F.fit(eng, train, test, max_epochs=args.max_epochs, patience=args.patience,
@@ -268,7 +272,7 @@ def main(argv=None):
         F.write_latent_coords(args.out + "_latent_coords.txt", pred, samples, args.latent_dim)
         if args.save_weights and full_weights is not None:  # popvae.py:429-435, 525-526: the best epoch's weights stay on disk
             from .weights_io import save_weights_hdf5
-            log("weights saved to " + save_weights_hdf5(args.out + "_weights.hdf5", full_weights, depth))
+            log("weights saved to " + save_weights_hdf5(args.out + "_weights.hdf5", full_weights, depth, residual=args.residual))
         try:
             F.plot_history(args.out + "_history.pdf", history)
         except Exception as ex:  # matplotlib absent or headless failure: the reference's pdf is cosmetic

@@ -9,6 +9,9 @@
   its Dense layers, so Keras numbers them in creation order: encoder hidden layers, z_mean, z_log_var, decoder layers,
   output layer), stored as datasets under that group.  Optimizer slots are not written (the reference never reads them).
 * ``<out>_weights.npz`` -- the same tensors as arrays ``t000, t001, ...`` (get_weights() order) plus ``names``.
+* A model with residual hidden layers (``--residual``, ``Engine.set_residual``) has the same tensors as a plain one, and its
+  file says so: a root attribute ``popvae_amd_residual`` (an array ``residual`` in .npz) that Keras does not look at.  Such a file
+  is loaded only by a caller that asks for a residual model.
 * ``<infile>.popvae.hdf5`` -- datasets ``derived_counts`` (float64 [N, L], values 0 / 0.5 / 1) and ``samples``
   (variable-length UTF-8 strings), popvae.py:205-209, 241-248.
 
@@ -32,12 +35,13 @@ def keras_weight_names(depth):
     return enc, dec
 
 
-def save_weights_hdf5(path, weights, depth):
-    """``weights``: list in ``vae.get_weights()`` order (``Engine.get_weights()``), float32."""
+def save_weights_hdf5(path, weights, depth, residual=False):
+    """``weights``: list in ``vae.get_weights()`` order (``Engine.get_weights()``), float32.  residual: of a model with residual
+    hidden layers."""
     enc, dec = keras_weight_names(depth)
     if len(weights) != len(enc) + len(dec):
         raise ValueError(f"depth {depth} has {len(enc) + len(dec)} tensors, got {len(weights)}")
-    root = h5lite.Group(attrs={"keras_version": b"2.15.0", "backend": b"tensorflow"})
+    root = h5lite.Group(attrs={"keras_version": b"2.15.0", "backend": b"tensorflow", **({"popvae_amd_residual": b"1"} if residual else {})})
     mw = root.group("model_weights", attrs={"layer_names": np.array([b"input_1", b"encoder", b"decoder"]),
                                             "backend": b"tensorflow", "keras_version": b"2.15.0"})
     mw.group("input_1", attrs={"weight_names": np.array([], dtype="S1")})
@@ -51,9 +55,10 @@ def save_weights_hdf5(path, weights, depth):
     return path
 
 
-def save_weights_npz(path, weights, depth):
+def save_weights_npz(path, weights, depth, residual=False):
     enc, dec = keras_weight_names(depth)
-    np.savez(path, names=np.array(enc + dec), **{f"t{i:03d}": np.asarray(w, np.float32) for i, w in enumerate(weights)})
+    np.savez(path, names=np.array(enc + dec), **({"residual": np.array(True)} if residual else {}),
+             **{f"t{i:03d}": np.asarray(w, np.float32) for i, w in enumerate(weights)})
     return path
 
 
@@ -61,14 +66,21 @@ def _names(a):
     return [x.decode() if isinstance(x, bytes) else str(x) for x in np.asarray(a).reshape(-1)]
 
 
-def load_weights_file(path):
+def load_weights_file(path, residual=False):
     """``vae.load_weights(path)`` without Keras: the tensors of a Keras HDF5 weight / full-model file, or of an ``.npz``
-    written by ``save_weights_npz``, as a list in ``get_weights()`` order -- ready for ``Engine.set_weights``."""
+    written by ``save_weights_npz``, as a list in ``get_weights()`` order -- ready for ``Engine.set_weights``.  The file of a
+    residual model needs ``residual=True``, and an engine with ``set_residual()``: in plain layers its weights are another model."""
+    def check(is_residual):
+        if is_residual and not residual:
+            raise ValueError(f"{path}: the weights of a model with residual hidden layers (--residual, Engine.set_residual)")
+
     if str(path).endswith(".npz"):
         with np.load(path, allow_pickle=False) as z:
+            check("residual" in z.files and bool(z["residual"]))
             keys = sorted(k for k in z.files if k.startswith("t") and k[1:].isdigit())
             return [np.array(z[k], dtype=np.float32) for k in keys]
     root = h5lite.read(path)
+    check("popvae_amd_residual" in root.attrs)
     top = root["model_weights"] if "model_weights" in root else root  # model.save(...) vs model.save_weights(...)
     if "layer_names" not in top.attrs:
         raise ValueError(f"{path}: no `layer_names` attribute -- not a Keras weight file")

@@ -224,3 +224,20 @@ def test_command_line(tmp_path):
     p = subprocess.run([sys.executable, os.path.join(root, "popvae.py"), "--infile", vcf, "--out", out, "--clip_norm", "-1"],
                        capture_output=True, text=True, timeout=100)
     assert p.returncode != 0 and "clip_norm" in p.stderr
+
+
+def test_weights_of_a_residual_model_on_the_command_line(tmp_path):
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    vcf = os.path.join(root, "tests", "golden", "pabu_test_genotypes.vcf.gz")
+    out = str(tmp_path / "run")
+
+    def run(*more):
+        return subprocess.run([sys.executable, os.path.join(root, "popvae.py"), "--infile", vcf, "--out", out, "--seed", "1", "--max_epochs", "2",
+                               "--depth", "3", *more], capture_output=True, text=True, timeout=100)
+
+    p = run("--residual", "--save_weights")
+    assert p.returncode == 0, p.stderr[-2000:]
+    p = run("--init_weights", out + "_weights.hdf5")
+    assert p.returncode != 0 and "residual" in p.stderr
+    p = run("--init_weights", out + "_weights.hdf5", "--residual")
+    assert p.returncode == 0, p.stderr[-2000:]

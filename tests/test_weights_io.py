@@ -122,3 +122,22 @@ def test_weight_file_with_extra_top_level_layers(tmp_path):
     h5lite.write(p3, root)
     with pytest.raises(ValueError, match="4 \\* depth \\+ 6"):
         weights_io.load_weights_file(p3)
+
+
+def test_a_residual_model_says_so_in_its_file(tmp_path):
+    """The tensors are those of a plain model: a file of a residual one is not taken for it."""
+    g = np.random.default_rng(5)
+    depth, L, W, K = 3, 40, 8, 2
+    shapes = [(L, W), (W,)] + [(W, W), (W,)] * (depth - 1) + [(W, K), (K,)] * 2 + [(K, W), (W,)] + [(W, W), (W,)] * (depth - 1) + [(W, L), (L,)]
+    w = [g.normal(size=s).astype(np.float32) for s in shapes]
+    for ext, save in ((".hdf5", weights_io.save_weights_hdf5), (".npz", weights_io.save_weights_npz)):
+        plain, res = (save(str(tmp_path / (name + ext)), w, depth, residual=r) for name, r in (("plain", False), ("res", True)))
+        with pytest.raises(ValueError, match="residual"):
+            weights_io.load_weights_file(res)
+        # a residual model may start from any weights of its shape
+        for path, residual in ((plain, False), (plain, True), (res, True)):
+            got = weights_io.load_weights_file(path, residual=residual)
+            assert len(got) == len(w) and all(np.array_equal(a, b) for a, b in zip(got, w))
+        if ext == ".hdf5":  # nothing but the attribute differs, and a plain file is what it was
+            a, b = h5lite.read(plain), h5lite.read(res)
+            assert "popvae_amd_residual" not in a.attrs and set(b.attrs) - set(a.attrs) == {"popvae_amd_residual"}
