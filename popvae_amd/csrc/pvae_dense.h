@@ -89,10 +89,11 @@ __device__ __forceinline__ float pvd_act_grad(float z, int act) { return pvd_act
 
 // ---------------------------------------------------------------------------------------------
 // g = dy f'(pre) of a 16-bit type enters the products in two terms, so that a gradient is rounded once, at its end, and fits
-// wherever its value does: g = UNIT (hi + LOW lo).  bf16: sixteen bits of g.  float16: UNIT keeps g of the largest dy and f'
-// below the type's largest value, LOW the second term of the smallest g above its least: 22 bits of g, to 2^-35 at worst.  hi is 0
-// only where g is, and infinite or NaN only where g is (lo is 0 there): what an infinite x or w makes of a gradient is in the
-// first terms' sums, and a second terms' sum that is not finite (0 times infinity, infinities of both signs) is dropped.
+// wherever its value does: g = UNIT (hi + LOW lo).  bf16: hi is cut off, not rounded, so that it is finite where g is; sixteen
+// bits of g in all.  float16: UNIT keeps g of the largest dy and f' below the type's largest value, LOW the second term of the
+// smallest g above its least: 22 bits of g, to 2^-35 at worst; hi is 0 only where g is.  What an infinite x or w makes of a
+// gradient is in the first terms' sums, and so is a g that is infinite or NaN: a second terms' sum that is not finite (0 times
+// infinity, infinities of both signs) is dropped.
 // One rounding of g to the type would save half of the matrix work and leave a gradient off by as much again as its own
 // rounding (4096 x 2048 x 4096 bf16 with GELU: 0.0024 relative to 64 bits instead of 0.0017).
 // ---------------------------------------------------------------------------------------------
@@ -100,15 +101,15 @@ template <int DT> struct PvdTerms { static constexpr float UNIT = 1.f, LOW = 1.f
 template <> struct PvdTerms<PVD_F16> { static constexpr float UNIT = 2.f, LOW = 1.f / 2048.f; };
 template <int DT> __device__ __forceinline__ void pvd_terms(float g, typename PvdType<DT>::T& hi, typename PvdType<DT>::T& lo) {
     static_assert(DT != PVD_F32, "float32 products take g as it is");
-    const float s = g * (1.f / PvdTerms<DT>::UNIT);
-    hi = pvd_from_f32<DT>(s);
     if constexpr (DT == PVD_BF16) {
-        if ((hi & 0x7fffu) == 0x7f80u && fabsf(s) < __builtin_inff()) hi -= 1;  // the largest value: lo takes the rest
+        hi = (unsigned short)(__float_as_uint(g) >> 16);  // a product's NaN is quiet: its bit stays
+        lo = __builtin_bit_cast(unsigned short, (__bf16)(g - pvm_bf16(hi)));
     } else {
+        const float s = g * (1.f / PvdTerms<DT>::UNIT);
+        hi = pvd_from_f32<DT>(s);
         if ((hi & 0x7fffu) == 0 && s != 0.f) hi |= 1;  // the least value, s's sign: lo takes it back
+        lo = pvd_from_f32<DT>((s - pvd_to_f32<DT>(hi)) * (1.f / PvdTerms<DT>::LOW));
     }
-    const float rest = (s - pvd_to_f32<DT>(hi)) * (1.f / PvdTerms<DT>::LOW);
-    lo = pvd_from_f32<DT>(fabsf(s) < __builtin_inff() ? rest : 0.f);
 }
 
 // ---------------------------------------------------------------------------------------------

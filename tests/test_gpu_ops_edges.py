@@ -123,12 +123,13 @@ def test_infinities_in_the_gradients_operands(m, k, n, act, dtype):
 
 
 def check_gradients_rounded_once(dy, x, w, z, act, dtype):
-    """dx and dw are off by what f' (16 u (1 + |z|)), g's two terms (bf16: 2^-17 of g; f16: 2^-21 and 2^-35; float32: u) and
+    """dx and dw are off by what f' (16 u (1 + |z|)), g's two terms (bf16: 2^-16 of g -- what cutting the first
+    off leaves is below 2^-7 of g, and the second is off by 2^-9 of that; f16: 2^-21 and 2^-35; float32: u) and
     float32 sums (u a term) are off by, and one rounding of the result: a rounding of g to a 16-bit type is not in it."""
     dx, dw, _ = ops.dense_backward(dy, x, w, z, act)
     X, W, DY, Z = f64(x), f64(w), f64(dy), f64(z)
     G = DY * dact64(Z, act)
-    rel, least = {F32: (2 * U, 0.0), BF16: (2.0 ** -17, 0.0), F16: (2.0 ** -21, 2.0 ** -35)}[dtype]
+    rel, least = {F32: (2 * U, 0.0), BF16: (2.0 ** -16, 0.0), F16: (2.0 ** -21, 2.0 ** -35)}[dtype]
     eg = 16 * U * (1 + Z.abs()) * DY.abs() + rel * G.abs() + least
     h, tiny = half(dtype)
     for what, got, want, e, terms, size in (
