@@ -128,8 +128,8 @@ def main(argv=None):
         raise SystemExit(0)
     if args.infile is None:
         raise SystemExit("--infile is required")
-    if args.clip_norm is not None and not args.clip_norm > 0:
-        raise SystemExit("--clip_norm: a positive number")
+    if args.clip_norm is not None and not np.float32(args.clip_norm) > 0:
+        raise SystemExit("--clip_norm: a positive number (in float32)")
     if args.clip_norm is not None and int(os.environ.get("WORLD_SIZE", "1")) > 1:
         raise SystemExit("--clip_norm: not with the SNP axis sharded over several GPUs (the norm spans all shards)")
 

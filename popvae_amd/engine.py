@@ -226,7 +226,10 @@ class Engine:
     def set_clip_norm(self, clip_norm):
         """Keras' ``Adam(global_clipnorm=...)``: train steps scale all gradients by ``min(1, clip_norm / norm)`` first; None or
         0: off.  One GPU per model only."""
-        self._ck(lib().pvae_set_clip_norm(self._h, 0.0 if clip_norm is None else float(clip_norm)))
+        c = 0.0 if clip_norm is None else float(clip_norm)
+        if c > 0 and np.float32(c) == 0:  # would turn clipping off
+            raise RuntimeError(f"clip_norm {c:g}: below the least float32")
+        self._ck(lib().pvae_set_clip_norm(self._h, c))
 
     @property
     def grad_norm(self):

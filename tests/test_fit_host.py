@@ -194,3 +194,10 @@ def test_test_flag_resolves_its_input(tmp_path, monkeypatch):
     os.makedirs(tmp_path / "data" / "pabu")
     (tmp_path / "data" / "pabu" / "pabu_test_genotypes.vcf").write_text("##fileformat=VCFv4.2\n")
     assert cli.test_infile() == os.path.join("data", "pabu", "pabu_test_genotypes.vcf")
+
+
+@pytest.mark.parametrize("bound", ["0", "-1", "nan", "1e-50"])
+def test_clip_norm_that_is_no_bound_is_refused_on_the_command_line(bound):
+    from popvae_amd import cli
+    with pytest.raises(SystemExit, match="clip_norm"):
+        cli.main(["--infile", "none.vcf", "--clip_norm", bound])

@@ -241,3 +241,14 @@ def test_weights_of_a_residual_model_on_the_command_line(tmp_path):
     assert p.returncode != 0 and "residual" in p.stderr
     p = run("--init_weights", out + "_weights.hdf5", "--residual")
     assert p.returncode == 0, p.stderr[-2000:]
+
+
+def test_a_bound_below_float32_is_refused_not_taken_for_off():
+    new, _, _ = make(300, 32, 2, 2, 32)
+    e = new()
+    with pytest.raises(RuntimeError, match="clip_norm"):
+        e.set_clip_norm(1e-50)
+    e.set_clip_norm(1e-40)  # a subnormal bound is one
+    e.train_step(np.arange(8, dtype=np.int32))
+    assert e.grad_norm > 0
+    e.close()
