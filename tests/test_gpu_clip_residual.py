@@ -252,3 +252,16 @@ def test_a_bound_below_float32_is_refused_not_taken_for_off():
     e.train_step(np.arange(8, dtype=np.int32))
     assert e.grad_norm > 0
     e.close()
+
+
+def test_residual_layers_in_the_step_that_allocates_nothing():
+    new, dc, w = make(900, 128, 4, 2, 32)
+    a, b = new(), new()
+    for e in (a, b):
+        e.set_residual()
+    g = np.random.default_rng(3)
+    for n in (32, 5):
+        rows, eps = g.choice(150, n, replace=False).astype(np.int32), g.normal(size=(n, 2)).astype(np.float32)
+        assert a.train_step(rows, eps) == b.train_step_noalloc(rows, eps)
+    assert all(np.array_equal(x, y) for x, y in zip(a.get_weights(), b.get_weights()))
+    a.close(), b.close()
