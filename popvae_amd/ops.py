@@ -52,11 +52,12 @@ _pack_dense = struct.Struct("@2i3qPqP2q2PqPqPq").pack
 _pack_bwd = struct.Struct("@2i3qPqPqP2qPqPqPq3P").pack
 
 _lib = None
+_norm_workspace = 0  # bytes
 
 
 def lib():
     """libpvae.so with the operators' signatures set."""
-    global _lib
+    global _lib, _norm_workspace
     if _lib is None:
         L = engine.lib()
         vp, i32, i64, f64, tp = C.c_void_p, C.c_int32, C.c_int64, C.c_double, C.POINTER(_Tensor)
@@ -69,6 +70,7 @@ def lib():
         L.pvae_global_norm.argtypes = [tp, i64, vp, vp, i64, vp]
         L.pvae_clip_by_global_norm.argtypes = [tp, tp, i64, f64, vp, vp, i64, vp]
         L.pvae_adam_step.argtypes = [tp, tp, tp, tp, i64, f64, f64, f64, f64, i64, vp, f64, vp, vp, i64, vp]
+        _norm_workspace = L.pvae_norm_workspace()
         _lib = L
     return _lib
 
@@ -137,7 +139,8 @@ def _no_history(*tensors):
                              "take the gradients from dense_backward")
 
 
-_changed = torch.autograd.graph.increment_version  # of some tensors: a later backward refuses those that it has saved
+# of a list of tensors: a later backward refuses those that it has saved (directly: the public function looks at types first)
+_changed = getattr(torch._C, "_increment_version", torch.autograd.graph.increment_version)
 
 
 def _stream(device):
@@ -286,7 +289,8 @@ def _device_of(s):
 
 def _scratch(device):
     """The norm that a call returns and its workspace."""
-    need = lib().pvae_norm_workspace()
+    lib()
+    need = _norm_workspace
     return torch.empty((), dtype=torch.float32, device=device), torch.empty(need, dtype=torch.uint8, device=device), need
 
 
