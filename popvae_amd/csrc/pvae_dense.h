@@ -160,7 +160,7 @@ template <int DT> __device__ __forceinline__ void pvd_finish4(const PvdOut& O, i
 // 32 x 32 of it; the contraction goes through LDS 128 bytes per row at a time, the next piece on its way to registers
 // meanwhile.  float32: v_mfma_f32_16x16x4 (exact float32 products); 16-bit types: 16x16x32.  It serves what neither fills the
 // large kernel's pipeline nor fits the slim kernel -- short contractions, few rows of weights that would have to be laid out --
-// and is bound by one round trip to memory per step: 1000 x 128 x 1000 bf16 8.9 us, 64 x 4001 x 4001 bf16 28 us (1.1 TB/s).
+// and is bound by one round trip to memory per step: 1000 x 128 x 1000 bf16 7.6 us, 64 x 4001 x 4001 bf16 22 us (1.5 TB/s).
 // ---------------------------------------------------------------------------------------------
 struct PvdOperand {  // element (row, k) at p[row * sr + k * sk]; one of the strides is 1
     const void* p;
@@ -315,8 +315,8 @@ template <int DT> __global__ __launch_bounds__(256) void pvk_dense_tile(const Pv
 // The slim kernel, for few rows or results too small to give the chip 64 x 64 tiles: a workgroup of eight waves makes 32 rows
 // x 16 columns.  The waves take runs of the contraction in turn and read both operands straight from memory into the matrix
 // instruction's registers -- one round trip instead of one per LDS step, which is what such a call spends its time on --
-// and the eight partial results meet in LDS, added in order.  32 x 128 x 128 in float32: 4.3 us, nearly all of it the launch
-// and two round trips; 16 x 4096 x 4096: 28 us (w at 2.4 TB/s).
+// and the eight partial results meet in LDS, added in order.  32 x 128 x 128 in float32: 5.0 us, nearly all of it the launch
+// and two round trips; 16 x 4096 x 4096: 27 us (w at 2.5 TB/s).
 // ---------------------------------------------------------------------------------------------
 enum { PVD_SM = 32, PVD_SN = 16, PVD_SW = 8 };
 
@@ -450,7 +450,7 @@ template <int DT> __global__ __launch_bounds__(512, 4) void pvk_dense_slim(const
 // lane holds sixteen bytes of a row of w and all rows' sums of those columns in registers; x, as float32, comes from LDS.  The
 // workgroup's eight waves, and pieces of the grid, split the contraction.  Matrix instructions would compute sixteen rows for
 // one and need w transposed on the way; plain ones keep up with memory as long as rows are few.  1 x 128 x 100000 in
-// float32: 10.9 us = 4.7 TB/s; 1 x 128 x 1000000: 93 us = 5.5 TB/s, in bf16 41 us = 6.2 TB/s.
+// float32: 11.0 us = 4.7 TB/s; 1 x 128 x 1000000: 90 us = 5.8 TB/s, in bf16 39 us = 6.6 TB/s.
 // w^T (contiguous along the contraction): sixteen lanes share a column instead and add up at the end.
 // ---------------------------------------------------------------------------------------------
 struct PvdRowsJob {
@@ -633,8 +633,8 @@ template <int DT, int G> __global__ __launch_bounds__(256) void pvk_dense_join(c
 // ---------------------------------------------------------------------------------------------
 // Gradients, one launch: the first workgroups make dx (x-side operand g, contraction over n), the next dw (rows of x^T,
 // contraction over m), the last 64 columns of dbias (and dpre) each.  g = dy f'(pre) is formed anew by every workgroup on the
-// way to the matrix instructions: for small layers a second launch costs more than that.  32 x 128 x 128 in float32: 5.7 us;
-// 1 x 32 x 10589 in bf16: 15.6 us.  Bound by the round trips to memory and the launch.
+// way to the matrix instructions: for small layers a second launch costs more than that.  32 x 128 x 128 in float32: 6.0 us;
+// 1 x 32 x 10589 in bf16: 15.2 us.  Bound by the round trips to memory and the launch.
 // ---------------------------------------------------------------------------------------------
 struct PvdBwdJob {
     PvdTileJob dx, dw;
@@ -686,8 +686,8 @@ template <int DT> __global__ __launch_bounds__(512) void pvk_dense_bwd_slim(cons
 // Large products, step 1: operands that the product kernel below cannot read as they are -- rows not aligned to sixteen bytes,
 // or a contraction that is no multiple of 128 bytes -- are laid out anew, and g is formed from dy and z, once instead of once
 // per tile: a source of R rows of C contiguous elements becomes [pad(R)][pad(C)] or its transpose [C][pad(R)], zeros behind the
-// end.  One launch for up to three sources; bound by memory: dy and z of 4096 x 4096 in bf16 to g, with db's partial sums,
-// 31 us (134 MB, 4.3 TB/s); of 2504 x 512 in float32 9.5 us, most of it launch and round trip.
+// end.  One launch for up to three sources; bound by memory: dy and z of 4096 x 4096 in bf16 to both terms of g, with
+// db's partial sums, 33 us (168 MB, 5.1 TB/s); of 2504 x 512 in float32 10 us, most of it launch and round trip.
 // ---------------------------------------------------------------------------------------------
 struct PvdPack {
     const void* p;
@@ -811,12 +811,14 @@ template <int DT> __global__ __launch_bounds__(256) void pvk_dense_pack(const Pv
 // Pairs of pieces (float32: runs of four) of a line are exchanged by the line's number so that the lines which are read
 // together lie in different banks.
 // The direct loads write lane after lane, so the lanes choose their source accordingly.
-//   Measured: 4096 x 4096 x 4096 bf16 with bias, SiLU, residual and z 142 us = 970 TFLOP/s (the products alone 122 us = 1.13
-// PFLOP/s; a library product reaches 1.24 to 1.31); both gradient products of 4096 x 2048 x 4096 in one launch 145 us = 950;
-// 2504 x 128 x 100000 float32 with sigmoid 666 us = 96 TFLOP/s, 1.6 TB/s (a library product: 150 TFLOP/s; here a tile has four
-// steps only, and 1 GB of results takes a sigmoid each).  What bounds it: the path from memory to LDS moves 64 bytes a clock
-// per CU, which 128 x 128 tiles of 16-bit types use to three quarters, and the results' way out, which the CU's other
-// workgroup hides only partly.
+//   Measured (200 calls in a row; from idle a tenth more, in a long run less, as a library product's 123 to 103 us): 4096 x
+// 4096 x 4096 bf16 with bias, SiLU, residual and z 145 us = 950 TFLOP/s, without them 133 us = 1.04 PFLOP/s (a library product
+// 1.12 to 1.34); both gradient products of 4096 x 2048 x 4096 in one launch 146 us = 940, with g in two terms 261 us, 1.05 PFLOP/s of
+// matrix work; 2504 x 128 x 100000 float32 with sigmoid 672 us = 95 TFLOP/s, 1.6 TB/s (a library product: 150 TFLOP/s; here a
+// tile has four steps only, and 1 GB of results takes a sigmoid each).  By counters the matrix pipe is busy 46 % of the first
+// kernel's time, 50 % with two terms, 62 % in the float32 one, LDS is read 36 % (none of it in bank conflicts), and what is
+// staged would take 46 % of it at 64 bytes a clock and CU: no unit is at its limit.  What bounds it are the waits of a step on
+// each other and the results' way out, which the CU's other workgroup hides only partly.
 //   Tiles are numbered so that the workgroups of one XCD (blockIdx % 8) work on neighbouring tiles and find each other's
 // operands in their L2.
 // ---------------------------------------------------------------------------------------------

@@ -9,9 +9,10 @@
 // updates) its share.  Squares and sums are float64: no float32 square over- or underflows on the way, and at 4 bytes per
 // element from memory the two float64 instructions per element cost nothing.  Bound by memory: 4 bytes per element for the
 // norm, 4 + 4 more for the scaled copy, 28 for the update.
-//   Measured: the norm of 1.02 GB of float32 in 160 us (6.4 TB/s), of 52 MB of bf16 in 9.5 us (5.5 TB/s); the scaled copy of
-// those 52 MB in 19 us (5.4 TB/s); the update of 256M parameters (7.2 GB) in 1374 us (5.2 TB/s; a plain copy of 4 GB reaches 4.8
-// with cached and 6.0 with nontemporal accesses).  For a model of 3887 SNPs the launches are the time: 4 + 6 and 4 + 12 us.
+//   Measured: the norm of 1.03 GB of float32 in 164 us (6.3 TB/s), of 52 MB of bf16 in 11 us (4.6 TB/s); the scaled copy of
+// those 52 MB in 19 us (5.5 TB/s); the update of 257M parameters (7.2 GB) in 1373 us (5.2 TB/s; a plain copy of 4 GB reaches 4.8
+// with cached and 6.0 with nontemporal accesses).  A model of 3887 SNPs: 4 + 6 us for clipping, mostly launches, and 4 + 13 us
+// for the update, whose 160 chunks leave CUs without work (its 33 MB would take 7 us at the copy's rate).
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>

@@ -185,9 +185,9 @@ Kernel dense_kernel(const pvae_dense_args& a) {
     return TILE;
 }
 // The gradients: slim while what its workgroups read stays small (every value of g is formed anew for each), else large, which
-// forms g once (float32 / bf16: 100 x 600 x 600 slim 13.2 / 25.7 us, large 18.4 / 18.6; 256 x 512 x 512: 20.8 / 31.9 and
-// 20.4 / 15.8; 500 x 16 x 500: 16.5 / 21.2 and 22.0 / 18.1; 4000 x 64 x 64, where the slim kernel sums db over long columns:
-// 117 / 157 and 24.4 / 24.4)
+// forms g once (float32 / bf16, GELU, in a graph: 100 x 256 x 256 slim 8.6 / 11.0 us, large 16.4 / 18.4; 100 x 600 x 600:
+// 16.7 / 30.7 and 20.3 / 21.6; 256 x 512 x 512: 28.4 / 40.7 and 22.4 / 22.5; 32 x 512 x 4000: 45.6 / 87.4 and 20.6 / 21.4; 4000 x 64
+// x 64, where the slim kernel sums db over long columns: 190 / 226 and 26.2 / 24.6)
 Kernel bwd_kernel(const pvae_dense_bwd_args& a) {
     const int64_t dx = a.dx ? ceil_div(a.m, PVD_SM) * ceil_div(a.k, PVD_SN) : 0, dw = a.dw ? ceil_div(a.k, PVD_SM) * ceil_div(a.n, PVD_SN) : 0;
     const int64_t reads = dx * 48 * a.n + dw * 48 * a.m, most = esize(a.dtype) == 4 ? int64_t(10) << 20 : int64_t(3) << 19;
@@ -343,8 +343,8 @@ struct NtBuilder {
             }
             return plan.two ? 2 * n : n;
         };
-        // 128 x 128 with eight waves, two workgroups to a CU (4096^3 bf16 with residual and z: 147 us; 128 x 256, one workgroup to
-        // a CU, whose results nothing hides: 163; the products alone are 124 and 121).  float32 takes 64 x 64 (five to a CU)
+        // 128 x 128 with eight waves, two workgroups to a CU (4096^3 bf16 with residual and z, in long runs: 147 us; 128 x 256, one
+        // workgroup to a CU, whose results nothing hides: 163; the products alone are 124 and 121).  float32 takes 64 x 64 (five to a CU)
         // where 128 x 128 would give the CUs less than 40 steps each -- matrix work is sixteen times slower there, and an
         // uneven last round counts -- or would spend a fifth of its work on rows and columns that are not there
         // (64 x 512 x 100000: 148 us, with 64 x 64 tiles 74).
